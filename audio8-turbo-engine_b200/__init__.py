@@ -12,4 +12,7 @@ def __getattr__(name):
     if name in ("FastEngine", "PackedStack", "Scratch", "permute_qk", "rope_tables", "interleave_w13"):
         from . import engine
         return getattr(engine, name)
+    if name == "KV4Cache":
+        from . import kv4
+        return kv4.KV4Cache
     raise AttributeError(name)

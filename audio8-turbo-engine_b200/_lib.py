@@ -112,6 +112,11 @@ class A8Resample(C.Structure):
                 ("half", c_ll)]
 
 
+class A8KV4(C.Structure):
+    _fields_ = [("buf", c_void_p), ("layers", c_int), ("cache_rows", c_int), ("nkv", c_int), ("hd", c_int),
+                ("cache_len", c_int)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "a8_device_ok": (c_int, []),
@@ -128,6 +133,16 @@ SIGNATURES = {
                                      c_int, c_void_p, c_int, c_int, c_float, c_void_p, c_int, c_void_p]),
     "a8_attention_noalloc": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                                      c_int, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p, c_int, c_void_p]),
+    "a8_kv4_bytes": (c_ll, [C.POINTER(A8KV4)]),
+    "a8_kv4_store": (c_int, [C.POINTER(A8KV4), c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                             c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),
+    "a8_kv4_load": (c_int, [C.POINTER(A8KV4), c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int,
+                            c_void_p]),
+    "a8_kv4_attention_workspace": (c_int, [C.POINTER(A8KV4), c_int, c_int, c_int, C.POINTER(c_ll), C.POINTER(c_int)]),
+    "a8_kv4_attention": (c_int, [C.POINTER(A8KV4), c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int,
+                                 c_float, c_void_p, c_int, c_void_p, c_ll, c_void_p, c_int, c_void_p]),
+    "a8_kv4_prefill_attention": (c_int, [C.POINTER(A8KV4), c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_int,
+                                         c_float, c_void_p, c_int, c_void_p]),
     "a8_rmsnorm": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_float,
                            c_void_p]),
     "a8_embed_frame": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,

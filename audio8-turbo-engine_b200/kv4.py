@@ -1,0 +1,165 @@
+"""A key/value cache held in 4 bits: written with RoPE, read back, attended by decode rows and by packed prompts.
+
+A bf16 cache (the reference's, serve/fast_engine.py:105-106) spends 16 bits an element and decode attention reads all
+of it every token; here an element is a 4-bit code with one bf16 scale per 32 of them (4.5 bits). The order of calls in
+a layer is that of the bf16 path: the qkv GEMM (``a8_gemm`` with its bias epilogue), ``store`` in place of its RoPE
+epilogue, then ``attention`` for decode rows or ``prefill_attention`` for packed prompts.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib as L
+
+BF16 = torch.bfloat16
+
+
+def _need(ok, what):
+    if not ok:
+        raise L.A8Error(f"kv4: {what}")
+
+
+class KV4Cache:
+    """`layers` caches of `cache_rows` rows x `nkv` heads x `cache_len` positions x `hd` (64 or 128) on `dev`, empty.
+    `buf` (uint8) holds them all; `desc` is the A8KV4 of the C ABI. Tensors given to a call live on the cache's device;
+    kernels go to that device's current stream."""
+
+    def __init__(self, cache_rows: int, nkv: int, hd: int, cache_len: int, dev=None, layers: int = 1):
+        self.layers, self.cache_rows, self.nkv, self.hd = int(layers), int(cache_rows), int(nkv), int(hd)
+        self.cache_len = int(cache_len)
+        self.desc = L.A8KV4(None, self.layers, self.cache_rows, self.nkv, self.hd, self.cache_len)
+        n = L.load().a8_kv4_bytes(C.byref(self.desc))
+        _need(n > 0, f"unsupported shape {(layers, cache_rows, nkv, hd, cache_len)} (hd 64 or 128)")
+        self.buf = torch.zeros(n, dtype=torch.uint8, device=torch.device("cuda" if dev is None else dev))
+        self.dev = self.buf.device
+        self.desc.buf = self.buf.data_ptr()
+        self._ref = C.byref(self.desc)
+        self._ws = {}
+
+    @property
+    def nbytes(self) -> int:
+        return self.buf.numel()
+
+    # ---- argument checks (host side, nothing launched by a refused call)
+    def _rows(self, t, rows, width, what):
+        _need(t.dtype == BF16 and t.device == self.dev and t.dim() == 2 and t.shape[0] >= rows and t.shape[1] >= width
+              and t.stride(1) == 1, f"{what}: bf16 rows of at least {width} on {self.dev}, at least {rows} of them")
+        # (the row stride of a single row means nothing: torch may give it any value)
+        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+    def _ints(self, t, n, what):
+        _need(t.dtype == torch.int32 and t.device == self.dev and t.is_contiguous() and t.numel() >= n,
+              f"{what}: {n} contiguous int32 on {self.dev}")
+        return t.data_ptr()
+
+    def _call(self, name, *args):
+        _need(self.dev.type == "cuda", "the cache is not on a GPU (there is no CPU fallback)")
+        if self.dev.index == torch.cuda.current_device():
+            L.check(getattr(L.load(), name)(self._ref, *args, torch.cuda.current_stream().cuda_stream), name)
+        else:
+            with torch.cuda.device(self.dev):
+                L.check(getattr(L.load(), name)(self._ref, *args, torch.cuda.current_stream().cuda_stream), name)
+
+    # ---- the operators
+    def store(self, qkv, pos, slot=None, *, layer: int = 0, nq: int = 0, cos=None, sin=None, ring: int = 0, q=None):
+        """Rows [q | k | v] of qkv [rows, (nq + 2 nkv) hd] into positions pos (int32 [rows]; negative: padding) of cache
+        rows slot (int32, None: the row index); with cos / sin [npos, hd] q and k are rotated (rotate_half). Returns the
+        query heads [rows, nq hd]: `q` if given (it may be qkv), else a new tensor (None with nq = 0); padding rows of it
+        are not written."""
+        rows, w = pos.numel(), (nq + 2 * self.nkv) * self.hd
+        ld = self._rows(qkv, rows, w, "qkv")
+        npos = 0
+        if cos is not None:
+            _need(sin is not None and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == self.hd
+                  and cos.dtype == sin.dtype == BF16 and cos.is_contiguous() and sin.is_contiguous()
+                  and cos.device == sin.device == self.dev, f"cos, sin: two contiguous bf16 [npos, {self.hd}] tables")
+            npos = cos.shape[0]
+        else:
+            _need(sin is None, "sin without cos")
+        if nq > 0 and q is None:
+            q = torch.empty(rows, nq * self.hd, dtype=BF16, device=self.dev)
+        ldq = self._rows(q, rows, nq * self.hd, "q") if nq > 0 else 0
+        if rows:
+            self._call("a8_kv4_store", layer, qkv.data_ptr(), ld, nq, None if cos is None else cos.data_ptr(),
+                       None if sin is None else sin.data_ptr(), npos, self._ints(pos, rows, "pos"),
+                       None if slot is None else self._ints(slot, rows, "slot"), rows, ring,
+                       q.data_ptr() if nq > 0 else None, ldq)
+        return q if nq > 0 else None
+
+    def load(self, pos, slot=None, *, layer: int = 0, k=None, v=None):
+        """(k, v) bf16 [rows, nkv, hd] at positions pos of cache rows slot (None: the row index): code * scale, rounded
+        once. Given tensors are written in place; rows with a negative position are left as they are (zero in new
+        tensors only by chance)."""
+        rows = pos.numel()
+        new = lambda: torch.empty(rows, self.nkv, self.hd, dtype=BF16, device=self.dev)
+        k, v = new() if k is None else k, new() if v is None else v
+        ld = [self._heads(t, rows, n) for t, n in ((k, "k"), (v, "v"))]
+        if rows:
+            self._call("a8_kv4_load", layer, self._ints(pos, rows, "pos"),
+                       None if slot is None else self._ints(slot, rows, "slot"), rows, k.data_ptr(), ld[0],
+                       v.data_ptr(), ld[1])
+        return k, v
+
+    def _heads(self, t, rows, what):
+        _need(t.dtype == BF16 and t.device == self.dev and t.dim() == 3 and t.shape[0] >= rows
+              and t.shape[1:] == (self.nkv, self.hd) and t.stride(2) == 1
+              and (self.nkv == 1 or t.stride(1) == self.hd),
+              f"{what}: bf16 [at least {rows}, {self.nkv}, {self.hd}] on {self.dev}, heads contiguous")
+        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), self.nkv * self.hd)
+
+    def workspace(self, nq: int, rows: int, max_len: int):
+        """A workspace (partials, tickets) for `attention` calls up to these sizes; one call at a time uses it."""
+        n, t = C.c_longlong(), C.c_int()
+        L.check(L.load().a8_kv4_attention_workspace(self._ref, nq, rows, max_len, C.byref(n), C.byref(t)),
+                "a8_kv4_attention_workspace")
+        return (torch.empty(max(1, n.value), dtype=torch.float32, device=self.dev),
+                torch.zeros(max(1, t.value), dtype=torch.int32, device=self.dev))
+
+    def _workspace(self, nq, rows, max_len):
+        # Calls on one stream run one after another and share a workspace; every other stream has its own. A captured
+        # call gets one of its own inside the graph's memory (cleared by the graph): replays of two graphs may overlap.
+        if torch.cuda.is_current_stream_capturing():
+            return self.workspace(nq, rows, max_len)
+        key = torch.cuda.current_stream(self.dev).cuda_stream
+        have = self._ws.get(key)
+        if have is None or nq > have[0] or rows > have[1] or max_len > have[2]:
+            if have is not None:
+                nq, rows, max_len = max(nq, have[0]), max(rows, have[1]), max(max_len, have[2])
+            with torch.cuda.device(self.dev):
+                have = self._ws[key] = (nq, rows, max_len, *self.workspace(nq, rows, max_len))
+        return have[3:]
+
+    def attention(self, q, lens, rowmap=None, *, layer: int = 0, max_len: int = 0, scale: float = 0.0, out=None, ws=None):
+        """Decode attention: q bf16 [rows, nq hd], row r over keys [0, min(lens[r], max_len)) of cache row rowmap[r]
+        (None: r); an empty row gives zeros. max_len bounds every row's keys (0: cache_len). Returns bf16 [rows, nq hd].
+        ws: a `workspace()` of the caller's (None: the stream's own)."""
+        rows, nq = q.shape[0], q.shape[1] // self.hd
+        _need(q.shape[1] % self.hd == 0, f"q: heads of {self.hd}")
+        max_len = max_len or self.cache_len
+        if out is None:
+            out = torch.empty(rows, nq * self.hd, dtype=BF16, device=self.dev)
+        ldq, ldo = self._rows(q, rows, nq * self.hd, "q"), self._rows(out, rows, nq * self.hd, "out")
+        lens = self._ints(lens, rows, "lens")
+        rowmap = None if rowmap is None else self._ints(rowmap, rows, "rowmap")
+        if rows:
+            w, t = ws if ws is not None else self._workspace(nq, rows, max_len)
+            self._call("a8_kv4_attention", layer, q.data_ptr(), ldq, nq, lens, rowmap, rows, max_len, float(scale),
+                       out.data_ptr(), ldo, w.data_ptr(), w.numel(), t.data_ptr(), t.numel())
+        return out
+
+    def prefill_attention(self, q, blocks, *, layer: int = 0, scale: float = 0.0, out=None):
+        """Packed causal attention: q bf16 [rows, nq hd], blocks int32 [n, 4] = (q0, n, slot, pos0) on the device (the
+        rows of `FastEngine.query_blocks`). Rows that no block covers are left as they are. Returns bf16 [rows, nq hd]."""
+        rows, nq = q.shape[0], q.shape[1] // self.hd
+        _need(q.shape[1] % self.hd == 0, f"q: heads of {self.hd}")
+        _need(blocks.dim() == 2 and blocks.shape[1] == 4, "blocks: int32 [n, 4]")
+        if out is None:
+            out = torch.empty(rows, nq * self.hd, dtype=BF16, device=self.dev)
+        ldq, ldo = self._rows(q, rows, nq * self.hd, "q"), self._rows(out, rows, nq * self.hd, "out")
+        if rows and blocks.shape[0]:
+            self._call("a8_kv4_prefill_attention", layer, q.data_ptr(), ldq, nq,
+                       self._ints(blocks, blocks.numel(), "blocks"), blocks.shape[0], rows, float(scale),
+                       out.data_ptr(), ldo)
+        return out

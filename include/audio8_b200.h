@@ -137,6 +137,58 @@ int a8_attention_noalloc(const void* q, int q_stride, const void* kc, const void
                          int nq, int nkv, int hd, int cache_len, int layer, const int* lens, const int* rowmap,
                          int rows, int max_len, float scale, void* out, int out_stride, a8_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------- 4-bit cache */
+/* A key/value cache held in 4 bits (4.5 with its scales, against 16 of a bf16 cache). No counterpart in the reference,
+ * whose caches are bf16 (serve/fast_engine.py:105-106). A head's hd dims at a position are hd codes in [-7, 7] and one
+ * bf16 scale s per 32 dims: s = bf16(max|x| / 7), code = rint(x / s) clamped (0 where s = 0), value = code * s. A group
+ * that holds an infinity or a NaN reads back as NaN. The buffer holds records of 16 positions, [layers][cache rows]
+ * [nkv][ceil(cache_len / 16)], 18 hd bytes each, codes beside their scales (a position's bytes: csrc/kv4.cu); a buffer
+ * of zeros is a valid, empty cache. */
+typedef struct A8KV4 {
+  void* buf;            /* a8_kv4_bytes() bytes of device memory, 16-byte aligned */
+  int layers, cache_rows, nkv, hd, cache_len;   /* hd 64 or 128 */
+} A8KV4;
+
+/* Bytes of the buffer (buf is not looked at); -1 for an unsupported shape. */
+long long a8_kv4_bytes(const A8KV4* c);
+
+/* Write packed rows: qkv bf16 [rows, ld], row r = [q (nq heads) | k (nkv) | v (nkv)] of hd (what a8_gemm with
+ * A8_EPI_BF16 and a bias gives), at position pos[r] of cache row slot[r] (NULL: r); with ring > 0 the cache position is
+ * pos % ring. cos / sin bf16 [npos, hd] rotate_half tables (both halves alike) rotate q and k at pos in fp32, rounded once
+ * to bf16; NULL: no rotation. q_out [rows, ldq] receives the query heads (it may be qkv itself with ldq = ld); nq = 0: k
+ * and v only, q_out unused. A row with pos < 0 is padding: nothing of it is read or written. A row whose cache row,
+ * cache position or table row is out of range is not written and records ERR_BOUNDS (a8_get_error). Rows of one call that
+ * share a cache row and position leave either row's codes or scales there (finite values; give a position once). Pointers
+ * 16-byte aligned, ld and ldq multiples of 8. The counterpart of A8_EPI_ROPE for this cache. */
+int a8_kv4_store(const A8KV4* c, int layer, const void* qkv, int ld, int nq, const void* cos, const void* sin, int npos,
+                 const int* pos, const int* slot, int rows, int ring, void* q_out, int ldq, a8_stream_t stream);
+
+/* Read positions back: k[r, h, :] = bf16(code * s) of position pos[r] of cache row slot[r] (NULL: r), v likewise; bf16
+ * rows of nkv * hd at strides ldk, ldv (multiples of 8); k or v may be NULL. Rows with pos < 0 are left as they are; an
+ * out-of-range row too, and it records ERR_BOUNDS. */
+int a8_kv4_load(const A8KV4* c, int layer, const int* pos, const int* slot, int rows, void* k, int ldk, void* v, int ldv,
+                a8_stream_t stream);
+
+/* Workspace of a8_kv4_attention for calls of up to `rows` rows with at most max_len keys each. */
+int a8_kv4_attention_workspace(const A8KV4* c, int nq, int rows, int max_len, long long* ws_floats, int* n_counters);
+
+/* a8_attention over the 4-bit cache, one query token a row: out[r, h, :] = softmax(scale q[r, h] . K[:L_r]) V[:L_r] over
+ * cache row rowmap[r] (NULL: r), kv head h / (nq / nkv), L_r = min(lens[r], max_len). q / out bf16 [rows, stride] (16-byte
+ * aligned, strides multiples of 8), nq / nkv from 1 to 16. L_r <= 0 gives zeros. A row whose cache row is out of range
+ * gives zeros and records ERR_BOUNDS. scale <= 0: hd^-0.5. counters: n_counters ints, zero before the first call (a call
+ * leaves them zero); ws and counters belong to one call at a time. The order of every sum depends only on the lens of the
+ * call, so equal calls give equal bits. */
+int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* lens, const int* rowmap,
+                     int rows, int max_len, float scale, void* out, int out_stride, float* ws, long long ws_floats,
+                     int* counters, int n_counters, a8_stream_t stream);
+
+/* a8_prefill_attention over the 4-bit cache: blocks int32 [nblocks][4] = (q0, n, slot, pos0) as there (n <= 64; rows
+ * q0 .. q0 + n - 1 at positions pos0 .. of cache row slot, each attending keys [0, its position], stored beforehand); a
+ * block with n <= 0 is skipped and rows of out that no block covers are left as they are. A block whose rows, cache row or
+ * positions are out of range writes nothing and records ERR_BOUNDS. hd 64 or 128, nq / nkv from 1 to 16. */
+int a8_kv4_prefill_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* blocks,
+                             int nblocks, int rows, float scale, void* out, int out_stride, a8_stream_t stream);
+
 /* ---------------------------------------------------------------------------------------------- row kernels */
 /* y = bf16(w * bf16(h * rsqrt(mean(h^2) + eps))), h = bf16(x + res) stored back into res (res may be NULL: h = x).
  * N <= 1024, a multiple of 8. Replaces rmsnorm (serve/fast_kernels.py:30-69). */

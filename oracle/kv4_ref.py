@@ -1,0 +1,50 @@
+"""The 4-bit key/value cache and its attention in 64 bits (test infrastructure): the definition in include/audio8_b200.h
+written with plain torch operations."""
+from __future__ import annotations
+
+import torch
+
+BF = torch.bfloat16
+GROUP = 32
+
+
+def rotate(x, cos, sin):
+    """rotate_half of heads x [rows, heads, hd] (bf16 values) by table rows [rows, hd]: an fp32 sum of exact products,
+    rounded to bf16. float64 in and out."""
+    h = x.shape[-1] // 2
+    a, b, c, s = x[..., :h].double(), x[..., h:].double(), cos[:, None, :h].double(), sin[:, None, :h].double()
+    return torch.cat([a * c - b * s, b * c + a * s], -1).float().to(BF).double()
+
+
+def quantise(x):
+    """(codes, scales) float64 of bf16-valued x [..., hd]; a group with an inf or NaN has scale NaN, codes 0."""
+    g = x.double().unflatten(-1, (-1, GROUP))
+    ok = torch.isfinite(g).all(-1)
+    g = torch.where(ok[..., None], g, torch.zeros_like(g))
+    s = (g.abs().amax(-1) / 7).float().to(BF).double()
+    c = torch.where(s[..., None] > 0, torch.round(g / s.clamp(min=1e-300)[..., None]), torch.zeros_like(g)).clamp(-7, 7)
+    return c, torch.where(ok, s, torch.full_like(s, float("nan")))
+
+
+def values(x):
+    """What the cache holds of bf16-valued x [..., hd], float64."""
+    c, s = quantise(x)
+    return (c * s[..., None]).flatten(-2)
+
+
+def attention(q, k, v, first, scale):
+    """(out, err) [m, hd] float64: row i of q [m, hd] over keys [0, first + i] of k / v [n, hd], and a bound of what a
+    kernel with fp32 sums and bf16 softmax weights may be off by. A rounding to bf16 is off by at most 2^-8 of its value:
+    one on every weight (together at most 2^-8 sum p|v| / sum p), one on the output (2^-8 |out|). An fp32 logit is off by
+    at most 2^-18 scale sum_d |q_d k_d| (a sum of at most 128 exact products, 16 at a time: fewer than 32 roundings of
+    2^-23), which moves a weight by as much of itself, in the numerator and in the sum below; the fp32 sums over keys by
+    at most n 2^-23, taken as 2^-10 (far above it at the lengths tested)."""
+    m, n = q.shape[0], k.shape[0]
+    z = q @ k.T * scale
+    far = torch.arange(n)[None, :] > first + torch.arange(m)[:, None]
+    z = z.masked_fill(far, float("-inf"))
+    p = torch.softmax(z, -1)
+    out = p @ v
+    pv = p @ v.abs()
+    logit = ((q.abs() @ k.abs().T * scale).masked_fill(far, 0).amax(-1, keepdim=True)) * 2.0 ** -18
+    return out, 2.0 ** -8 * out.abs() + (2.0 ** -8 + 2.0 ** -10 + 2 * logit) * pv + 1e-30
