@@ -219,50 +219,554 @@ __global__ void __launch_bounds__(256) k_kv4_load(const Kv4LoadArgs a) {
   }
 }
 
-// ------------------------------------------------------------------------------------------------ attention
+// ------------------------------------------------------------------------------------------------ decode attention
 struct Kv4AttnArgs {
   Kv4View c;
   const __nv_bfloat16* q;
-  int q_stride, nq;
+  int q_stride, nq, group;
   const int *lens, *rowmap;   // decode: keys of row r; cache row of row r (null: r)
   const int* blocks;          // packed prompts: [nblocks][4] = (q0, n, slot, pos0)
   int rows, max_len;
   float scale_log2;
   __nv_bfloat16* out;
   int out_stride;
+  float* ws;                  // [CTAs][2][part]: a CTA's share of the units it cuts: O [group][hd], then (max, sum) [group]
+  int part;
+  int* counters;              // [rows * nkv] tickets, zero between calls
 };
+
+constexpr int KV4_CTAS = 148;         // one a SM
+constexpr int KV4_CTA_RECS = 16;      // fewer records than CTAs x this: fewer CTAs
+constexpr float KV4_LAZY = 8.f;       // a running maximum moves when a logit passes it by 2^8
+
+template <int HD, int NT>
+struct Kv4DecSmem {
+  static constexpr int NW = HD == 128 && NT == 2 ? 8 : 16;        // warps (each holds O [hd][8 NT] in registers)
+  static constexpr int NST = NW == 8 ? 8 : HD == 128 ? 4 : 8;     // records in flight a warp
+  static constexpr int RING = NST * Kv4<HD>::REC;
+  static constexpr int PART = (8 * NT * HD + 16 * NT) * 4;        // bytes: O [8 NT][hd], (max, sum) [8 NT]
+  static constexpr int HEADP = NW * RING;                         // first partials; the last ones go into the rings
+  static constexpr int PRE = HEADP + NW * PART;                   // prefix of the rows' records by thread
+  static constexpr int META = PRE + (NW * 32 + 4) * 4;            // int [2 NW][3]: unit, its first and end record
+  static constexpr int BARS = META + 2 * NW * 3 * 4;
+  static constexpr int TOTAL = BARS + NW * NST * 8 + 16;
+  static_assert(PART <= RING && TOTAL <= 227 * 1024 && BARS % 8 == 0, "");
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Codes n of the two 16-bit halves of w as bf16: the nibble u is the low mantissa bits of 128 + u; less 136 is exact.
+template <int N>
+__device__ __forceinline__ uint32_t kv4_pair(uint32_t w) {
+  uint32_t d;
+  asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, 0x000F000F, 0x43004300, 0xEA;\n\tadd.rn.bf16x2 %0, t, %2;\n\t}"
+      : "=r"(d)
+      : "r"(w >> (4 * N)), "r"(0xC308C308u));
+  return d;
+}
+
+// Row r's keys and cache row; (0, -) for a row that attends nothing.
+__device__ __forceinline__ int kv4_row(const Kv4AttnArgs& a, int r, int& crow) {
+  crow = a.rowmap != nullptr ? a.rowmap[r] : r;
+  const int n = max(0, min(a.lens[r], a.max_len));
+  return crow >= 0 && crow < a.c.cache_rows ? n : 0;
+}
+
+// A place in the records of all units (row-major, then kv head): row r, head h, record blk of nb; len keys.
+struct Kv4Cursor {
+  int r, h, blk, nb, len;
+  const uint8_t* base;          // the unit's first record
+};
+
+template <int HD>
+__device__ __forceinline__ void kv4_cursor_unit(const Kv4AttnArgs& a, Kv4Cursor& c, int crow) {
+  c.nb = (c.len + KV4_BLK - 1) / KV4_BLK;
+  c.base = kv4_rec(a.c, Kv4<HD>::REC, crow, c.h, 0);
+}
+// On to the next unit's first record (there is one).
+template <int HD>
+__device__ __forceinline__ void kv4_cursor_next(const Kv4AttnArgs& a, Kv4Cursor& c) {
+  int crow;
+  if (++c.h == a.c.nkv) {
+    c.h = 0;
+    do {
+      ++c.r;
+      c.len = c.r < a.rows ? kv4_row(a, c.r, crow) : 1;
+    } while (c.len == 0);
+    if (c.r >= a.rows) return;
+  } else {
+    c.len = kv4_row(a, c.r, crow);
+  }
+  c.blk = 0;
+  kv4_cursor_unit<HD>(a, c, crow);
+}
+
+// The records of all rows and kv heads form one sequence; CTA b of G takes the b-th of G equal parts of it, its warps
+// equal parts of that: the work is even whatever the lengths. A warp runs through its records alone (its own ring of bulk
+// copies, no barrier with the others) and writes the units that lie wholly in its part; what it has of the unit it begins
+// and the unit it ends within goes to shared memory, where the CTA joins its warps' pieces, and units that span CTAs are
+// joined, in order, by the CTA that comes last.
+//   S = Q K^T (M: the query heads of the kv head, N: 8 keys), O^T = V^T P^T (M: 16 dims, K: 16 keys): the accumulator
+//   layout of S is the B operand of the second product. Scales: S gathers s_k(key, group) q.code per group in fp32; P is
+//   multiplied by s_v(key, group) in fp32 before its rounding to bf16.
+template <int HD, int NT>
+__global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(const Kv4AttnArgs a) {
+  using F = Kv4<HD>;
+  using SM = Kv4DecSmem<HD, NT>;
+  constexpr int NW = SM::NW, NST = SM::NST, G = F::G, NTHR = NW * 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  int* pre = reinterpret_cast<int*>(smem + SM::PRE);
+  int* meta = reinterpret_cast<int*>(smem + SM::META);
+  __shared__ int s_sum[32], s_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::BARS) + warp * NST;
+  uint8_t* ring = smem + warp * SM::RING;
+  pdl_launch();
+  if (lane == 0)
+    for (int s = 0; s < NST; ++s) mbar_init(&full[s], 1);
+  fence_mbar_init();
+  if (tid < 2 * NW) meta[3 * tid] = -1;
+  pdl_wait();
+
+  // ---- how many records every row has: a prefix by thread (rows in equal runs), and zeros into rows without keys
+  const int run = (a.rows + NTHR - 1) / NTHR;
+  int mine = 0;
+  for (int r = tid * run; r < min(a.rows, (tid + 1) * run); ++r) {
+    int crow;
+    const int n = kv4_row(a, r, crow);
+    mine += (n + KV4_BLK - 1) / KV4_BLK;
+    if (n == 0 && r % gridDim.x == blockIdx.x) {
+      if (a.lens[r] > 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_ATTN, r);
+      uint4* o = reinterpret_cast<uint4*>(a.out + (size_t)r * a.out_stride);
+      for (int i = 0; i < a.nq * HD / 8; ++i) o[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  int inc = mine;
+#pragma unroll
+  for (int k = 1; k < 32; k <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, inc, k);
+    if (lane >= k) inc += up;
+  }
+  if (lane == 31) s_sum[warp] = inc;
+  __syncthreads();
+  int below = 0, total = 0;
+  for (int w = 0; w < NW; ++w) {
+    if (w < warp) below += s_sum[w];
+    total += s_sum[w];
+  }
+  pre[tid] = below + inc - mine;
+  __syncthreads();
+  const int T = total * a.c.nkv;                       // records of all units
+  const int ctas = min((int)gridDim.x, (T + KV4_CTA_RECS - 1) / KV4_CTA_RECS);
+  if ((int)blockIdx.x >= ctas) return;
+  const int b0 = int((long long)T * blockIdx.x / ctas), b1 = int((long long)T * (blockIdx.x + 1) / ctas);
+  const int w0 = b0 + int((long long)(b1 - b0) * warp / NW), w1 = b0 + int((long long)(b1 - b0) * (warp + 1) / NW);
+  const int n = w1 - w0;
+
+  if (n > 0) {
+    // ---- where the warp's part begins
+    Kv4Cursor cc;
+    {
+      int lo = 0, hi = NTHR - 1;                       // the last thread whose rows begin at or before w0
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pre[mid] * a.c.nkv <= w0) lo = mid; else hi = mid - 1;
+      }
+      int r = lo * run, at = pre[lo] * a.c.nkv, crow = 0, len = 0;
+      for (; r < a.rows; ++r) {
+        len = kv4_row(a, r, crow);
+        const int span = (len + KV4_BLK - 1) / KV4_BLK * a.c.nkv;
+        if (at + span > w0) break;
+        at += span;
+      }
+      cc.r = r;
+      cc.len = len;
+      cc.nb = (len + KV4_BLK - 1) / KV4_BLK;
+      cc.h = (w0 - at) / cc.nb;
+      cc.blk = (w0 - at) % cc.nb;
+      kv4_cursor_unit<HD>(a, cc, crow);
+    }
+    Kv4Cursor pc = cc;
+    int issued = 0;
+    auto issue = [&](int s) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[s], F::REC);
+        bulk_load(ring + s * F::REC, pc.base + (size_t)pc.blk * F::REC, F::REC, &full[s]);
+      }
+      ++issued;
+      if (++pc.blk == pc.nb && issued < n) kv4_cursor_next<HD>(a, pc);
+    };
+    for (int s = 0; s < NST && s < n; ++s) issue(s);
+
+    uint32_t qa[G][2][2 * NT];
+    float o[NT][G][2][4], m[NT], l[NT];
+    int first = cc.blk, slot = 0, ph = 0;              // the segment's first record; its ring position
+    bool fresh = true, ok = true;
+    const int kj[2] = {4 * (g & 1) + ((g & 1) ? (g >> 1) ^ 3 : g >> 1), 8 + 4 * (g & 1) + ((g & 1) ? (g >> 1) ^ 3 : g >> 1)};
+    for (int i = 0; i < n; ++i) {
+      if (fresh) {
+        fresh = false;
+        first = cc.blk;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          m[u] = -INFINITY;
+          l[u] = 0.f;
+          const bool have = g + 8 * u < a.group;
+          const __nv_bfloat16* qr = a.q + (size_t)cc.r * a.q_stride + (cc.h * a.group + g + 8 * u) * HD + 8 * t;
+#pragma unroll
+          for (int s = 0; s < G; ++s) {
+            const int grp = (s & 1) * (G / 2) + s / 2;
+            const uint4 x = have ? *reinterpret_cast<const uint4*>(qr + 32 * grp) : make_uint4(0, 0, 0, 0);
+            // dims (n, n + 4) of the word's eight: x.x = (0, 1), x.y = (2, 3), x.z = (4, 5), x.w = (6, 7)
+            qa[s][0][u] = __byte_perm(x.x, x.z, 0x5410);
+            qa[s][0][NT + u] = __byte_perm(x.x, x.z, 0x7632);
+            qa[s][1][u] = __byte_perm(x.y, x.w, 0x5410);
+            qa[s][1][NT + u] = __byte_perm(x.y, x.w, 0x7632);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) o[u][s][k][0] = o[u][s][k][1] = o[u][s][k][2] = o[u][s][k][3] = 0.f;
+          }
+        }
+      }
+      ok = mbar_wait_all(&full[slot], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_ATTN);
+      if (!ok) break;
+      const uint8_t* rec = ring + slot * F::REC;
+      // ---- scales of this lane's four keys (i = 0..3): K and V, G each
+      uint32_t ks[4][G / 2], vs[4][G / 2];
+      if constexpr (G == 4) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint4 x = *reinterpret_cast<const uint4*>(rec + F::KS0 + t * 32 + k * 16);
+          ks[2 * k][0] = x.x; ks[2 * k][1] = x.y; ks[2 * k + 1][0] = x.z; ks[2 * k + 1][1] = x.w;
+          const uint4 y = *reinterpret_cast<const uint4*>(rec + F::VS0 + t * 32 + k * 16);
+          vs[2 * k][0] = y.x; vs[2 * k][1] = y.y; vs[2 * k + 1][0] = y.z; vs[2 * k + 1][1] = y.w;
+        }
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(rec + F::KS0 + t * 16);
+        ks[0][0] = x.x; ks[1][0] = x.y; ks[2][0] = x.z; ks[3][0] = x.w;
+        const uint4 y = *reinterpret_cast<const uint4*>(rec + F::VS0 + t * 16);
+        vs[0][0] = y.x; vs[1][0] = y.y; vs[2][0] = y.z; vs[3][0] = y.w;
+      }
+      auto sf = [](const uint32_t* w, int s) {
+        return __uint_as_float((s & 1) ? w[s >> 1] & 0xFFFF0000u : w[s >> 1] << 16);
+      };
+      // ---- S: v[u][i] of query head g + 8 u and this lane's key i
+      float v[NT][4];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) v[u][0] = v[u][1] = v[u][2] = v[u][3] = 0.f;
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        uint32_t w[G];
+        if constexpr (G == 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(rec + kj[nb] * 64 + t * 16);
+          w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(rec + kj[nb] * 32 + t * 8);
+          w[0] = x.x; w[1] = x.y;
+        }
+#pragma unroll
+        for (int s = 0; s < G; ++s) {
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t a0[4] = {qa[s][0][0], NT == 2 ? qa[s][0][1] : 0u, qa[s][0][NT], NT == 2 ? qa[s][0][2 * NT - 1] : 0u};
+          uint32_t a1[4] = {qa[s][1][0], NT == 2 ? qa[s][1][1] : 0u, qa[s][1][NT], NT == 2 ? qa[s][1][2 * NT - 1] : 0u};
+          mma_bf16(acc, a0, kv4_pair<0>(w[s]), kv4_pair<1>(w[s]));
+          mma_bf16(acc, a1, kv4_pair<2>(w[s]), kv4_pair<3>(w[s]));
+#pragma unroll
+          for (int u = 0; u < NT; ++u) {
+            v[u][2 * nb] = fmaf(sf(ks[2 * nb], s), acc[2 * u], v[u][2 * nb]);
+            v[u][2 * nb + 1] = fmaf(sf(ks[2 * nb + 1], s), acc[2 * u + 1], v[u][2 * nb + 1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[u][k] *= a.scale_log2;
+      const int left = cc.len - cc.blk * KV4_BLK;      // keys of the row from this record on
+      if (left < KV4_BLK) {
+        // past the row's end: whatever the record holds there (its scales may be NaN) counts for nothing
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (4 * k + ((k & 1) ? t ^ 3 : t) >= left) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u) v[u][k] = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < G / 2; ++s) vs[k][s] = 0u;
+          }
+        }
+      }
+      // ---- the running maximum moves only when a logit passes it by 2^8 (p stays below 2^8, the sums are fp32)
+      bool over = false;
+      float mx[NT];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        mx[u] = fmaxf(fmaxf(v[u][0], v[u][1]), fmaxf(v[u][2], v[u][3]));
+        over = over || mx[u] > m[u] + KV4_LAZY;
+      }
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 1));
+          mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 2));
+          const float nm = fmaxf(m[u], mx[u]);
+          const float al = m[u] == -INFINITY ? 0.f : ex2(m[u] - nm);
+          m[u] = nm;
+          l[u] *= al;
+          const float c0 = __shfl_sync(0xffffffffu, al, 8 * t), c1 = __shfl_sync(0xffffffffu, al, 8 * t + 4);
+#pragma unroll
+          for (int s = 0; s < G; ++s)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              o[u][s][k][0] *= c0;
+              o[u][s][k][1] *= c1;
+              o[u][s][k][2] *= c0;
+              o[u][s][k][3] *= c1;
+            }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[u][k] = ex2(v[u][k] - m[u]);
+          l[u] += v[u][k];
+        }
+      // ---- O^T += V^T P^T
+      uint32_t vw[4][G / 2];                           // this lane's dims (4 g .. + 3 of every group) of its four keys
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = 4 * k + ((k & 1) ? t ^ 3 : t);
+        if constexpr (G == 4) {
+          const uint2 x = *reinterpret_cast<const uint2*>(rec + F::V0 + j * 64 + ((g ^ F::vsw(j)) << 3));
+          vw[k][0] = x.x;
+          vw[k][1] = x.y;
+        } else {
+          vw[k][0] = *reinterpret_cast<const uint32_t*>(rec + F::V0 + j * 32 + g * 4);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < G; ++s) {
+        const uint32_t u01 = __byte_perm(vw[0][s >> 1], vw[1][s >> 1], (s & 1) ? 0x7632 : 0x5410);
+        const uint32_t u23 = __byte_perm(vw[2][s >> 1], vw[3][s >> 1], (s & 1) ? 0x7632 : 0x5410);
+        uint32_t b[NT][2];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          b[u][0] = pack_bf16(v[u][0] * sf(vs[0], s), v[u][1] * sf(vs[1], s));
+          b[u][1] = pack_bf16(v[u][2] * sf(vs[2], s), v[u][3] * sf(vs[3], s));
+        }
+        const uint32_t lo[4] = {kv4_pair<0>(u01), kv4_pair<1>(u01), kv4_pair<0>(u23), kv4_pair<1>(u23)};
+        const uint32_t hi[4] = {kv4_pair<2>(u01), kv4_pair<3>(u01), kv4_pair<2>(u23), kv4_pair<3>(u23)};
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          mma_bf16(o[u][s][0], lo, b[u][0], b[u][1]);
+          mma_bf16(o[u][s][1], hi, b[u][0], b[u][1]);
+        }
+      }
+      __syncwarp();
+      if (issued < n) issue(slot);
+      if (++slot == NST) {
+        slot = 0;
+        ph ^= 1;
+      }
+      // ---- the unit or the warp's part ends here
+      ++cc.blk;
+      if (cc.blk == cc.nb || i == n - 1) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+          l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+        }
+        const bool whole = first == 0 && cc.blk == cc.nb;
+        const int head = i + 1 == cc.blk - first ? 0 : 1;              // the warp's first segment, or a later one
+        float* part = reinterpret_cast<float*>(head == 0 ? smem + SM::HEADP + warp * SM::PART : ring);
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          const float l0 = __shfl_sync(0xffffffffu, l[u], 8 * t), l1 = __shfl_sync(0xffffffffu, l[u], 8 * t + 4);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int qh = 2 * t + e + 8 * u;
+            if (qh >= a.group) continue;
+            const float inv = 1.f / (e ? l1 : l0);
+#pragma unroll
+            for (int s = 0; s < G; ++s) {
+              const int d = 32 * ((s & 1) * (G / 2) + s / 2) + 4 * g;
+              const float4 x = make_float4(o[u][s][0][e], o[u][s][0][2 + e], o[u][s][1][e], o[u][s][1][2 + e]);
+              if (whole)
+                *reinterpret_cast<uint2*>(a.out + (size_t)cc.r * a.out_stride + (cc.h * a.group + qh) * HD + d) =
+                    make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+              else
+                *reinterpret_cast<float4*>(part + qh * HD + d) = x;
+            }
+          }
+          if (!whole && t == 0) {
+            part[8 * NT * HD + 2 * (g + 8 * u)] = m[u];
+            part[8 * NT * HD + 2 * (g + 8 * u) + 1] = l[u];
+          }
+        }
+        if (!whole && lane == 0) {
+          int* e = meta + 3 * (2 * warp + head);
+          e[0] = cc.r * a.c.nkv + cc.h;
+          e[1] = w0 + i + 1 - cc.blk;                  // the unit's first record, and its end
+          e[2] = e[1] + cc.nb;
+        }
+        if (cc.blk == cc.nb && i + 1 < n) kv4_cursor_next<HD>(a, cc);
+        fresh = true;
+      }
+    }
+    if (!ok)                                           // a copy did not arrive: wait (bounded) for what is in flight
+      for (int s = 0; s < NST; ++s) mbar_wait_all(&full[s], ph ^ (s < slot), ERR_TIMEOUT_FULL, KERNEL_ID_KV4_ATTN);
+  }
+  __syncthreads();
+
+  // ---- join the warps' pieces of each unit, in key order
+  const int nel = a.group * HD / 4;                    // float4 elements of a unit
+  int cut[2] = {-1, -1}, cut0[2], cut1[2], ncut = 0;   // units that other CTAs share
+  for (int e = 0; e < 2 * NW;) {
+    const int u = meta[3 * e];
+    if (u < 0) {
+      ++e;
+      continue;
+    }
+    const int us = meta[3 * e + 1], ue = meta[3 * e + 2];
+    int e1 = e + 1;
+    while (e1 < 2 * NW && (meta[3 * e1] == u || meta[3 * e1] < 0)) ++e1;
+    const bool mineall = us >= b0 && ue <= b1;
+    float* dst = a.ws + ((size_t)blockIdx.x * 2 + (us <= b0 ? 0 : 1)) * a.part;
+    for (int idx = tid; idx < nel; idx += NTHR) {
+      const int qh = idx / (HD / 4), d4 = idx % (HD / 4);
+      float M = -INFINITY;
+      for (int k = e; k < e1; ++k)
+        if (meta[3 * k] == u) {
+          const float* p = reinterpret_cast<const float*>((k & 1) ? smem + (k >> 1) * SM::RING
+                                                                  : smem + SM::HEADP + (k >> 1) * SM::PART);
+          M = fmaxf(M, p[8 * NT * HD + 2 * qh]);
+        }
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      float L = 0.f;
+      for (int k = e; k < e1; ++k)
+        if (meta[3 * k] == u) {
+          const float* p = reinterpret_cast<const float*>((k & 1) ? smem + (k >> 1) * SM::RING
+                                                                  : smem + SM::HEADP + (k >> 1) * SM::PART);
+          const float f = ex2(p[8 * NT * HD + 2 * qh] - M);
+          const float4 y = *reinterpret_cast<const float4*>(p + qh * HD + 4 * d4);
+          x.x += f * y.x;
+          x.y += f * y.y;
+          x.z += f * y.z;
+          x.w += f * y.w;
+          L += f * p[8 * NT * HD + 2 * qh + 1];
+        }
+      if (mineall) {
+        const float inv = 1.f / L;
+        *reinterpret_cast<uint2*>(a.out + (size_t)(u / a.c.nkv) * a.out_stride + (u % a.c.nkv * a.group + qh) * HD +
+                                  4 * d4) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(dst + qh * HD + 4 * d4) = x;
+        if (d4 == 0) *reinterpret_cast<float2*>(dst + a.group * HD + 2 * qh) = make_float2(M, L);
+      }
+    }
+    if (!mineall) {
+      cut[ncut] = u;
+      cut0[ncut] = us;
+      cut1[ncut] = ue;
+      ++ncut;
+    }
+    e = e1;
+  }
+  if (ncut == 0) return;
+  __threadfence();
+  __syncthreads();
+
+  // ---- units that span CTAs: the last of their CTAs joins them, in order
+  auto cta_of = [&](int x) { return int(((long long)(x + 1) * ctas - 1) / T); };
+  float* wgt = reinterpret_cast<float*>(smem);                        // [parts][16] weights, then [16] 1 / sum
+  float* winv = wgt + KV4_CTAS * 16;
+  float4* red = reinterpret_cast<float4*>(winv + 16);                 // [splits][nel]
+  for (int k = 0; k < ncut; ++k) {
+    const int u = cut[k], us = cut0[k], c0 = cta_of(us), np = cta_of(cut1[k] - 1) - c0 + 1;
+    if (tid == 0) s_flag = atomicInc(reinterpret_cast<unsigned*>(&a.counters[u]), np - 1) == unsigned(np - 1);
+    __syncthreads();
+    const bool last = s_flag != 0;
+    __syncthreads();
+    if (!last) continue;
+    __threadfence();
+    auto src = [&](int p) {
+      const int b = c0 + p;
+      return a.ws + ((size_t)b * 2 + (us <= int((long long)T * b / ctas) ? 0 : 1)) * a.part;
+    };
+    for (int qh = warp; qh < a.group; qh += NW) {
+      float M = -INFINITY, L = 0.f;
+      for (int p = lane; p < np; p += 32) M = fmaxf(M, __ldcg(src(p) + a.group * HD + 2 * qh));
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+      for (int p = lane; p < np; p += 32) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(src(p) + a.group * HD + 2 * qh));
+        const float f = ex2(ml.x - M);
+        wgt[p * 16 + qh] = f;
+        L += f * ml.y;
+      }
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+      if (lane == 0) winv[qh] = 1.f / L;
+    }
+    __syncthreads();
+    const int splits = max(1, min(NTHR / nel, np));                   // thread groups over the parts
+    const int step = NTHR / splits;
+    for (int idx = tid; idx < (nel > NTHR ? nel : step * splits); idx += NTHR) {
+      const int sp = nel > NTHR ? 0 : idx / step, el = nel > NTHR ? idx : idx % step;
+      if (el >= nel) continue;
+      const int qh = el / (HD / 4);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int p = sp; p < np; p += splits) {
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(src(p)) + el);
+        const float f = wgt[p * 16 + qh];
+        x.x += f * y.x;
+        x.y += f * y.y;
+        x.z += f * y.z;
+        x.w += f * y.w;
+      }
+      red[sp * nel + el] = x;
+    }
+    __syncthreads();
+    for (int el = tid; el < nel; el += NTHR) {
+      const int qh = el / (HD / 4);
+      float4 x = red[el];
+      for (int sp = 1; sp < splits; ++sp) {
+        const float4 y = red[sp * nel + el];
+        x.x += y.x;
+        x.y += y.y;
+        x.z += y.z;
+        x.w += y.w;
+      }
+      const float inv = winv[qh];
+      *reinterpret_cast<uint2*>(a.out + (size_t)(u / a.c.nkv) * a.out_stride + (u % a.c.nkv * a.group + qh) * HD +
+                                4 * (el % (HD / 4))) =
+          make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+    }
+    __syncthreads();
+  }
+}
 
 // One warp a (query row, query head): a lane holds hd / 32 dims, the keys come one after another.
 template <int HD>
-__global__ void __launch_bounds__(128) k_kv4_attn_simple(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(128) k_kv4_prefill_simple(const Kv4AttnArgs a) {
   using F = Kv4<HD>;
   constexpr int D = HD / 32;
   pdl_launch();
   pdl_wait();
   const int lane = threadIdx.x & 31, head = blockIdx.y * 4 + (threadIdx.x >> 5);
   if (head >= a.nq) return;
-  int r = blockIdx.x, len, crow;
-  if (a.blocks != nullptr) {
-    const int* b = a.blocks + 4 * (blockIdx.x / 64);
-    const int i = blockIdx.x % 64;
-    if (i >= b[1]) return;
-    if (b[0] < 0 || b[1] > 64 || b[0] > a.rows - b[1] || b[2] < 0 || b[2] >= a.c.cache_rows || b[3] < 0 ||
-        b[3] > a.c.cache_len - b[1]) {
-      if (i == 0 && lane == 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_ATTN, blockIdx.x / 64);
-      return;
-    }
-    r = b[0] + i;
-    crow = b[2];
-    len = b[3] + i + 1;
-  } else {
-    len = a.lens[r];
-    crow = a.rowmap != nullptr ? a.rowmap[r] : r;
+  const int* b = a.blocks + 4 * (blockIdx.x / 64);
+  const int i = blockIdx.x % 64;
+  if (i >= b[1]) return;
+  if (b[0] < 0 || b[1] > 64 || b[0] > a.rows - b[1] || b[2] < 0 || b[2] >= a.c.cache_rows || b[3] < 0 ||
+      b[3] > a.c.cache_len - b[1]) {
+    if (i == 0 && lane == 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_ATTN, blockIdx.x / 64);
+    return;
   }
-  len = max(0, min(len, a.max_len));
-  if (crow < 0 || crow >= a.c.cache_rows) {
-    if (lane == 0 && head == 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_ATTN, r);
-    len = 0;
-  }
+  const int r = b[0] + i, crow = b[2], len = b[3] + i + 1;
   const int h = head / (a.nq / a.c.nkv);
   float q[D], o[D], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -308,6 +812,16 @@ static cudaError_t kv4_launch(const void* fn, dim3 grid, int threads, size_t sme
   cfg.numAttrs = 1;
   ++g_launches;
   return cudaLaunchKernelExC(&cfg, fn, args);
+}
+
+// Dynamic shared memory above 48 KB is a kernel's attribute on each device: set once a device (bit of `ready`).
+static bool kv4_smem_ready(std::atomic<uint64_t>& ready, const void* fn, int bytes) {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (ready.load(std::memory_order_relaxed) >> dev & 1) return true;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return true;
 }
 
 static bool kv4_shape_ok(const A8KV4* c) {
@@ -416,6 +930,7 @@ static int kv4_attn_args(Kv4AttnArgs* a, const A8KV4* c, int layer, const void* 
   a->q = reinterpret_cast<const __nv_bfloat16*>(q);
   a->q_stride = q_stride;
   a->nq = nq;
+  a->group = nq / c->nkv;
   a->rows = rows;
   a->max_len = c->cache_len;
   a->scale_log2 = (scale > 0 ? scale : 1.0f / sqrtf((float)c->hd)) * 1.4426950408889634f;
@@ -424,14 +939,31 @@ static int kv4_attn_args(Kv4AttnArgs* a, const A8KV4* c, int layer, const void* 
   return A8_OK;
 }
 
+// CTAs of a decode call: one an SM, fewer when the rows cannot hold enough records.
+static int kv4_ctas(const A8KV4* c, int rows, int max_len) {
+  const long long recs = (long long)rows * c->nkv * ((max_len + KV4_BLK - 1) / KV4_BLK);
+  return (int)std::min<long long>(KV4_CTAS, (recs + KV4_CTA_RECS - 1) / KV4_CTA_RECS);
+}
+static int kv4_part(const A8KV4* c, int nq) { return (nq / c->nkv * (c->hd + 2) + 3) / 4 * 4; }
+
 extern "C" int a8_kv4_attention_workspace(const A8KV4* c, int nq, int rows, int max_len, long long* ws_floats,
                                           int* n_counters) {
-  if (!kv4_shape_ok(c) || nq <= 0 || nq % c->nkv != 0 || nq / c->nkv > 16 || rows <= 0 || max_len <= 0 ||
-      max_len > c->cache_len)
+  if (!kv4_shape_ok(c) || nq <= 0 || nq % c->nkv != 0 || nq / c->nkv > 16 || rows <= 0 || rows > (1 << 24) ||
+      max_len <= 0 || max_len > c->cache_len || (long long)rows * c->nkv >= (1ll << 31))
     return A8_ERR_ARG;
-  if (ws_floats) *ws_floats = 0;
-  if (n_counters) *n_counters = 0;
+  if (ws_floats) *ws_floats = 2ll * kv4_ctas(c, rows, max_len) * kv4_part(c, nq);
+  if (n_counters) *n_counters = rows * c->nkv;
   return A8_OK;
+}
+
+template <int HD, int NT>
+static int kv4_attn_launch(Kv4AttnArgs& a, int ctas, cudaStream_t s) {
+  using SM = Kv4DecSmem<HD, NT>;
+  const void* fn = (const void*)k_kv4_attn<HD, NT>;
+  static std::atomic<uint64_t> ready{0};
+  if (!kv4_smem_ready(ready, fn, SM::TOTAL)) return A8_ERR_CUDA;
+  void* args[] = {&a};
+  return kv4_launch(fn, dim3(ctas), SM::NW * 32, SM::TOTAL, args, s) == cudaSuccess ? A8_OK : A8_ERR_CUDA;
 }
 
 extern "C" int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* lens,
@@ -441,13 +973,21 @@ extern "C" int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_
   int rc = kv4_attn_args(&a, c, layer, q, q_stride, nq, rows, scale, out, out_stride);
   if (rc) return rc;
   if (lens == nullptr || max_len <= 0 || max_len > c->cache_len) return A8_ERR_ARG;
+  // the records of all rows are counted in 32 bits
+  if (rows > (1 << 24) || (long long)rows * c->nkv * ((max_len + KV4_BLK - 1) / KV4_BLK) >= (1ll << 31)) return A8_ERR_SIZE;
+  const int ctas = kv4_ctas(c, rows, max_len);
+  a.part = kv4_part(c, nq);
+  if (ws == nullptr || ws_floats < 2ll * ctas * a.part || counters == nullptr || n_counters < (long long)rows * c->nkv)
+    return A8_ERR_SIZE;
+  if (reinterpret_cast<uintptr_t>(ws) & 15) return A8_ERR_ALIGN;
   a.lens = lens;
   a.rowmap = rowmap;
   a.max_len = max_len;
-  void* args[] = {&a};
-  return kv4_launch(c->hd == 64 ? (const void*)k_kv4_attn_simple<64> : (const void*)k_kv4_attn_simple<128>,
-                    dim3(rows, (nq + 3) / 4), 128, 0, args, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess
-             ? A8_OK : A8_ERR_CUDA;
+  a.ws = ws;
+  a.counters = counters;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a.group <= 8) return c->hd == 64 ? kv4_attn_launch<64, 1>(a, ctas, s) : kv4_attn_launch<128, 1>(a, ctas, s);
+  return c->hd == 64 ? kv4_attn_launch<64, 2>(a, ctas, s) : kv4_attn_launch<128, 2>(a, ctas, s);
 }
 
 extern "C" int a8_kv4_prefill_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq,
@@ -459,7 +999,7 @@ extern "C" int a8_kv4_prefill_attention(const A8KV4* c, int layer, const void* q
   if (blocks == nullptr || nblocks <= 0 || nblocks > (1 << 24)) return A8_ERR_ARG;
   a.blocks = blocks;
   void* args[] = {&a};
-  return kv4_launch(c->hd == 64 ? (const void*)k_kv4_attn_simple<64> : (const void*)k_kv4_attn_simple<128>,
+  return kv4_launch(c->hd == 64 ? (const void*)k_kv4_prefill_simple<64> : (const void*)k_kv4_prefill_simple<128>,
                     dim3(nblocks * 64, (nq + 3) / 4), 128, 0, args, reinterpret_cast<cudaStream_t>(stream)) ==
                  cudaSuccess ? A8_OK : A8_ERR_CUDA;
 }

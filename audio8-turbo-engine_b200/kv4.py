@@ -141,11 +141,11 @@ class KV4Cache:
         if out is None:
             out = torch.empty(rows, nq * self.hd, dtype=BF16, device=self.dev)
         ldq, ldo = self._rows(q, rows, nq * self.hd, "q"), self._rows(out, rows, nq * self.hd, "out")
-        lens = self._ints(lens, rows, "lens")
-        rowmap = None if rowmap is None else self._ints(rowmap, rows, "rowmap")
+        plens = self._ints(lens, rows, "lens")           # (the tensors stay referenced until the launch)
+        pmap = None if rowmap is None else self._ints(rowmap, rows, "rowmap")
         if rows:
             w, t = ws if ws is not None else self._workspace(nq, rows, max_len)
-            self._call("a8_kv4_attention", layer, q.data_ptr(), ldq, nq, lens, rowmap, rows, max_len, float(scale),
+            self._call("a8_kv4_attention", layer, q.data_ptr(), ldq, nq, plens, pmap, rows, max_len, float(scale),
                        out.data_ptr(), ldo, w.data_ptr(), w.numel(), t.data_ptr(), t.numel())
         return out
 
