@@ -15,6 +15,9 @@
 //   V half (q, slot):  dims 32 g + 4 q .. + 3 at byte   j hd / 2 + ((q ^ sw) G + slot) 2,  sw = 4 (j >> 1 & 1) at hd 128
 //   scale (j, slot):   element (4 t + i) G + slot
 // slot orders the groups so that group g and g + G / 2 (the two dims of a RoPE pair) are neighbours: 0, 2, 1, 3 at hd 128.
+#include <atomic>
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace a8 {
@@ -236,19 +239,21 @@ struct Kv4AttnArgs {
 };
 
 constexpr int KV4_CTAS = 148;         // one a SM
-constexpr int KV4_CTA_RECS = 16;      // fewer records than CTAs x this: fewer CTAs
+constexpr int KV4_CTA_RECS = 48;      // fewer records than CTAs x this: fewer CTAs
 constexpr float KV4_LAZY = 8.f;       // a running maximum moves when a logit passes it by 2^8
 
 template <int HD, int NT>
 struct Kv4DecSmem {
-  static constexpr int NW = HD == 128 && NT == 2 ? 8 : 16;        // warps (each holds O [hd][8 NT] in registers)
-  static constexpr int NST = NW == 8 ? 8 : HD == 128 ? 4 : 8;     // records in flight a warp
+  static constexpr int NW = HD == 64 ? 16 : NT == 1 ? 12 : 8;     // warps (each holds O [hd][8 NT] in registers)
+  static constexpr int NST = NW == 12 ? 6 : 8;                    // records in flight a warp
   static constexpr int RING = NST * Kv4<HD>::REC;
   static constexpr int PART = (8 * NT * HD + 16 * NT) * 4;        // bytes: O [8 NT][hd], (max, sum) [8 NT]
   static constexpr int HEADP = NW * RING;                         // first partials; the last ones go into the rings
   static constexpr int PRE = HEADP + NW * PART;                   // prefix of the rows' records by thread
-  static constexpr int META = PRE + (NW * 32 + 4) * 4;            // int [2 NW][3]: unit, its first and end record
-  static constexpr int BARS = META + 2 * NW * 3 * 4;
+  static constexpr int META = PRE + (NW * 32 + 4) * 4;            // int [2 NW][4]: unit, its first and end record, run
+  static constexpr int RUNS = META + 2 * NW * 4 * 4;              // int [2 NW][2]: a unit's pieces [from, to)
+  static constexpr int WGT = RUNS + 2 * NW * 2 * 4;               // float [2 NW][8 NT]: a piece's weight in its unit
+  static constexpr int BARS = WGT + 2 * NW * 8 * NT * 4;
   static constexpr int TOTAL = BARS + NW * NST * 8 + 16;
   static_assert(PART <= RING && TOTAL <= 227 * 1024 && BARS % 8 == 0, "");
 };
@@ -267,6 +272,34 @@ __device__ __forceinline__ uint32_t kv4_pair(uint32_t w) {
       : "r"(w >> (4 * N)), "r"(0xC308C308u));
   return d;
 }
+// The same codes as fp16 with an offset: nibbles 0 and 2 of a half as 1024 + u, 1 and 3 as 1024 + 16 u (mask with or).
+__device__ __forceinline__ uint32_t kv4_lo16(uint32_t w) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(d) : "r"(w));
+  return d;
+}
+__device__ __forceinline__ uint32_t kv4_hi16(uint32_t w) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, 0x00F000F0, 0x64006400, 0xEA;" : "=r"(d) : "r"(w));
+  return d;
+}
+__device__ __forceinline__ void kv4_mma_bf16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+constexpr float KV4_OFF_LO = 1032.f, KV4_OFF_HI = 1152.f;   // code 0 in the two forms: 1024 + 8, 1024 + 16 x 8
+// d = a b (+ c): fp16 products of one 16-dim step
+__device__ __forceinline__ void mma_f16_first(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
 // Row r's keys and cache row; (0, -) for a row that attends nothing.
 __device__ __forceinline__ int kv4_row(const Kv4AttnArgs& a, int r, int& crow) {
@@ -278,13 +311,13 @@ __device__ __forceinline__ int kv4_row(const Kv4AttnArgs& a, int r, int& crow) {
 // A place in the records of all units (row-major, then kv head): row r, head h, record blk of nb; len keys.
 struct Kv4Cursor {
   int r, h, blk, nb, len;
-  const uint8_t* base;          // the unit's first record
+  const uint8_t* at;            // the record
 };
 
 template <int HD>
 __device__ __forceinline__ void kv4_cursor_unit(const Kv4AttnArgs& a, Kv4Cursor& c, int crow) {
   c.nb = (c.len + KV4_BLK - 1) / KV4_BLK;
-  c.base = kv4_rec(a.c, Kv4<HD>::REC, crow, c.h, 0);
+  c.at = kv4_rec(a.c, Kv4<HD>::REC, crow, c.h, c.blk);
 }
 // On to the next unit's first record (there is one).
 template <int HD>
@@ -320,7 +353,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   extern __shared__ __align__(128) uint8_t smem[];
   int* pre = reinterpret_cast<int*>(smem + SM::PRE);
   int* meta = reinterpret_cast<int*>(smem + SM::META);
-  __shared__ int s_sum[32], s_flag;
+  __shared__ int s_sum[32], s_runs, s_last[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::BARS) + warp * NST;
   uint8_t* ring = smem + warp * SM::RING;
@@ -328,7 +361,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   if (lane == 0)
     for (int s = 0; s < NST; ++s) mbar_init(&full[s], 1);
   fence_mbar_init();
-  if (tid < 2 * NW) meta[3 * tid] = -1;
+  if (tid < 2 * NW) meta[4 * tid] = -1;
   pdl_wait();
 
   // ---- how many records every row has: a prefix by thread (rows in equal runs), and zeros into rows without keys
@@ -358,11 +391,42 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     total += s_sum[w];
   }
   pre[tid] = below + inc - mine;
+  if (tid == 0) pre[NTHR] = total;
   __syncthreads();
   const int T = total * a.c.nkv;                       // records of all units
   const int ctas = min((int)gridDim.x, (T + KV4_CTA_RECS - 1) / KV4_CTA_RECS);
   if ((int)blockIdx.x >= ctas) return;
-  const int b0 = int((long long)T * blockIdx.x / ctas), b1 = int((long long)T * (blockIdx.x + 1) / ctas);
+  // the row that holds record x: its first record (at) and its records a head (nb)
+  auto locate = [&](int x, int& at, int& nb) {
+    int lo = 0, hi = NTHR - 1;                         // the last thread whose rows begin at or before x
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pre[mid] * a.c.nkv <= x) lo = mid; else hi = mid - 1;
+    }
+    int r = lo * run;
+    at = pre[lo] * a.c.nkv;
+    nb = pre[lo + 1] - pre[lo];
+    if (run > 1)
+      for (;; ++r) {
+        int crow;
+        nb = (kv4_row(a, r, crow) + KV4_BLK - 1) / KV4_BLK;
+        if (at + nb * a.c.nkv > x) break;
+        at += nb * a.c.nkv;
+      }
+    return r;
+  };
+  // where CTA b's part begins: an equal share, moved to the nearer end of a unit that is small against it (a cut unit
+  // costs a pass through global memory and a ticket, about 4 us)
+  const int share = T / ctas;
+  auto begin = [&](int b) {
+    const int x = int((long long)T * b / ctas);
+    if (b == 0 || b == ctas) return x;
+    int at, nb;
+    locate(x, at, nb);
+    const int in = (x - at) % nb;
+    return 4 * nb > share ? x : 2 * in < nb ? x - in : x - in + nb;
+  };
+  const int b0 = begin(blockIdx.x), b1 = begin(blockIdx.x + 1);
   const int w0 = b0 + int((long long)(b1 - b0) * warp / NW), w1 = b0 + int((long long)(b1 - b0) * (warp + 1) / NW);
   const int n = w1 - w0;
 
@@ -370,21 +434,9 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     // ---- where the warp's part begins
     Kv4Cursor cc;
     {
-      int lo = 0, hi = NTHR - 1;                       // the last thread whose rows begin at or before w0
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (pre[mid] * a.c.nkv <= w0) lo = mid; else hi = mid - 1;
-      }
-      int r = lo * run, at = pre[lo] * a.c.nkv, crow = 0, len = 0;
-      for (; r < a.rows; ++r) {
-        len = kv4_row(a, r, crow);
-        const int span = (len + KV4_BLK - 1) / KV4_BLK * a.c.nkv;
-        if (at + span > w0) break;
-        at += span;
-      }
-      cc.r = r;
-      cc.len = len;
-      cc.nb = (len + KV4_BLK - 1) / KV4_BLK;
+      int at, crow;
+      cc.r = locate(w0, at, cc.nb);
+      cc.len = kv4_row(a, cc.r, crow);
       cc.h = (w0 - at) / cc.nb;
       cc.blk = (w0 - at) % cc.nb;
       kv4_cursor_unit<HD>(a, cc, crow);
@@ -394,115 +446,75 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     auto issue = [&](int s) {
       if (lane == 0) {
         mbar_arrive_expect_tx(&full[s], F::REC);
-        bulk_load(ring + s * F::REC, pc.base + (size_t)pc.blk * F::REC, F::REC, &full[s]);
+        bulk_load(ring + s * F::REC, pc.at, F::REC, &full[s]);
       }
       ++issued;
+      pc.at += F::REC;
       if (++pc.blk == pc.nb && issued < n) kv4_cursor_next<HD>(a, pc);
     };
     for (int s = 0; s < NST && s < n; ++s) issue(s);
 
     uint32_t qa[G][2][2 * NT];
-    float o[NT][G][2][4], m[NT], l[NT];
-    int first = cc.blk, slot = 0, ph = 0;              // the segment's first record; its ring position
-    bool fresh = true, ok = true;
-    const int kj[2] = {4 * (g & 1) + ((g & 1) ? (g >> 1) ^ 3 : g >> 1), 8 + 4 * (g & 1) + ((g & 1) ? (g >> 1) ^ 3 : g >> 1)};
-    for (int i = 0; i < n; ++i) {
-      if (fresh) {
-        fresh = false;
-        first = cc.blk;
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          m[u] = -INFINITY;
-          l[u] = 0.f;
-          const bool have = g + 8 * u < a.group;
-          const __nv_bfloat16* qr = a.q + (size_t)cc.r * a.q_stride + (cc.h * a.group + g + 8 * u) * HD + 8 * t;
-#pragma unroll
-          for (int s = 0; s < G; ++s) {
-            const int grp = (s & 1) * (G / 2) + s / 2;
-            const uint4 x = have ? *reinterpret_cast<const uint4*>(qr + 32 * grp) : make_uint4(0, 0, 0, 0);
-            // dims (n, n + 4) of the word's eight: x.x = (0, 1), x.y = (2, 3), x.z = (4, 5), x.w = (6, 7)
-            qa[s][0][u] = __byte_perm(x.x, x.z, 0x5410);
-            qa[s][0][NT + u] = __byte_perm(x.x, x.z, 0x7632);
-            qa[s][1][u] = __byte_perm(x.y, x.w, 0x5410);
-            qa[s][1][NT + u] = __byte_perm(x.y, x.w, 0x7632);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) o[u][s][k][0] = o[u][s][k][1] = o[u][s][k][2] = o[u][s][k][3] = 0.f;
-          }
-        }
-      }
-      ok = mbar_wait_all(&full[slot], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_ATTN);
-      if (!ok) break;
-      const uint8_t* rec = ring + slot * F::REC;
-      // ---- scales of this lane's four keys (i = 0..3): K and V, G each
-      uint32_t ks[4][G / 2], vs[4][G / 2];
+    float o[NT][G][2][4], m[NT], l[NT], qs[NT], off[NT][G];
+    int slot = 0, ph = 0;                              // ring position of the next record
+    bool ok = true;
+    // this lane's places in a record: K words of its key in the first half (the second: 8 positions on), scales, and V
+    // words of its even and odd positions
+    const int kw = (4 * (g & 1) + ((g & 1) ? (g >> 1) ^ 3 : g >> 1)) * (HD / 2) + t * (4 * G);
+    const int ve = F::vhalf(t, g, 0), vo = F::vhalf(4 + (t ^ 3), g, 0), sc0 = t * (8 * G);
+    auto sf2 = [](uint32_t x, uint32_t y, int s) {     // two bf16 scales as fp32
+      return (s & 1) ? make_float2(__uint_as_float(x & 0xFFFF0000u), __uint_as_float(y & 0xFFFF0000u))
+                     : make_float2(__uint_as_float(x << 16), __uint_as_float(y << 16));
+    };
+    // S of a record: v[u][h] of query head g + 8 u and this lane's keys (2 h, 2 h + 1), in units of qs
+    auto scores = [&](const uint8_t* rec, float2 (&v)[NT][2]) {
+      uint32_t ks[4][G / 2];
       if constexpr (G == 4) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const uint4 x = *reinterpret_cast<const uint4*>(rec + F::KS0 + t * 32 + k * 16);
+          const uint4 x = *reinterpret_cast<const uint4*>(rec + sc0 + F::KS0 + k * 16);
           ks[2 * k][0] = x.x; ks[2 * k][1] = x.y; ks[2 * k + 1][0] = x.z; ks[2 * k + 1][1] = x.w;
-          const uint4 y = *reinterpret_cast<const uint4*>(rec + F::VS0 + t * 32 + k * 16);
-          vs[2 * k][0] = y.x; vs[2 * k][1] = y.y; vs[2 * k + 1][0] = y.z; vs[2 * k + 1][1] = y.w;
         }
       } else {
-        const uint4 x = *reinterpret_cast<const uint4*>(rec + F::KS0 + t * 16);
+        const uint4 x = *reinterpret_cast<const uint4*>(rec + sc0 + F::KS0);
         ks[0][0] = x.x; ks[1][0] = x.y; ks[2][0] = x.z; ks[3][0] = x.w;
-        const uint4 y = *reinterpret_cast<const uint4*>(rec + F::VS0 + t * 16);
-        vs[0][0] = y.x; vs[1][0] = y.y; vs[2][0] = y.z; vs[3][0] = y.w;
       }
-      auto sf = [](const uint32_t* w, int s) {
-        return __uint_as_float((s & 1) ? w[s >> 1] & 0xFFFF0000u : w[s >> 1] << 16);
-      };
-      // ---- S: v[u][i] of query head g + 8 u and this lane's key i
-      float v[NT][4];
-#pragma unroll
-      for (int u = 0; u < NT; ++u) v[u][0] = v[u][1] = v[u][2] = v[u][3] = 0.f;
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb) {
         uint32_t w[G];
         if constexpr (G == 4) {
-          const uint4 x = *reinterpret_cast<const uint4*>(rec + kj[nb] * 64 + t * 16);
+          const uint4 x = *reinterpret_cast<const uint4*>(rec + kw + nb * 8 * (HD / 2));
           w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
         } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(rec + kj[nb] * 32 + t * 8);
+          const uint2 x = *reinterpret_cast<const uint2*>(rec + kw + nb * 8 * (HD / 2));
           w[0] = x.x; w[1] = x.y;
         }
 #pragma unroll
         for (int s = 0; s < G; ++s) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t a0[4] = {qa[s][0][0], NT == 2 ? qa[s][0][1] : 0u, qa[s][0][NT], NT == 2 ? qa[s][0][2 * NT - 1] : 0u};
-          uint32_t a1[4] = {qa[s][1][0], NT == 2 ? qa[s][1][1] : 0u, qa[s][1][NT], NT == 2 ? qa[s][1][2 * NT - 1] : 0u};
-          mma_bf16(acc, a0, kv4_pair<0>(w[s]), kv4_pair<1>(w[s]));
-          mma_bf16(acc, a1, kv4_pair<2>(w[s]), kv4_pair<3>(w[s]));
+          float acc[4];
+          const uint32_t a0[4] = {qa[s][0][0], NT == 2 ? qa[s][0][1] : 0u, qa[s][0][NT],
+                                  NT == 2 ? qa[s][0][2 * NT - 1] : 0u};
+          const uint32_t a1[4] = {qa[s][1][0], NT == 2 ? qa[s][1][1] : 0u, qa[s][1][NT],
+                                  NT == 2 ? qa[s][1][2 * NT - 1] : 0u};
+          mma_f16_first(acc, a0, kv4_lo16(w[s]), kv4_hi16(w[s]));
+          const uint32_t w8 = w[s] >> 8;
+          mma_f16(acc, a1, kv4_lo16(w8), kv4_hi16(w8));
+          const float2 sc = sf2(ks[2 * nb][s >> 1], ks[2 * nb + 1][s >> 1], s);
 #pragma unroll
           for (int u = 0; u < NT; ++u) {
-            v[u][2 * nb] = fmaf(sf(ks[2 * nb], s), acc[2 * u], v[u][2 * nb]);
-            v[u][2 * nb + 1] = fmaf(sf(ks[2 * nb + 1], s), acc[2 * u + 1], v[u][2 * nb + 1]);
+            const float2 d = make_float2(acc[2 * u] - off[u][s], acc[2 * u + 1] - off[u][s]);
+            v[u][nb] = s == 0 ? fmul2(d, sc) : ffma2(d, sc, v[u][nb]);
           }
         }
       }
-#pragma unroll
-      for (int u = 0; u < NT; ++u)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[u][k] *= a.scale_log2;
-      const int left = cc.len - cc.blk * KV4_BLK;      // keys of the row from this record on
-      if (left < KV4_BLK) {
-        // past the row's end: whatever the record holds there (its scales may be NaN) counts for nothing
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (4 * k + ((k & 1) ? t ^ 3 : t) >= left) {
-#pragma unroll
-            for (int u = 0; u < NT; ++u) v[u][k] = -INFINITY;
-#pragma unroll
-            for (int s = 0; s < G / 2; ++s) vs[k][s] = 0u;
-          }
-        }
-      }
-      // ---- the running maximum moves only when a logit passes it by 2^8 (p stays below 2^8, the sums are fp32)
+    };
+    // the running maximum m (in logits of base 2) moves only when a logit passes it by 2^8: p stays below 2^8
+    auto raise = [&](const float2 (&v)[NT][2]) {
       bool over = false;
       float mx[NT];
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
-        mx[u] = fmaxf(fmaxf(v[u][0], v[u][1]), fmaxf(v[u][2], v[u][3]));
+        mx[u] = fmaxf(fmaxf(v[u][0].x, v[u][0].y), fmaxf(v[u][1].x, v[u][1].y)) * qs[u];
         over = over || mx[u] > m[u] + KV4_LAZY;
       }
       if (__any_sync(0xffffffffu, over)) {
@@ -526,24 +538,45 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
             }
         }
       }
+    };
+    // O^T += V^T P^T of a record; CUT: only its first `left` positions count
+    auto values = [&](auto cut, const uint8_t* rec, float2 (&v)[NT][2], int left) {
+      constexpr bool CUT = decltype(cut)::value;
 #pragma unroll
       for (int u = 0; u < NT; ++u)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[u][k] = ex2(v[u][k] - m[u]);
-          l[u] += v[u][k];
+        for (int k = 0; k < 2; ++k) {
+          v[u][k].x = ex2(fmaf(v[u][k].x, qs[u], -m[u]));
+          v[u][k].y = ex2(fmaf(v[u][k].y, qs[u], -m[u]));
+          l[u] += v[u][k].x + v[u][k].y;
         }
-      // ---- O^T += V^T P^T
-      uint32_t vw[4][G / 2];                           // this lane's dims (4 g .. + 3 of every group) of its four keys
+      uint32_t vs[4][G / 2], vw[4][G / 2];             // this lane's scales; dims 4 g .. + 3 of every group of its keys
+      if constexpr (G == 4) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint4 y = *reinterpret_cast<const uint4*>(rec + sc0 + F::VS0 + k * 16);
+          vs[2 * k][0] = y.x; vs[2 * k][1] = y.y; vs[2 * k + 1][0] = y.z; vs[2 * k + 1][1] = y.w;
+        }
+      } else {
+        const uint4 y = *reinterpret_cast<const uint4*>(rec + sc0 + F::VS0);
+        vs[0][0] = y.x; vs[1][0] = y.y; vs[2][0] = y.z; vs[3][0] = y.w;
+      }
+      if constexpr (CUT) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (4 * k + ((k & 1) ? t ^ 3 : t) >= left)
+#pragma unroll
+            for (int s = 0; s < G / 2; ++s) vs[k][s] = 0u;
+      }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int j = 4 * k + ((k & 1) ? t ^ 3 : t);
+        const uint8_t* at = rec + ((k & 1) ? vo : ve) + (k >> 1) * 8 * (HD / 2);
         if constexpr (G == 4) {
-          const uint2 x = *reinterpret_cast<const uint2*>(rec + F::V0 + j * 64 + ((g ^ F::vsw(j)) << 3));
+          const uint2 x = *reinterpret_cast<const uint2*>(at);
           vw[k][0] = x.x;
           vw[k][1] = x.y;
         } else {
-          vw[k][0] = *reinterpret_cast<const uint32_t*>(rec + F::V0 + j * 32 + g * 4);
+          vw[k][0] = *reinterpret_cast<const uint32_t*>(at);
         }
       }
 #pragma unroll
@@ -553,196 +586,298 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
         uint32_t b[NT][2];
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-          b[u][0] = pack_bf16(v[u][0] * sf(vs[0], s), v[u][1] * sf(vs[1], s));
-          b[u][1] = pack_bf16(v[u][2] * sf(vs[2], s), v[u][3] * sf(vs[3], s));
+          const float2 p0 = fmul2(v[u][0], sf2(vs[0][s >> 1], vs[1][s >> 1], s)),
+                       p1 = fmul2(v[u][1], sf2(vs[2][s >> 1], vs[3][s >> 1], s));
+          b[u][0] = pack_bf16(p0.x, p0.y);
+          b[u][1] = pack_bf16(p1.x, p1.y);
         }
         const uint32_t lo[4] = {kv4_pair<0>(u01), kv4_pair<1>(u01), kv4_pair<0>(u23), kv4_pair<1>(u23)};
         const uint32_t hi[4] = {kv4_pair<2>(u01), kv4_pair<3>(u01), kv4_pair<2>(u23), kv4_pair<3>(u23)};
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-          mma_bf16(o[u][s][0], lo, b[u][0], b[u][1]);
-          mma_bf16(o[u][s][1], hi, b[u][0], b[u][1]);
+          kv4_mma_bf16(o[u][s][0], lo, b[u][0], b[u][1]);
+          kv4_mma_bf16(o[u][s][1], hi, b[u][0], b[u][1]);
         }
       }
-      __syncwarp();
-      if (issued < n) issue(slot);
+    };
+    auto arrived = [&] { return mbar_wait_all(&full[slot], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_ATTN); };
+    auto step = [&] {
       if (++slot == NST) {
         slot = 0;
         ph ^= 1;
       }
-      // ---- the unit or the warp's part ends here
-      ++cc.blk;
-      if (cc.blk == cc.nb || i == n - 1) {
+    };
+
+    for (int i = 0; i < n && ok;) {
+      // ---- a segment: the warp's records of one unit. The query heads as fp16: scaled by a power of two so that the
+      // largest is in [2^7, 2^8) (exact down to 2^-18 of it), every other dim divided by 16 against its 16 u, and what
+      // the offsets of the codes add up to in each group
+      const int first = cc.blk, seg = min(cc.nb - cc.blk, n - i);
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-          l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+      for (int u = 0; u < NT; ++u) {
+        m[u] = -INFINITY;
+        l[u] = 0.f;
+        const bool have = g + 8 * u < a.group;
+        const __nv_bfloat16* qr = a.q + (size_t)cc.r * a.q_stride + (cc.h * a.group + g + 8 * u) * HD + 8 * t;
+        uint4 x[G];
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < G; ++s) {
+          x[s] = have ? *reinterpret_cast<const uint4*>(qr + 32 * ((s & 1) * (G / 2) + s / 2)) : make_uint4(0, 0, 0, 0);
+          const uint32_t e[4] = {x[s].x, x[s].y, x[s].z, x[s].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = max(top, max(e[k] & 0x7FFFu, (e[k] >> 16) & 0x7FFFu));
         }
-        const bool whole = first == 0 && cc.blk == cc.nb;
-        const int head = i + 1 == cc.blk - first ? 0 : 1;              // the warp's first segment, or a later one
-        float* part = reinterpret_cast<float*>(head == 0 ? smem + SM::HEADP + warp * SM::PART : ring);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t ex = max(top >> 7, 8u);
+        const float up = __uint_as_float((261u - ex) << 23);
+        qs[u] = a.scale_log2 * __uint_as_float((ex - 7u) << 23);
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          const float l0 = __shfl_sync(0xffffffffu, l[u], 8 * t), l1 = __shfl_sync(0xffffffffu, l[u], 8 * t + 4);
+        for (int s = 0; s < G; ++s) {
+          const float2 d01 = unpack_bf16(x[s].x), d23 = unpack_bf16(x[s].y), d45 = unpack_bf16(x[s].z),
+                       d67 = unpack_bf16(x[s].w);
+          // dims (n, n + 4) of the word's eight
+          qa[s][0][u] = pack_f16(d01.x * up, d45.x * up);
+          qa[s][0][NT + u] = pack_f16(d01.y * up * 0.0625f, d45.y * up * 0.0625f);
+          qa[s][1][u] = pack_f16(d23.x * up, d67.x * up);
+          qa[s][1][NT + u] = pack_f16(d23.y * up * 0.0625f, d67.y * up * 0.0625f);
+          const float2 e0 = unpack_f16(qa[s][0][u]), e1 = unpack_f16(qa[s][1][u]), h0 = unpack_f16(qa[s][0][NT + u]),
+                       h1 = unpack_f16(qa[s][1][NT + u]);
+          float f = KV4_OFF_LO * ((e0.x + e0.y) + (e1.x + e1.y)) + KV4_OFF_HI * ((h0.x + h0.y) + (h1.x + h1.y));
+          f += __shfl_xor_sync(0xffffffffu, f, 1);
+          f += __shfl_xor_sync(0xffffffffu, f, 2);
+          off[u][s] = f;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int qh = 2 * t + e + 8 * u;
-            if (qh >= a.group) continue;
-            const float inv = 1.f / (e ? l1 : l0);
-#pragma unroll
-            for (int s = 0; s < G; ++s) {
-              const int d = 32 * ((s & 1) * (G / 2) + s / 2) + 4 * g;
-              const float4 x = make_float4(o[u][s][0][e], o[u][s][0][2 + e], o[u][s][1][e], o[u][s][1][2 + e]);
-              if (whole)
-                *reinterpret_cast<uint2*>(a.out + (size_t)cc.r * a.out_stride + (cc.h * a.group + qh) * HD + d) =
-                    make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
-              else
-                *reinterpret_cast<float4*>(part + qh * HD + d) = x;
-            }
-          }
-          if (!whole && t == 0) {
-            part[8 * NT * HD + 2 * (g + 8 * u)] = m[u];
-            part[8 * NT * HD + 2 * (g + 8 * u) + 1] = l[u];
-          }
+          for (int k = 0; k < 2; ++k) o[u][s][k][0] = o[u][s][k][1] = o[u][s][k][2] = o[u][s][k][3] = 0.f;
         }
-        if (!whole && lane == 0) {
-          int* e = meta + 3 * (2 * warp + head);
-          e[0] = cc.r * a.c.nkv + cc.h;
-          e[1] = w0 + i + 1 - cc.blk;                  // the unit's first record, and its end
-          e[2] = e[1] + cc.nb;
-        }
-        if (cc.blk == cc.nb && i + 1 < n) kv4_cursor_next<HD>(a, cc);
-        fresh = true;
       }
+      // the scores of a record are formed while the values of the one before are gathered: two independent streams
+      const int left = cc.len - (first + seg - 1) * KV4_BLK;           // keys of the segment's last record
+      if (!(ok = arrived())) break;
+      const uint8_t* rec = ring + slot * F::REC;
+      float2 v[NT][2];
+      scores(rec, v);
+      int here = slot;
+      step();
+      for (int j = 1; j < seg; ++j) {
+        raise(v);
+        if (!(ok = arrived())) break;
+        const uint8_t* next = ring + slot * F::REC;
+        float2 w[NT][2];
+        scores(next, w);
+        values(std::false_type(), rec, v, KV4_BLK);
+        __syncwarp();
+        if (issued < n) issue(here);
+        here = slot;
+        step();
+        rec = next;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          v[u][0] = w[u][0];
+          v[u][1] = w[u][1];
+        }
+      }
+      if (!ok) break;
+      // past the row's end: whatever the record holds there (its scales may be NaN) counts for nothing
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (4 * k + ((k & 1) ? t ^ 3 : t) >= left)
+#pragma unroll
+          for (int u = 0; u < NT; ++u) ((k & 1) ? v[u][k >> 1].y : v[u][k >> 1].x) = -INFINITY;
+      raise(v);
+      values(std::true_type(), rec, v, left);
+      __syncwarp();
+      if (issued < n) issue(here);
+      if (!ok) break;
+      // ---- the segment's result: the unit's, or a piece of it
+      i += seg;
+      cc.blk += seg;
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+      }
+      const bool whole = seg == cc.nb;
+      const int piece = i == seg ? 0 : 1;              // the warp's first segment, or a later one (then its last)
+      float* part = reinterpret_cast<float*>(piece == 0 ? smem + SM::HEADP + warp * SM::PART : ring);
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const float l0 = __shfl_sync(0xffffffffu, l[u], 8 * t), l1 = __shfl_sync(0xffffffffu, l[u], 8 * t + 4);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int qh = 2 * t + e + 8 * u;
+          if (qh >= a.group) continue;
+          const float inv = 1.f / (e ? l1 : l0);
+#pragma unroll
+          for (int s = 0; s < G; ++s) {
+            const int d = 32 * ((s & 1) * (G / 2) + s / 2) + 4 * g;
+            const float4 x = make_float4(o[u][s][0][e], o[u][s][0][2 + e], o[u][s][1][e], o[u][s][1][2 + e]);
+            if (whole)
+              *reinterpret_cast<uint2*>(a.out + (size_t)cc.r * a.out_stride + (cc.h * a.group + qh) * HD + d) =
+                  make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+            else
+              *reinterpret_cast<float4*>(part + qh * HD + d) = x;
+          }
+        }
+        if (!whole && t == 0) {
+          part[8 * NT * HD + 2 * (g + 8 * u)] = m[u];
+          part[8 * NT * HD + 2 * (g + 8 * u) + 1] = l[u];
+        }
+      }
+      if (!whole && lane == 0) {
+        int* e = meta + 4 * (2 * warp + piece);
+        e[0] = cc.r * a.c.nkv + cc.h;
+        e[1] = w0 + i - cc.blk;                        // the unit's first record, and its end
+        e[2] = e[1] + cc.nb;
+      }
+      if (i < n) kv4_cursor_next<HD>(a, cc);
     }
     if (!ok)                                           // a copy did not arrive: wait (bounded) for what is in flight
       for (int s = 0; s < NST; ++s) mbar_wait_all(&full[s], ph ^ (s < slot), ERR_TIMEOUT_FULL, KERNEL_ID_KV4_ATTN);
   }
   __syncthreads();
 
-  // ---- join the warps' pieces of each unit, in key order
-  const int nel = a.group * HD / 4;                    // float4 elements of a unit
-  int cut[2] = {-1, -1}, cut0[2], cut1[2], ncut = 0;   // units that other CTAs share
-  for (int e = 0; e < 2 * NW;) {
-    const int u = meta[3 * e];
-    if (u < 0) {
-      ++e;
-      continue;
+  // ---- join the warps' pieces of each unit, in key order: the runs of pieces of one unit, each piece's weight
+  int* runs = reinterpret_cast<int*>(smem + SM::RUNS);
+  float* wgt = reinterpret_cast<float*>(smem + SM::WGT);
+  auto piece_at = [&](int e) {
+    return reinterpret_cast<const float*>((e & 1) ? smem + (e >> 1) * SM::RING : smem + SM::HEADP + (e >> 1) * SM::PART);
+  };
+  constexpr int ML = 8 * NT * HD;                      // (max, sum) behind a piece's O
+  if (warp == 0) {
+    const int u = lane < 2 * NW ? meta[4 * lane] : -1;
+    const uint32_t valid = __ballot_sync(0xffffffffu, u >= 0), before = (1u << lane) - 1;
+    const int prev = (valid & before) ? 31 - __clz(valid & before) : lane;
+    const int pu = __shfl_sync(0xffffffffu, u, prev);
+    const bool starts = u >= 0 && (prev == lane || pu != u);
+    const uint32_t heads = __ballot_sync(0xffffffffu, starts);
+    if (lane < 2 * NW) meta[4 * lane + 3] = __popc(heads & (before | (1u << lane))) - 1;
+    if (starts) {
+      const uint32_t later = heads & ~(before | (1u << lane));
+      runs[2 * __popc(heads & before)] = lane;
+      runs[2 * __popc(heads & before) + 1] = later ? __ffs(later) - 1 : 2 * NW;
     }
-    const int us = meta[3 * e + 1], ue = meta[3 * e + 2];
-    int e1 = e + 1;
-    while (e1 < 2 * NW && (meta[3 * e1] == u || meta[3 * e1] < 0)) ++e1;
-    const bool mineall = us >= b0 && ue <= b1;
-    float* dst = a.ws + ((size_t)blockIdx.x * 2 + (us <= b0 ? 0 : 1)) * a.part;
-    for (int idx = tid; idx < nel; idx += NTHR) {
-      const int qh = idx / (HD / 4), d4 = idx % (HD / 4);
-      float M = -INFINITY;
-      for (int k = e; k < e1; ++k)
-        if (meta[3 * k] == u) {
-          const float* p = reinterpret_cast<const float*>((k & 1) ? smem + (k >> 1) * SM::RING
-                                                                  : smem + SM::HEADP + (k >> 1) * SM::PART);
-          M = fmaxf(M, p[8 * NT * HD + 2 * qh]);
-        }
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      float L = 0.f;
-      for (int k = e; k < e1; ++k)
-        if (meta[3 * k] == u) {
-          const float* p = reinterpret_cast<const float*>((k & 1) ? smem + (k >> 1) * SM::RING
-                                                                  : smem + SM::HEADP + (k >> 1) * SM::PART);
-          const float f = ex2(p[8 * NT * HD + 2 * qh] - M);
-          const float4 y = *reinterpret_cast<const float4*>(p + qh * HD + 4 * d4);
-          x.x += f * y.x;
-          x.y += f * y.y;
-          x.z += f * y.z;
-          x.w += f * y.w;
-          L += f * p[8 * NT * HD + 2 * qh + 1];
-        }
-      if (mineall) {
-        const float inv = 1.f / L;
-        *reinterpret_cast<uint2*>(a.out + (size_t)(u / a.c.nkv) * a.out_stride + (u % a.c.nkv * a.group + qh) * HD +
-                                  4 * d4) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
-      } else {
-        *reinterpret_cast<float4*>(dst + qh * HD + 4 * d4) = x;
-        if (d4 == 0) *reinterpret_cast<float2*>(dst + a.group * HD + 2 * qh) = make_float2(M, L);
-      }
-    }
-    if (!mineall) {
-      cut[ncut] = u;
-      cut0[ncut] = us;
-      cut1[ncut] = ue;
-      ++ncut;
-    }
-    e = e1;
+    if (lane == 0) s_runs = __popc(heads);
   }
-  if (ncut == 0) return;
-  __threadfence();
   __syncthreads();
-
-  // ---- units that span CTAs: the last of their CTAs joins them, in order
-  auto cta_of = [&](int x) { return int(((long long)(x + 1) * ctas - 1) / T); };
-  float* wgt = reinterpret_cast<float*>(smem);                        // [parts][16] weights, then [16] 1 / sum
-  float* winv = wgt + KV4_CTAS * 16;
-  float4* red = reinterpret_cast<float4*>(winv + 16);                 // [splits][nel]
-  for (int k = 0; k < ncut; ++k) {
-    const int u = cut[k], us = cut0[k], c0 = cta_of(us), np = cta_of(cut1[k] - 1) - c0 + 1;
-    if (tid == 0) s_flag = atomicInc(reinterpret_cast<unsigned*>(&a.counters[u]), np - 1) == unsigned(np - 1);
-    __syncthreads();
-    const bool last = s_flag != 0;
-    __syncthreads();
-    if (!last) continue;
-    __threadfence();
-    auto src = [&](int p) {
-      const int b = c0 + p;
-      return a.ws + ((size_t)b * 2 + (us <= int((long long)T * b / ctas) ? 0 : 1)) * a.part;
-    };
-    for (int qh = warp; qh < a.group; qh += NW) {
-      float M = -INFINITY, L = 0.f;
-      for (int p = lane; p < np; p += 32) M = fmaxf(M, __ldcg(src(p) + a.group * HD + 2 * qh));
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-      for (int p = lane; p < np; p += 32) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(src(p) + a.group * HD + 2 * qh));
-        const float f = ex2(ml.x - M);
-        wgt[p * 16 + qh] = f;
-        L += f * ml.y;
-      }
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
-      if (lane == 0) winv[qh] = 1.f / L;
-    }
-    __syncthreads();
-    const int splits = max(1, min(NTHR / nel, np));                   // thread groups over the parts
-    const int step = NTHR / splits;
-    for (int idx = tid; idx < (nel > NTHR ? nel : step * splits); idx += NTHR) {
-      const int sp = nel > NTHR ? 0 : idx / step, el = nel > NTHR ? idx : idx % step;
-      if (el >= nel) continue;
-      const int qh = el / (HD / 4);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int p = sp; p < np; p += splits) {
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(src(p)) + el);
-        const float f = wgt[p * 16 + qh];
+  const int nruns = s_runs;
+  for (int i = tid; i < 2 * NW * a.group; i += NTHR) {
+    const int e = i / a.group, qh = i % a.group;
+    if (meta[4 * e] < 0) continue;
+    const int k = meta[4 * e + 3];
+    float M = -INFINITY;
+    for (int p = runs[2 * k]; p < runs[2 * k + 1]; ++p)
+      if (meta[4 * p] >= 0) M = fmaxf(M, piece_at(p)[ML + 2 * qh]);
+    wgt[e * 8 * NT + qh] = ex2(piece_at(e)[ML + 2 * qh] - M);
+  }
+  __syncthreads();
+  auto cta_of = [&](int x) { return int(((long long)(x + 1) * ctas - 1) / T); };    // by equal shares
+  const int nel = a.group * HD / 4;                    // float4 elements of a unit
+  for (int i = tid; i < nruns * nel; i += NTHR) {
+    const int k = i / nel, el = i % nel, qh = el / (HD / 4), from = runs[2 * k], to = runs[2 * k + 1];
+    const int u = meta[4 * from], us = meta[4 * from + 1], ue = meta[4 * from + 2];
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float L = 0.f, M = -INFINITY;
+    for (int e = from; e < to; ++e)
+      if (meta[4 * e] >= 0) {
+        const float f = wgt[e * 8 * NT + qh];
+        const float4 y = reinterpret_cast<const float4*>(piece_at(e))[el];
         x.x += f * y.x;
         x.y += f * y.y;
         x.z += f * y.z;
         x.w += f * y.w;
+        L += f * piece_at(e)[ML + 2 * qh + 1];
+        M = fmaxf(M, piece_at(e)[ML + 2 * qh]);
+      }
+    if (us >= b0 && ue <= b1) {
+      const float inv = 1.f / L;
+      *reinterpret_cast<uint2*>(a.out + (size_t)(u / a.c.nkv) * a.out_stride + (u % a.c.nkv * a.group) * HD + 4 * el) =
+          make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+    } else {                                           // cut: in the unit's first CTA place 1, in later ones place 0
+      float* dst = a.ws + ((size_t)blockIdx.x * 2 + (cta_of(us) == (int)blockIdx.x)) * a.part;
+      reinterpret_cast<float4*>(dst)[el] = x;
+      if (el % (HD / 4) == 0) *reinterpret_cast<float2*>(dst + a.group * HD + 2 * qh) = make_float2(M, L);
+    }
+  }
+  // only the first and the last run can belong to a unit that other CTAs share
+  int cut_from[2] = {nruns > 0 ? runs[0] : -1, nruns > 1 ? runs[2 * nruns - 2] : -1};
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (cut_from[k] >= 0 && meta[4 * cut_from[k] + 1] >= b0 && meta[4 * cut_from[k] + 2] <= b1) cut_from[k] = -1;
+  if (cut_from[0] < 0 && cut_from[1] < 0) return;
+  __threadfence();
+  __syncthreads();
+
+  // ---- units that span CTAs: the last of their CTAs joins them, in order
+  if (tid < 2) {
+    const int e = cut_from[tid];
+    s_last[tid] = 0;
+    if (e >= 0) {
+      const unsigned others = cta_of(meta[4 * e + 2] - 1) - cta_of(meta[4 * e + 1]);
+      s_last[tid] = atomicInc(reinterpret_cast<unsigned*>(&a.counters[meta[4 * e]]), others) == others;
+    }
+  }
+  __syncthreads();
+  __threadfence();
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    if (!s_last[k]) continue;
+    const int e = cut_from[k], u = meta[4 * e], c0 = cta_of(meta[4 * e + 1]), np = cta_of(meta[4 * e + 2] - 1) - c0 + 1;
+    // thread groups take every splits-th part, four loads in flight each, and join through shared memory (the rings)
+    const int splits = max(1, min(NTHR / nel, np)), step = splits > 1 ? NTHR / splits : max(nel, 1);
+    float4* red = reinterpret_cast<float4*>(smem);                    // [splits][nel], then (max, sum) [splits][nel]
+    float2* redm = reinterpret_cast<float2*>(red + splits * nel);
+    for (int i = tid; i < step * splits; i += NTHR) {
+      const int sp = i / step, el = i % step, qh = el / (HD / 4);
+      if (el >= nel) continue;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      float M = -INFINITY, L = 0.f;
+      for (int p = sp; p < np; p += 4 * splits) {
+        float2 ml[4];
+        float4 y[4];
+        float nm = M;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int pp = p + j * splits;
+          const float* src = a.ws + ((size_t)(c0 + pp) * 2 + (pp == 0)) * a.part;
+          ml[j] = pp < np ? __ldcg(reinterpret_cast<const float2*>(src + a.group * HD) + qh) : make_float2(-INFINITY, 0.f);
+          y[j] = pp < np ? __ldcg(reinterpret_cast<const float4*>(src) + el) : make_float4(0.f, 0.f, 0.f, 0.f);
+          nm = fmaxf(nm, ml[j].x);
+        }
+        const float f0 = p == sp ? 0.f : ex2(M - nm);
+        x = make_float4(x.x * f0, x.y * f0, x.z * f0, x.w * f0);
+        L *= f0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float f = p + j * splits < np ? ex2(ml[j].x - nm) : 0.f;
+          x.x += f * y[j].x;
+          x.y += f * y[j].y;
+          x.z += f * y[j].z;
+          x.w += f * y[j].w;
+          L += f * ml[j].y;
+        }
+        M = nm;
       }
       red[sp * nel + el] = x;
+      redm[sp * nel + el] = make_float2(M, L);
     }
     __syncthreads();
     for (int el = tid; el < nel; el += NTHR) {
-      const int qh = el / (HD / 4);
-      float4 x = red[el];
-      for (int sp = 1; sp < splits; ++sp) {
+      float M = -INFINITY, L = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int sp = 0; sp < splits; ++sp) M = fmaxf(M, redm[sp * nel + el].x);
+      for (int sp = 0; sp < splits; ++sp) {
+        const float f = ex2(redm[sp * nel + el].x - M);
         const float4 y = red[sp * nel + el];
-        x.x += y.x;
-        x.y += y.y;
-        x.z += y.z;
-        x.w += y.w;
+        x.x += f * y.x;
+        x.y += f * y.y;
+        x.z += f * y.z;
+        x.w += f * y.w;
+        L += f * redm[sp * nel + el].y;
       }
-      const float inv = winv[qh];
-      *reinterpret_cast<uint2*>(a.out + (size_t)(u / a.c.nkv) * a.out_stride + (u % a.c.nkv * a.group + qh) * HD +
-                                4 * (el % (HD / 4))) =
+      const float inv = 1.f / L;
+      *reinterpret_cast<uint2*>(a.out + (size_t)(u / a.c.nkv) * a.out_stride + (u % a.c.nkv * a.group) * HD + 4 * el) =
           make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
     }
     __syncthreads();

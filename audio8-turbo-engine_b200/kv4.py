@@ -35,7 +35,10 @@ class KV4Cache:
         self.buf = torch.zeros(n, dtype=torch.uint8, device=torch.device("cuda" if dev is None else dev))
         self.dev = self.buf.device
         self.desc.buf = self.buf.data_ptr()
+        if self.dev.type == "cuda" and self.dev.index is None:
+            self.dev = torch.device("cuda", torch.cuda.current_device())
         self._ref = C.byref(self.desc)
+        self._lib = L.load()
         self._ws = {}
 
     @property
@@ -44,23 +47,30 @@ class KV4Cache:
 
     # ---- argument checks (host side, nothing launched by a refused call)
     def _rows(self, t, rows, width, what):
-        _need(t.dtype == BF16 and t.device == self.dev and t.dim() == 2 and t.shape[0] >= rows and t.shape[1] >= width
-              and t.stride(1) == 1, f"{what}: bf16 rows of at least {width} on {self.dev}, at least {rows} of them")
+        shape = t.shape
+        if not (len(shape) == 2 and t.dtype is BF16 and t.device == self.dev and shape[0] >= rows and shape[1] >= width):
+            _need(False, f"{what}: bf16 rows of at least {width} on {self.dev}, at least {rows} of them")
+        ld, one = t.stride()
+        _need(one == 1, f"{what}: contiguous rows")
         # (the row stride of a single row means nothing: torch may give it any value)
-        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+        return ld if shape[0] > 1 else max(ld, shape[1])
 
     def _ints(self, t, n, what):
-        _need(t.dtype == torch.int32 and t.device == self.dev and t.is_contiguous() and t.numel() >= n,
-              f"{what}: {n} contiguous int32 on {self.dev}")
+        if not (t.dtype is torch.int32 and t.device == self.dev and t.is_contiguous() and t.numel() >= n):
+            _need(False, f"{what}: {n} contiguous int32 on {self.dev}")
         return t.data_ptr()
 
-    def _call(self, name, *args):
-        _need(self.dev.type == "cuda", "the cache is not on a GPU (there is no CPU fallback)")
-        if self.dev.index == torch.cuda.current_device():
-            L.check(getattr(L.load(), name)(self._ref, *args, torch.cuda.current_stream().cuda_stream), name)
+    def _call(self, fn, *args):
+        # (kept lean: a decode step is a few microseconds on the GPU)
+        dev = self.dev.index
+        _need(dev is not None, "the cache is not on a GPU (there is no CPU fallback)")
+        if dev == torch._C._cuda_getDevice():
+            rc = fn(self._ref, *args, torch._C._cuda_getCurrentRawStream(dev))
         else:
-            with torch.cuda.device(self.dev):
-                L.check(getattr(L.load(), name)(self._ref, *args, torch.cuda.current_stream().cuda_stream), name)
+            with torch.cuda.device(dev):
+                rc = fn(self._ref, *args, torch._C._cuda_getCurrentRawStream(dev))
+        if rc:
+            L.check(rc, fn.__name__)
 
     # ---- the operators
     def store(self, qkv, pos, slot=None, *, layer: int = 0, nq: int = 0, cos=None, sin=None, ring: int = 0, q=None):
@@ -82,7 +92,7 @@ class KV4Cache:
             q = torch.empty(rows, nq * self.hd, dtype=BF16, device=self.dev)
         ldq = self._rows(q, rows, nq * self.hd, "q") if nq > 0 else 0
         if rows:
-            self._call("a8_kv4_store", layer, qkv.data_ptr(), ld, nq, None if cos is None else cos.data_ptr(),
+            self._call(self._lib.a8_kv4_store, layer, qkv.data_ptr(), ld, nq, None if cos is None else cos.data_ptr(),
                        None if sin is None else sin.data_ptr(), npos, self._ints(pos, rows, "pos"),
                        None if slot is None else self._ints(slot, rows, "slot"), rows, ring,
                        q.data_ptr() if nq > 0 else None, ldq)
@@ -97,7 +107,7 @@ class KV4Cache:
         k, v = new() if k is None else k, new() if v is None else v
         ld = [self._heads(t, rows, n) for t, n in ((k, "k"), (v, "v"))]
         if rows:
-            self._call("a8_kv4_load", layer, self._ints(pos, rows, "pos"),
+            self._call(self._lib.a8_kv4_load, layer, self._ints(pos, rows, "pos"),
                        None if slot is None else self._ints(slot, rows, "slot"), rows, k.data_ptr(), ld[0],
                        v.data_ptr(), ld[1])
         return k, v
@@ -120,9 +130,11 @@ class KV4Cache:
     def _workspace(self, nq, rows, max_len):
         # Calls on one stream run one after another and share a workspace; every other stream has its own. A captured
         # call gets one of its own inside the graph's memory (cleared by the graph): replays of two graphs may overlap.
-        if torch.cuda.is_current_stream_capturing():
+        dev = self.dev.index
+        _need(dev is not None, "the cache is not on a GPU (there is no CPU fallback)")
+        if torch._C._cuda_isCurrentStreamCapturing():
             return self.workspace(nq, rows, max_len)
-        key = torch.cuda.current_stream(self.dev).cuda_stream
+        key = torch._C._cuda_getCurrentRawStream(dev)
         have = self._ws.get(key)
         if have is None or nq > have[0] or rows > have[1] or max_len > have[2]:
             if have is not None:
@@ -145,7 +157,7 @@ class KV4Cache:
         pmap = None if rowmap is None else self._ints(rowmap, rows, "rowmap")
         if rows:
             w, t = ws if ws is not None else self._workspace(nq, rows, max_len)
-            self._call("a8_kv4_attention", layer, q.data_ptr(), ldq, nq, plens, pmap, rows, max_len, float(scale),
+            self._call(self._lib.a8_kv4_attention, layer, q.data_ptr(), ldq, nq, plens, pmap, rows, max_len, float(scale),
                        out.data_ptr(), ldo, w.data_ptr(), w.numel(), t.data_ptr(), t.numel())
         return out
 
@@ -159,7 +171,7 @@ class KV4Cache:
             out = torch.empty(rows, nq * self.hd, dtype=BF16, device=self.dev)
         ldq, ldo = self._rows(q, rows, nq * self.hd, "q"), self._rows(out, rows, nq * self.hd, "out")
         if rows and blocks.shape[0]:
-            self._call("a8_kv4_prefill_attention", layer, q.data_ptr(), ldq, nq,
+            self._call(self._lib.a8_kv4_prefill_attention, layer, q.data_ptr(), ldq, nq,
                        self._ints(blocks, blocks.numel(), "blocks"), blocks.shape[0], rows, float(scale),
                        out.data_ptr(), ldo)
         return out
