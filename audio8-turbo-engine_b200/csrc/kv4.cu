@@ -884,55 +884,6 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   }
 }
 
-// One warp a (query row, query head): a lane holds hd / 32 dims, the keys come one after another.
-template <int HD>
-__global__ void __launch_bounds__(128) k_kv4_prefill_simple(const Kv4AttnArgs a) {
-  using F = Kv4<HD>;
-  constexpr int D = HD / 32;
-  pdl_launch();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, head = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (head >= a.nq) return;
-  const int* b = a.blocks + 4 * (blockIdx.x / 64);
-  const int i = blockIdx.x % 64;
-  if (i >= b[1]) return;
-  if (b[0] < 0 || b[1] > 64 || b[0] > a.rows - b[1] || b[2] < 0 || b[2] >= a.c.cache_rows || b[3] < 0 ||
-      b[3] > a.c.cache_len - b[1]) {
-    if (i == 0 && lane == 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_ATTN, blockIdx.x / 64);
-    return;
-  }
-  const int r = b[0] + i, crow = b[2], len = b[3] + i + 1;
-  const int h = head / (a.nq / a.c.nkv);
-  float q[D], o[D], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int d = 0; d < D; ++d) {
-    q[d] = __bfloat162float(a.q[(size_t)r * a.q_stride + head * HD + lane * D + d]) * a.scale_log2;
-    o[d] = 0.f;
-  }
-  const int dim = lane * D, grp = dim / 32, s = F::slot(grp);
-  for (int p = 0; p < len; ++p) {
-    const int j = p % KV4_BLK;
-    const uint8_t* rec = kv4_rec(a.c, F::REC, crow, h, p / KV4_BLK);
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(rec + F::kword(j, (dim % 32) / 8, s)) >> (4 * (dim % 8));
-    const uint32_t vw = *reinterpret_cast<const uint16_t*>(rec + F::vhalf(j, (dim % 32) / 4, s)) >> (4 * (dim % 4));
-    const float ks = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(rec + F::KS0 + F::scale(j, s)));
-    const float vs = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(rec + F::VS0 + F::scale(j, s)));
-    float x = 0.f;
-#pragma unroll
-    for (int d = 0; d < D; ++d) x += q[d] * (float(int((kw >> (4 * d)) & 15u) - 8) * ks);
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
-    const float n = fmaxf(m, x), al = m == -INFINITY ? 0.f : exp2f(m - n), e = exp2f(x - n);
-    m = n;
-    l = l * al + e;
-#pragma unroll
-    for (int d = 0; d < D; ++d) o[d] = o[d] * al + e * (float(int((vw >> (4 * d)) & 15u) - 8) * vs);
-  }
-#pragma unroll
-  for (int d = 0; d < D; ++d)
-    a.out[(size_t)r * a.out_stride + head * HD + dim + d] = __float2bfloat16_rn(len > 0 ? o[d] / l : 0.f);
-}
-
 // ------------------------------------------------------------------------------------------------ host
 static cudaError_t kv4_launch(const void* fn, dim3 grid, int threads, size_t smem, void** args, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
@@ -1123,18 +1074,4 @@ extern "C" int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (a.group <= 8) return c->hd == 64 ? kv4_attn_launch<64, 1>(a, ctas, s) : kv4_attn_launch<128, 1>(a, ctas, s);
   return c->hd == 64 ? kv4_attn_launch<64, 2>(a, ctas, s) : kv4_attn_launch<128, 2>(a, ctas, s);
-}
-
-extern "C" int a8_kv4_prefill_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq,
-                                        const int* blocks, int nblocks, int rows, float scale, void* out,
-                                        int out_stride, a8_stream_t stream) {
-  Kv4AttnArgs a;
-  int rc = kv4_attn_args(&a, c, layer, q, q_stride, nq, rows, scale, out, out_stride);
-  if (rc) return rc;
-  if (blocks == nullptr || nblocks <= 0 || nblocks > (1 << 24)) return A8_ERR_ARG;
-  a.blocks = blocks;
-  void* args[] = {&a};
-  return kv4_launch(c->hd == 64 ? (const void*)k_kv4_prefill_simple<64> : (const void*)k_kv4_prefill_simple<128>,
-                    dim3(nblocks * 64, (nq + 3) / 4), 128, 0, args, reinterpret_cast<cudaStream_t>(stream)) ==
-                 cudaSuccess ? A8_OK : A8_ERR_CUDA;
 }

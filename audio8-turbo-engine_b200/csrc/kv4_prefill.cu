@@ -1,0 +1,473 @@
+// Packed causal prompt attention over the 4-bit cache on the tensor cores (tcgen05).
+//
+// A query block is up to 64 consecutive positions of one request (q0, n, slot, pos0). One CTA takes a block, a kv head and
+// up to four of its query heads: two 128-row tiles (64 positions x 2 heads each) share every 64-key tile, which is
+// brought to 16 bits once.
+//   warps 0-7   softmax, one query vector a thread (its TMEM lane): tile warp / 4
+//   warps 8-11  K: codes -> fp16 [64 keys][hd], K-major, 128-byte swizzle
+//   warps 12-15 V: codes -> fp16 V^T [hd][64 keys]
+//   warp 16     bulk copies of the key tiles' records (a tile is four records, one copy)
+//   warp 17     MMA issue: S = Q K^T, O += P V
+// fp16, not bf16: code * s has 8 + 3 significant bits, so K and V are exact in fp16's 11 where bf16 would round each to 8.
+// Its narrow range is met by powers of two: a tile's K is divided by 2^ek (its largest scale in [1, 2)), which the softmax
+// multiplies back into its logit scale; V by 2^E, the largest scale met so far, which joins the running maximum's factor
+// on O when it grows; a query vector by its own largest element. P is fp16 with weights up to 2^14 (the running maximum
+// is moved only when a logit passes it by 2^8), rounded to 11 bits; sums and O in fp32.
+// Within a chunk of eight dims Q and K keep the order 0 4 1 5 2 6 3 7, in which the codes come out of their words.
+#include "common.cuh"
+
+namespace a8 {
+
+constexpr int KERNEL_ID_KV4_PREFILL = 12;
+constexpr int KV4P_SOFT = 8, KV4P_DEQ = 4;               // softmax warps; warps of each of K and V
+constexpr int KV4P_THREADS = (KV4P_SOFT + 2 * KV4P_DEQ + 2) * 32;
+constexpr int KV4P_RAW = 3;                              // raw key tiles in flight
+constexpr float KV4P_BIAS = 6.f;                         // p = 2^(x - m + 6)
+
+template <int HD>
+struct Kv4PreSmem {
+  static constexpr int Q = 0;                            // 2 tiles x HD / 64 atoms x [128 rows][128 B]
+  static constexpr int QT = HD / 64 * 16384;
+  static constexpr int K = Q + 2 * QT;                   // 2 stages x HD / 64 atoms x [64 keys][128 B]
+  static constexpr int KT = HD / 64 * 8192;
+  static constexpr int V = K + 2 * KT;                   // 2 stages x [HD rows][128 B]
+  static constexpr int VT = HD * 128;
+  static constexpr int P = V + 2 * VT;                   // 2 tiles x [128 rows][128 B]
+  static constexpr int RAW = P + 2 * 16384;
+  static constexpr int RAWT = 4 * Kv4<HD>::REC;
+  static constexpr int SCK = RAW + KV4P_RAW * RAWT;      // fp16 [64 keys][G]: K scales of the tile, divided
+  static constexpr int SCV = SCK + 64 * (HD / 32) * 2;   // fp16 [G][64 keys]
+  static constexpr int MISC = SCV + 64 * (HD / 32) * 2;  // int ek[4], ev[4], red[2][4], nanv[4]
+  static constexpr int BARS = MISC + 128;
+  static constexpr int TOTAL = BARS + 32 * 8 + 16 + 1024;
+  static constexpr uint32_t COLS = HD == 128 ? 512 : 256;     // TMEM: S0, S1 (64 each), O0, O1 (HD each)
+  static_assert(TOTAL <= 227 * 1024, "");
+};
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+      "%29,%30,%31};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
+      "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// The pairs (n, n + 4) of a word's (or of a key pair's) codes, n = 0..3, as fp16 whole numbers.
+__device__ __forceinline__ void kv4_codes_f16(uint32_t w, __half2* c) {
+  const __half2 off = __half2half2(__ushort_as_half(0xE408));                     // -1032
+  const __half2 sixteenth = __half2half2(__ushort_as_half(0x2C00)), off16 = __half2half2(__ushort_as_half(0xD480));  // 1/16, -72
+  const uint32_t w8 = w >> 8;
+  uint32_t x;
+  x = kv4_lo16(w);
+  c[0] = __hadd2(*reinterpret_cast<__half2*>(&x), off);
+  x = kv4_hi16(w);
+  c[1] = __hfma2(*reinterpret_cast<__half2*>(&x), sixteenth, off16);
+  x = kv4_lo16(w8);
+  c[2] = __hadd2(*reinterpret_cast<__half2*>(&x), off);
+  x = kv4_hi16(w8);
+  c[3] = __hfma2(*reinterpret_cast<__half2*>(&x), sixteenth, off16);
+}
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// 2^(e - 127) for a biased exponent e, and its inverse; both normal for e in [1, 253]
+__device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float(uint32_t(e) << 23); }
+__device__ __forceinline__ float pow2_biased_inv(int e) { return __uint_as_float(uint32_t(254 - e) << 23); }
+
+template <int HD>
+__global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a) {
+  using F = Kv4<HD>;
+  using SM = Kv4PreSmem<HD>;
+  constexpr int G = F::G;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  int* ek = reinterpret_cast<int*>(smem + SM::MISC);     // by tile % 4
+  int* ev = ek + 4;
+  int* red = ev + 4;                                     // [2][4] warp maxima of K / V
+  int* nanv = red + 8;                                   // [4] first position whose V group is NaN
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + SM::BARS);
+  uint64_t *raw_full = q_full + 1, *raw_free = raw_full + KV4P_RAW, *k_full = raw_free + KV4P_RAW, *k_free = k_full + 2,
+           *v_full = k_free + 2, *v_free = v_full + 2, *s_full = v_free + 2, *s_free = s_full + 2, *p_full = s_free + 2,
+           *p_free = p_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_free + 2);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_launch();
+  pdl_wait();
+  // the last blocks first: they attend the most keys of a prompt
+  const int bi = gridDim.x - 1 - blockIdx.x, kvh = blockIdx.y;
+  const int q0 = a.blocks[4 * bi], nrow = a.blocks[4 * bi + 1], crow = a.blocks[4 * bi + 2], pos0 = a.blocks[4 * bi + 3];
+  if (nrow <= 0) return;                                 // (uniform over the CTA, before any barrier)
+  if (q0 < 0 || nrow > 64 || q0 > a.rows - nrow || crow < 0 || crow >= a.c.cache_rows || pos0 < 0 ||
+      pos0 > a.c.cache_len - nrow) {
+    if (tid == 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_PREFILL, bi);
+    return;
+  }
+  const int heads = min(4, a.group - 4 * int(blockIdx.z));
+  const int head0 = kvh * a.group + 4 * blockIdx.z;
+  const int ntx = (heads + 1) / 2;                       // tiles in use
+  const int klen = pos0 + nrow, nt = (klen + 63) / 64;
+
+  if (tid == 0) {
+    mbar_init(q_full, KV4P_SOFT);
+    for (int s = 0; s < KV4P_RAW; ++s) {
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_free[s], 2 * KV4P_DEQ);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], KV4P_DEQ);
+      mbar_init(&k_free[s], 1);
+      mbar_init(&v_full[s], KV4P_DEQ);
+      mbar_init(&v_free[s], 1);
+      mbar_init(&s_full[s], 2);                          // the MMAs' completion, and the issuer itself (for ek, ev)
+      mbar_init(&s_free[s], 4);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&p_free[s], 1);
+    }
+    fence_mbar_init();
+    for (int g = 0; g < 4; ++g) nanv[g] = 0x7FFFFFFF;
+  }
+  if (warp == 17) tmem_alloc(tmem_slot, SM::COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < KV4P_SOFT) {
+    // ---- softmax: thread = query vector (head 2 x + half, position pos0 + r)
+    const int x = warp >> 2, row = (warp & 3) * 32 + lane, r = row & 63, hi = row >> 6;
+    const int head = 2 * x + hi;
+    const bool live = r < nrow && head < heads;
+    const int pos = pos0 + min(r, nrow - 1);
+    const uint32_t tS = tmem + x * 64 + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t tO = tmem + 128 + x * HD + (uint32_t((warp & 3) * 32) << 16);
+    // the query vector: fp16, divided by the power of two of its largest element
+    float qs;
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(q0 + r) * a.q_stride + (head0 + head) * HD);
+      uint32_t top = 0;
+      if (live)
+        for (int c = 0; c < HD / 8; ++c) {
+          const uint4 w = src[c];
+          const uint32_t e[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = max(top, max(e[k] & 0x7FFFu, (e[k] >> 16) & 0x7FFFu));
+        }
+      const int ex = min(max(int(top >> 7), 1), 253);
+      const float down = pow2_biased_inv(ex);
+      qs = a.scale_log2 * pow2_biased(ex);
+      uint8_t* dst = smem + SM::Q + x * SM::QT;
+      for (int c = 0; c < HD / 8; ++c) {
+        const uint4 w = live ? src[c] : make_uint4(0, 0, 0, 0);
+        const float2 d01 = unpack_bf16(w.x), d23 = unpack_bf16(w.y), d45 = unpack_bf16(w.z), d67 = unpack_bf16(w.w);
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * 16384 + sw128(row, c & 7)) =
+            make_uint4(pack_f16(d01.x * down, d45.x * down), pack_f16(d01.y * down, d45.y * down),
+                       pack_f16(d23.x * down, d67.x * down), pack_f16(d23.y * down, d67.y * down));
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    float m = -INFINITY, l = 0.f;
+    int E = 0;
+    bool ok = true;
+    for (int j = 0; x < ntx && j < nt; ++j) {
+      if (!(ok = mbar_wait_all(&s_full[x], j & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
+      tc_fence_after();
+      float sv[64];
+      tmem_ld32(tS, sv);
+      tmem_ld32(tS + 32, sv + 32);
+      const float f = qs * pow2_biased(ek[j & 3]);
+      const int Ej = ev[j & 3];
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_free[x]);
+      const int kmax = pos - 64 * j;                     // keys c <= kmax of this tile are causal for this row
+      if (__any_sync(0xffffffffu, kmax < 63)) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) sv[c] = c <= kmax ? sv[c] : -INFINITY;
+      }
+      float mx = sv[0];
+#pragma unroll
+      for (int c = 1; c < 64; ++c) mx = fmaxf(mx, sv[c]);
+      mx *= f;
+      bool waited = false;
+      if (__any_sync(0xffffffffu, mx > m + 8.f || Ej > E)) {
+        const float nm = mx > m + 8.f ? mx : m;
+        const float al = m == -INFINITY ? 0.f : ex2(m - nm);
+        l *= al;
+        m = nm;
+        if (j > 0) {
+          // O is at rest once the previous tile's product is complete: scale it in place
+          const float oa = al * (Ej > E ? pow2_biased(max(127 + E - Ej, 0)) : 1.f);
+          if (!(ok = mbar_wait_all(&p_free[x], (j - 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL))) break;
+          waited = true;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
+            float ov[32];
+            tmem_ld32(tO + c, ov);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) ov[k] *= oa;
+            tmem_st32(tO + c, ov);
+          }
+        }
+        E = max(E, Ej);
+      }
+      const float mb = KV4P_BIAS - m;
+      float ls = 0.f;
+      uint32_t pk[32];
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        const float p0 = ex2(fmaf(sv[c], f, mb)), p1 = ex2(fmaf(sv[c + 1], f, mb));
+        ls += p0 + p1;
+        pk[c >> 1] = pack_f16(p0, p1);
+      }
+      l += ls;
+      if (j > 0 && !waited &&
+          !(ok = mbar_wait_all(&p_free[x], (j - 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL)))
+        break;
+      uint8_t* prow = smem + SM::P + x * 16384;
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<uint4*>(prow + sw128(row, c)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[x]);
+    }
+    if (x < ntx && ok) {
+      ok = mbar_wait_all(&p_free[x], (nt - 1) & 1, ERR_TIMEOUT_ACCUM, KERNEL_ID_KV4_PREFILL);
+      tc_fence_after();
+      if (ok) {
+        const float inv = pow2_biased(E) / l;
+        __nv_bfloat16* dst = a.out + (size_t)(q0 + r) * a.out_stride + (head0 + head) * HD;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          float ov[32];
+          tmem_ld32(tO + c, ov);
+          const int grp = c / 32, slot = F::slot(grp);
+          const float w = nanv[slot] <= pos ? __int_as_float(0x7FFFFFFF) : inv;
+          if (live)
+#pragma unroll
+            for (int k = 0; k < 32; k += 8)
+              *reinterpret_cast<uint4*>(dst + c + k) =
+                  make_uint4(pack_bf16(ov[k] * w, ov[k + 1] * w), pack_bf16(ov[k + 2] * w, ov[k + 3] * w),
+                             pack_bf16(ov[k + 4] * w, ov[k + 5] * w), pack_bf16(ov[k + 6] * w, ov[k + 7] * w));
+        }
+      }
+    }
+  } else if (warp < KV4P_SOFT + 2 * KV4P_DEQ) {
+    // ---- codes to fp16: 128 threads for K, 128 for V
+    const bool isv = warp >= KV4P_SOFT + KV4P_DEQ;
+    const int dw = (warp - KV4P_SOFT) & 3, dt = dw * 32 + lane, bar = isv ? 2 : 1;
+    int E = 1;                                           // V: the largest exponent so far
+    for (int j = 0; j < nt; ++j) {
+      const int rs = j % KV4P_RAW, st = j & 1;
+      if (!mbar_wait_all(&raw_full[rs], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL)) break;
+      const uint8_t* raw = smem + SM::RAW + rs * SM::RAWT;
+      // the tile's scales, two threads a key: the largest exponent, then fp16 scales divided by its power of two
+      const int key = dt >> 1, half = dt & 1;            // slots half * G / 2 ..
+      const bool valid = 64 * j + key < klen;
+      uint32_t sc[G / 2];
+      {
+        const uint8_t* p = raw + (key >> 4) * F::REC + (isv ? F::VS0 : F::KS0) + F::scale(key & 15, half * (G / 2));
+        if constexpr (G == 4) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+          sc[0] = w & 0xFFFFu;
+          sc[1] = w >> 16;
+        } else {
+          sc[0] = *reinterpret_cast<const uint16_t*>(p);
+        }
+      }
+      int top = 0;
+#pragma unroll
+      for (int k = 0; k < G / 2; ++k) {
+        if (!valid) sc[k] = 0;
+        if (sc[k] >= 0x7F80u) {                          // NaN: V counts as zero here and is put back at the end
+          if (isv) {
+            atomicMin(&nanv[half * (G / 2) + k], 64 * j + key);
+            sc[k] = 0;
+          }
+        } else {
+          top = max(top, int(sc[k] >> 7));
+        }
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) red[(isv ? 4 : 0) + dw] = top;
+      named_bar_sync(bar, 128);
+      top = max(max(red[isv ? 4 : 0], red[isv ? 5 : 1]), max(red[isv ? 6 : 2], red[isv ? 7 : 3]));
+      top = min(max(top, 1), 253);
+      if (isv) E = top = max(top, E);
+      const float down = pow2_biased_inv(top);
+      __half* table = reinterpret_cast<__half*>(smem + (isv ? SM::SCV : SM::SCK));
+#pragma unroll
+      for (int k = 0; k < G / 2; ++k) {
+        const __half h = __float2half_rn(__uint_as_float(sc[k] << 16) * down);
+        table[isv ? (half * (G / 2) + k) * 64 + key : key * G + half * (G / 2) + k] = h;
+      }
+      if (dt == 0) (isv ? ev : ek)[j & 3] = top;
+      named_bar_sync(bar, 128);
+      if (!isv) {
+        if (j >= 2 && !mbar_wait_all(&k_free[st], ((j >> 1) - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL)) break;
+        uint8_t* dst = smem + SM::K + st * SM::KT;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                    // a thread: word t8 of a key, all groups
+          const int r = i * 32 + (dt >> 2), t8 = dt & 3;
+          const uint8_t* src = raw + (r >> 4) * F::REC + F::kword(r & 15, t8, 0);
+          uint32_t w[G];
+          uint2 hs;
+          if constexpr (G == 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(src);
+            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+            hs = *reinterpret_cast<const uint2*>(table + r * G);
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(src);
+            w[0] = u.x; w[1] = u.y;
+            hs.x = *reinterpret_cast<const uint32_t*>(table + r * G);
+            hs.y = 0;
+          }
+#pragma unroll
+          for (int s = 0; s < G; ++s) {
+            const int grp = (s & 1) * (G / 2) + s / 2;
+            const uint32_t hw = s < 2 ? hs.x : hs.y, hb = (s & 1) ? __byte_perm(hw, 0, 0x3232) : __byte_perm(hw, 0, 0x1010);
+            const __half2 h = *reinterpret_cast<const __half2*>(&hb);
+            __half2 c[4];
+            kv4_codes_f16(w[s], c);
+            *reinterpret_cast<uint4*>(dst + (grp >> 1) * 8192 + sw128(r, (grp & 1) * 4 + t8)) =
+                make_uint4(h2u(__hmul2(c[0], h)), h2u(__hmul2(c[1], h)), h2u(__hmul2(c[2], h)), h2u(__hmul2(c[3], h)));
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&k_full[st]);
+          mbar_arrive(&raw_free[rs]);
+        }
+      } else {
+        if (j >= 2 && !mbar_wait_all(&v_free[st], ((j >> 1) - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL)) break;
+        uint8_t* dst = smem + SM::V + st * SM::VT;
+        // a thread: dims 4 q .. + 3 of G / 2 groups, of eight keys
+        const int oct = dt & 7, q = (dt >> 3) & 7, part = dt >> 6;
+        uint32_t w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int j8 = (oct & 1) * 8 + k;
+          const uint8_t* src = raw + (oct >> 1) * F::REC + F::vhalf(j8, q, part * (G / 2));
+          w[k] = G == 4 ? *reinterpret_cast<const uint32_t*>(src) : *reinterpret_cast<const uint16_t*>(src);
+        }
+#pragma unroll
+        for (int sl = 0; sl < G / 2; ++sl) {
+          const int s = part * (G / 2) + sl, grp = (s & 1) * (G / 2) + s / 2;
+          const uint4 hs = *reinterpret_cast<const uint4*>(table + s * 64 + oct * 8);
+          const uint32_t hp[4] = {hs.x, hs.y, hs.z, hs.w};
+          uint32_t o[4][4];
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const uint32_t u = __byte_perm(w[2 * p], w[2 * p + 1], sl ? 0x7632 : 0x5410);
+            const __half2 h = *reinterpret_cast<const __half2*>(&hp[p]);
+            __half2 c[4];
+            kv4_codes_f16(u, c);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k][p] = h2u(__hmul2(c[k], h));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<uint4*>(dst + sw128(32 * grp + 4 * q + k, oct)) = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&v_full[st]);
+          mbar_arrive(&raw_free[rs]);
+        }
+      }
+    }
+  } else if (warp == 16) {
+    if (lane == 0) {
+      const uint8_t* src = kv4_rec(a.c, F::REC, crow, kvh, 0);
+      int issued = 0;
+      for (int j = 0; j < nt; ++j) {
+        const int rs = j % KV4P_RAW;
+        if (j >= KV4P_RAW && !mbar_wait(&raw_free[rs], (j / KV4P_RAW - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL))
+          break;
+        const uint32_t bytes = min(4, a.c.nblk - 4 * j) * F::REC;
+        mbar_arrive_expect_tx(&raw_full[rs], bytes);
+        bulk_load(smem + SM::RAW + rs * SM::RAWT, src + (size_t)j * 4 * F::REC, bytes, &raw_full[rs]);
+        issued = j + 1;
+      }
+      // every requested copy has landed before the CTA can finish (bounded after an error)
+      for (int j = max(0, issued - KV4P_RAW); j < issued; ++j)
+        mbar_wait(&raw_full[j % KV4P_RAW], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
+    }
+  } else {
+    if (lane == 0) {
+      const uint32_t idS = umma_idesc(128, 64, 0), idO = umma_idesc(128, HD, 0);
+      bool ok = mbar_wait(q_full, 0, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
+      for (int j = 0; ok && j <= nt; ++j) {
+        if (j < nt) {
+          if (!(ok = mbar_wait(&k_full[j & 1], (j >> 1) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
+          // (softmax reads ev too: it is written before V's own tile, so wait for that tile as well)
+          if (!(ok = mbar_wait(&v_full[j & 1], (j >> 1) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
+          for (int x = 0; ok && x < ntx; ++x) {
+            if (j > 0) ok = mbar_wait(&s_free[x], (j - 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+              umma_f16(tmem + x * 64, umma_desc_sw128(smem + SM::Q + x * SM::QT + (k >> 2) * 16384) + 2 * (k & 3),
+                       umma_desc_sw128(smem + SM::K + (j & 1) * SM::KT + (k >> 2) * 8192) + 2 * (k & 3), idS, k != 0);
+            umma_commit(&s_full[x]);
+            mbar_arrive(&s_full[x]);
+          }
+          umma_commit(&k_free[j & 1]);
+        }
+        if (ok && j > 0) {
+          const int p = j - 1;
+          for (int x = 0; ok && x < ntx; ++x) {
+            if (!(ok = mbar_wait(&p_full[x], p & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f16(tmem + 128 + x * HD, umma_desc_sw128(smem + SM::P + x * 16384) + 2 * k,
+                       umma_desc_sw128(smem + SM::V + (p & 1) * SM::VT) + 2 * k, idO, (p | k) != 0);
+            umma_commit(&p_free[x]);
+          }
+          umma_commit(&v_free[p & 1]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 17) tmem_dealloc(tmem, SM::COLS);
+}
+
+template <int HD>
+static int kv4_prefill_launch(Kv4AttnArgs& a, int nblocks, cudaStream_t s) {
+  const void* fn = (const void*)k_kv4_prefill<HD>;
+  static std::atomic<uint64_t> ready{0};
+  if (!kv4_smem_ready(ready, fn, Kv4PreSmem<HD>::TOTAL)) return A8_ERR_CUDA;
+  void* args[] = {&a};
+  return kv4_launch(fn, dim3(nblocks, a.c.nkv, (a.group + 3) / 4), KV4P_THREADS, Kv4PreSmem<HD>::TOTAL, args, s) ==
+                 cudaSuccess ? A8_OK : A8_ERR_CUDA;
+}
+
+}  // namespace a8
+
+using namespace a8;
+
+extern "C" int a8_kv4_prefill_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq,
+                                        const int* blocks, int nblocks, int rows, float scale, void* out,
+                                        int out_stride, a8_stream_t stream) {
+  Kv4AttnArgs a;
+  int rc = kv4_attn_args(&a, c, layer, q, q_stride, nq, rows, scale, out, out_stride);
+  if (rc) return rc;
+  if (blocks == nullptr || nblocks <= 0 || c->nkv > 65535) return A8_ERR_ARG;
+  a.blocks = blocks;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return c->hd == 64 ? kv4_prefill_launch<64>(a, nblocks, s) : kv4_prefill_launch<128>(a, nblocks, s);
+}
