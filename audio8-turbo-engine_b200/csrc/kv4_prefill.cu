@@ -20,8 +20,16 @@ namespace a8 {
 
 constexpr int KERNEL_ID_KV4_PREFILL = 12;
 constexpr int KV4P_SOFT = 8, KV4P_DEQ = 4;               // softmax warps; warps of each of K and V
-constexpr int KV4P_THREADS = (KV4P_SOFT + 2 * KV4P_DEQ + 2) * 32;
-constexpr int KV4P_RAW = 3;                              // raw key tiles in flight
+constexpr int KV4P_THREADS = (KV4P_SOFT + 2 * KV4P_DEQ + 4) * 32;   // five warpgroups (the last: warps 16, 17 and two idle)
+// Registers a thread after the warpgroups' redistribution: 256 x 120 + 256 x 80 + 128 x 80, all of the 640 x 96 = 61,440
+// that the block is launched with.
+#define A8_SETMAXNREG(op, n) asm volatile("setmaxnreg." op ".sync.aligned.u32 %0;" ::"n"(n))
+constexpr int KV4P_RAW = 6;                              // raw key tiles in flight
+constexpr int KV4P_VST = 3;                              // V tiles at hand
+#ifndef PO
+#define PO 0
+#endif
+constexpr int KV4P_POLY = PO;
 constexpr float KV4P_BIAS = 6.f;                         // p = 2^(x - m + 6)
 
 template <int HD>
@@ -30,17 +38,16 @@ struct Kv4PreSmem {
   static constexpr int QT = HD / 64 * 16384;
   static constexpr int K = Q + 2 * QT;                   // 2 stages x HD / 64 atoms x [64 keys][128 B]
   static constexpr int KT = HD / 64 * 8192;
-  static constexpr int V = K + 2 * KT;                   // 2 stages x [HD rows][128 B]
+  static constexpr int V = K + 2 * KT;                   // KV4P_VST stages x [HD rows][128 B]
   static constexpr int VT = HD * 128;
-  static constexpr int P = V + 2 * VT;                   // 2 tiles x [128 rows][128 B]
-  static constexpr int RAW = P + 2 * 16384;
+  static constexpr int RAW = V + KV4P_VST * VT;
   static constexpr int RAWT = 4 * Kv4<HD>::REC;
-  static constexpr int SCK = RAW + KV4P_RAW * RAWT;      // fp16 [64 keys][G]: K scales of the tile, divided
-  static constexpr int SCV = SCK + 64 * (HD / 32) * 2;   // fp16 [G][64 keys]
-  static constexpr int MISC = SCV + 64 * (HD / 32) * 2;  // int ek[4], ev[4], red[2][4], nanv[4]
-  static constexpr int BARS = MISC + 128;
+  static constexpr int SCV = RAW + KV4P_RAW * RAWT;      // fp16 [4 warps][G / 2][64 keys]: V scales of the tile, divided
+  static constexpr int MISC = SCV + 4 * 64 * (HD / 64) * 2;  // int ek[8], ev[8], nanv[4]
+  static constexpr int BARS = MISC + 96;
   static constexpr int TOTAL = BARS + 32 * 8 + 16 + 1024;
-  static constexpr uint32_t COLS = HD == 128 ? 512 : 256;     // TMEM: S0, S1 (64 each), O0, O1 (HD each)
+  static constexpr uint32_t COLS = 512;                  // TMEM: S of tile 0 and 1, two stages of 64 each (P takes
+                                                         // the first half of its S); O (HD each)
   static_assert(TOTAL <= 227 * 1024, "");
 };
 
@@ -55,6 +62,33 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
       "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// 2^x for a pair, x <= 127 (below -126 as 2^-126), on the FMA units: x = i + f, |f| <= 1/2, 2^f by a degree-4 polynomial
+// fitted here for least relative error (2.6e-6), i added to its exponent.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 magic = f2(12582912.f);                   // 1.5 x 2^23: the low bits of the sum are round(x)
+  const float2 t = fadd2(x, magic);
+  const float2 f = fsub2(x, fsub2(t, magic));
+  float2 p = ffma2(f2(0.009570068679749966f), f, f2(0.055917806923389435f));
+  p = ffma2(p, f, f2(0.240247443318367f));
+  p = ffma2(p, f, f2(0.6931218504905701f));
+  p = ffma2(p, f, f2(0.9999992847442627f));
+  return make_float2(__uint_as_float(__float_as_uint(t.x) * 0x800000u + __float_as_uint(p.x)),
+                     __uint_as_float(__float_as_uint(t.y) * 0x800000u + __float_as_uint(p.y)));
+}
+
+// D += A B with A (128 rows x 16 fp16, two a column) in tensor memory, B in shared memory
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 
 // The pairs (n, n + 4) of a word's (or of a key pair's) codes, n = 0..3, as fp16 whole numbers.
@@ -84,21 +118,20 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
   constexpr int G = F::G;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  int* ek = reinterpret_cast<int*>(smem + SM::MISC);     // by tile % 4
-  int* ev = ek + 4;
-  int* red = ev + 4;                                     // [2][4] warp maxima of K / V
-  int* nanv = red + 8;                                   // [4] first position whose V group is NaN
+  int* ek = reinterpret_cast<int*>(smem + SM::MISC);     // by tile % 8
+  int* ev = ek + 8;
+  int* nanv = ev + 8;                                    // [4] first position whose V group is NaN
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + SM::BARS);
-  uint64_t *raw_full = q_full + 1, *raw_free = raw_full + KV4P_RAW, *k_full = raw_free + KV4P_RAW, *k_free = k_full + 2,
-           *v_full = k_free + 2, *v_free = v_full + 2, *s_full = v_free + 2, *s_free = s_full + 2, *p_full = s_free + 2,
-           *p_free = p_full + 2;
+  uint64_t *raw_full = q_full + 1, *raw_free = raw_full + KV4P_RAW, *kv_full = raw_free + KV4P_RAW, *k_free = kv_full + 4,
+           *v_free = k_free + 2, *s_full = v_free + KV4P_VST, *p_full = s_full + 4, *p_free = p_full + 2;   // s_full: [tile][stage]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_free + 2);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch();
   pdl_wait();
-  // the last blocks first: they attend the most keys of a prompt
-  const int bi = gridDim.x - 1 - blockIdx.x, kvh = blockIdx.y;
+  // the last blocks first, all their heads together: they attend the most keys of a prompt
+  const int hq = (a.group + 3) / 4, per = a.c.nkv * hq;
+  const int bi = int(gridDim.x) / per - 1 - int(blockIdx.x) / per, kvh = blockIdx.x % per / hq, hpart = blockIdx.x % hq;
   const int q0 = a.blocks[4 * bi], nrow = a.blocks[4 * bi + 1], crow = a.blocks[4 * bi + 2], pos0 = a.blocks[4 * bi + 3];
   if (nrow <= 0) return;                                 // (uniform over the CTA, before any barrier)
   if (q0 < 0 || nrow > 64 || q0 > a.rows - nrow || crow < 0 || crow >= a.c.cache_rows || pos0 < 0 ||
@@ -106,8 +139,8 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
     if (tid == 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_PREFILL, bi);
     return;
   }
-  const int heads = min(4, a.group - 4 * int(blockIdx.z));
-  const int head0 = kvh * a.group + 4 * blockIdx.z;
+  const int heads = min(4, a.group - 4 * hpart);
+  const int head0 = kvh * a.group + 4 * hpart;
   const int ntx = (heads + 1) / 2;                       // tiles in use
   const int klen = pos0 + nrow, nt = (klen + 63) / 64;
 
@@ -118,14 +151,14 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       mbar_init(&raw_free[s], 2 * KV4P_DEQ);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], KV4P_DEQ);
       mbar_init(&k_free[s], 1);
-      mbar_init(&v_full[s], KV4P_DEQ);
-      mbar_init(&v_free[s], 1);
-      mbar_init(&s_full[s], 2);                          // the MMAs' completion, and the issuer itself (for ek, ev)
-      mbar_init(&s_free[s], 4);
-      mbar_init(&p_full[s], 4);
+      mbar_init(&p_full[s], 4 * ntx);
       mbar_init(&p_free[s], 1);
+    }
+    for (int s = 0; s < KV4P_VST; ++s) mbar_init(&v_free[s], 1);
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&kv_full[s], 2 * KV4P_DEQ);              // K of tile j and V of tile j - 1
+      mbar_init(&s_full[s], 2);                          // the MMAs' completion, and the issuer itself (for ek, ev)
     }
     fence_mbar_init();
     for (int g = 0; g < 4; ++g) nanv[g] = 0x7FFFFFFF;
@@ -137,13 +170,14 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
   const uint32_t tmem = *tmem_slot;
 
   if (warp < KV4P_SOFT) {
+    A8_SETMAXNREG("inc", 120);
     // ---- softmax: thread = query vector (head 2 x + half, position pos0 + r)
     const int x = warp >> 2, row = (warp & 3) * 32 + lane, r = row & 63, hi = row >> 6;
     const int head = 2 * x + hi;
     const bool live = r < nrow && head < heads;
     const int pos = pos0 + min(r, nrow - 1);
-    const uint32_t tS = tmem + x * 64 + (uint32_t((warp & 3) * 32) << 16);
-    const uint32_t tO = tmem + 128 + x * HD + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t tS = tmem + x * 128 + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t tO = tmem + 256 + x * HD + (uint32_t((warp & 3) * 32) << 16);
     // the query vector: fp16, divided by the power of two of its largest element
     float qs;
     {
@@ -175,26 +209,27 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
     int E = 0;
     bool ok = true;
     for (int j = 0; x < ntx && j < nt; ++j) {
-      if (!(ok = mbar_wait_all(&s_full[x], j & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
+      const int b = 2 * x + (j & 1), ph = (j >> 1) & 1;
+      if (!(ok = kv4_wait(&s_full[b], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
       tc_fence_after();
       float sv[64];
-      tmem_ld32(tS, sv);
-      tmem_ld32(tS + 32, sv + 32);
-      const float f = qs * pow2_biased(ek[j & 3]);
-      const int Ej = ev[j & 3];
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_free[x]);
+      tmem_ld32(tS + (j & 1) * 64, sv);
+      tmem_ld32(tS + (j & 1) * 64 + 32, sv + 32);
+      const float f = qs * pow2_biased(ek[j & 7]);
+      const int Ej = ev[j & 7];
       const int kmax = pos - 64 * j;                     // keys c <= kmax of this tile are causal for this row
       if (__any_sync(0xffffffffu, kmax < 63)) {
 #pragma unroll
         for (int c = 0; c < 64; ++c) sv[c] = c <= kmax ? sv[c] : -INFINITY;
       }
-      float mx = sv[0];
+      float m4[4] = {sv[0], sv[1], sv[2], sv[3]};
 #pragma unroll
-      for (int c = 1; c < 64; ++c) mx = fmaxf(mx, sv[c]);
-      mx *= f;
-      bool waited = false;
+      for (int c = 4; c < 60; c += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m4[k] = fmaxf(fmaxf(m4[k], sv[c + k]), sv[c + 4 + k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], sv[60 + k]);
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
       if (__any_sync(0xffffffffu, mx > m + 8.f || Ej > E)) {
         const float nm = mx > m + 8.f ? mx : m;
         const float al = m == -INFINITY ? 0.f : ex2(m - nm);
@@ -203,8 +238,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
         if (j > 0) {
           // O is at rest once the previous tile's product is complete: scale it in place
           const float oa = al * (Ej > E ? pow2_biased(max(127 + E - Ej, 0)) : 1.f);
-          if (!(ok = mbar_wait_all(&p_free[x], (j - 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL))) break;
-          waited = true;
+          if (!(ok = kv4_wait(&p_free[(j - 1) & 1], ((j - 1) >> 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL))) break;
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
@@ -217,30 +251,27 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
         }
         E = max(E, Ej);
       }
-      const float mb = KV4P_BIAS - m;
-      float ls = 0.f;
+      const float2 f_2 = f2(f), mb = f2(KV4P_BIAS - m);
+      float2 ls[2] = {f2(0.f), f2(0.f)};
       uint32_t pk[32];
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        const float p0 = ex2(fmaf(sv[c], f, mb)), p1 = ex2(fmaf(sv[c + 1], f, mb));
-        ls += p0 + p1;
-        pk[c >> 1] = pack_f16(p0, p1);
-      }
-      l += ls;
-      if (j > 0 && !waited &&
-          !(ok = mbar_wait_all(&p_free[x], (j - 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL)))
-        break;
-      uint8_t* prow = smem + SM::P + x * 16384;
+      for (int c = 0; c < 64; c += 8) {
 #pragma unroll
-      for (int c = 0; c < 8; ++c)
-        *reinterpret_cast<uint4*>(prow + sw128(row, c)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
-      fence_proxy_async_smem();
+        for (int k = 0; k < 4; ++k) {
+          const float2 z = ffma2(make_float2(sv[c + 2 * k], sv[c + 2 * k + 1]), f_2, mb);
+          const float2 p = k < KV4P_POLY ? exp2_fma(z) : make_float2(ex2(z.x), ex2(z.y));
+          ls[k & 1] = fadd2(ls[k & 1], p);
+          pk[c / 2 + k] = pack_f16(p.x, p.y);
+        }
+      }
+      tmem_st32(tS + (j & 1) * 64, reinterpret_cast<const float*>(pk));
+      l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[x]);
+      if (lane == 0) mbar_arrive(&p_full[j & 1]);
     }
     if (x < ntx && ok) {
-      ok = mbar_wait_all(&p_free[x], (nt - 1) & 1, ERR_TIMEOUT_ACCUM, KERNEL_ID_KV4_PREFILL);
+      ok = kv4_wait(&p_free[(nt - 1) & 1], ((nt - 1) >> 1) & 1, ERR_TIMEOUT_ACCUM, KERNEL_ID_KV4_PREFILL);
       tc_fence_after();
       if (ok) {
         const float inv = pow2_biased(E) / l;
@@ -261,80 +292,72 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       }
     }
   } else if (warp < KV4P_SOFT + 2 * KV4P_DEQ) {
+    A8_SETMAXNREG("dec", 80);
     // ---- codes to fp16: 128 threads for K, 128 for V
     const bool isv = warp >= KV4P_SOFT + KV4P_DEQ;
-    const int dw = (warp - KV4P_SOFT) & 3, dt = dw * 32 + lane, bar = isv ? 2 : 1;
-    int E = 1;                                           // V: the largest exponent so far
+    const int dw = (warp - KV4P_SOFT) & 3, dt = dw * 32 + lane;
+    int E = 1;                                           // V's largest exponent so far
+    if (isv && lane == 0) mbar_arrive(&kv_full[0]);      // (no V comes before the first K)
     for (int j = 0; j < nt; ++j) {
       const int rs = j % KV4P_RAW, st = j & 1;
-      if (!mbar_wait_all(&raw_full[rs], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL)) break;
+      if (!kv4_wait(&raw_full[rs], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL)) break;
       const uint8_t* raw = smem + SM::RAW + rs * SM::RAWT;
-      // the tile's scales, two threads a key: the largest exponent, then fp16 scales divided by its power of two
-      const int key = dt >> 1, half = dt & 1;            // slots half * G / 2 ..
-      const bool valid = 64 * j + key < klen;
-      uint32_t sc[G / 2];
-      {
-        const uint8_t* p = raw + (key >> 4) * F::REC + (isv ? F::VS0 : F::KS0) + F::scale(key & 15, half * (G / 2));
+      const int left = klen - 64 * j;                    // positions of the tile that hold keys
+      // the exponent of the tile's largest scale (every warp finds it for itself: a lane takes 2 G of the 64 G scales)
+      auto largest = [&](int from) {
+        const uint8_t* p = raw + (lane >> 3) * F::REC + from + (lane & 7) * (4 * G);
+        uint32_t w[G], top = 0;
         if constexpr (G == 4) {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-          sc[0] = w & 0xFFFFu;
-          sc[1] = w >> 16;
+          const uint4 u = *reinterpret_cast<const uint4*>(p);
+          w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
         } else {
-          sc[0] = *reinterpret_cast<const uint16_t*>(p);
+          const uint2 u = *reinterpret_cast<const uint2*>(p);
+          w[0] = u.x; w[1] = u.y;
         }
-      }
-      int top = 0;
+        // two positions: the i-th and (i + 1)-th of lane-in-quad t, G / 2 words each
+        const int t = (lane & 7) >> 1, i = (lane & 1) * 2, k0 = (lane >> 3) * 16 + 4 * i + t,
+                  k1 = (lane >> 3) * 16 + 4 * (i + 1) + (t ^ 3);
 #pragma unroll
-      for (int k = 0; k < G / 2; ++k) {
-        if (!valid) sc[k] = 0;
-        if (sc[k] >= 0x7F80u) {                          // NaN: V counts as zero here and is put back at the end
-          if (isv) {
-            atomicMin(&nanv[half * (G / 2) + k], 64 * j + key);
-            sc[k] = 0;
-          }
-        } else {
-          top = max(top, int(sc[k] >> 7));
+        for (int k = 0; k < G; ++k) {
+          uint32_t lo = w[k] & 0xFFFFu, hi = w[k] >> 16;
+          if ((k < G / 2 ? k0 : k1) >= left) lo = hi = 0;
+          top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));      // (NaN does not count)
         }
+        return min(max(int(__reduce_max_sync(0xffffffffu, top) >> 7), 1), 253);
+      };
+      E = max(largest(F::VS0), E);
+      const int ex = isv ? E : largest(F::KS0);
+      const float down = pow2_biased_inv(ex);
+      if (!isv && dt == 0) {                             // (read by the softmax after k_full)
+        ek[j & 7] = ex;
+        ev[j & 7] = E;
       }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) red[(isv ? 4 : 0) + dw] = top;
-      named_bar_sync(bar, 128);
-      top = max(max(red[isv ? 4 : 0], red[isv ? 5 : 1]), max(red[isv ? 6 : 2], red[isv ? 7 : 3]));
-      top = min(max(top, 1), 253);
-      if (isv) E = top = max(top, E);
-      const float down = pow2_biased_inv(top);
-      __half* table = reinterpret_cast<__half*>(smem + (isv ? SM::SCV : SM::SCK));
-#pragma unroll
-      for (int k = 0; k < G / 2; ++k) {
-        const __half h = __float2half_rn(__uint_as_float(sc[k] << 16) * down);
-        table[isv ? (half * (G / 2) + k) * 64 + key : key * G + half * (G / 2) + k] = h;
-      }
-      if (dt == 0) (isv ? ev : ek)[j & 3] = top;
-      named_bar_sync(bar, 128);
       if (!isv) {
-        if (j >= 2 && !mbar_wait_all(&k_free[st], ((j >> 1) - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL)) break;
+        if (j >= 2 && !kv4_wait(&k_free[st], ((j >> 1) - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL)) break;
         uint8_t* dst = smem + SM::K + st * SM::KT;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {                    // a thread: word t8 of a key, all groups
           const int r = i * 32 + (dt >> 2), t8 = dt & 3;
           const uint8_t* src = raw + (r >> 4) * F::REC + F::kword(r & 15, t8, 0);
-          uint32_t w[G];
-          uint2 hs;
+          uint32_t w[G], ks[G / 2];
           if constexpr (G == 4) {
             const uint4 u = *reinterpret_cast<const uint4*>(src);
             w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-            hs = *reinterpret_cast<const uint2*>(table + r * G);
+            const uint2 v = *reinterpret_cast<const uint2*>(raw + (r >> 4) * F::REC + F::KS0 + F::scale(r & 15, 0));
+            ks[0] = v.x; ks[1] = v.y;
           } else {
             const uint2 u = *reinterpret_cast<const uint2*>(src);
             w[0] = u.x; w[1] = u.y;
-            hs.x = *reinterpret_cast<const uint32_t*>(table + r * G);
-            hs.y = 0;
+            ks[0] = *reinterpret_cast<const uint32_t*>(raw + (r >> 4) * F::REC + F::KS0 + F::scale(r & 15, 0));
           }
+          if (r >= left)
+#pragma unroll
+            for (int s = 0; s < G / 2; ++s) ks[s] = 0;
 #pragma unroll
           for (int s = 0; s < G; ++s) {
             const int grp = (s & 1) * (G / 2) + s / 2;
-            const uint32_t hw = s < 2 ? hs.x : hs.y, hb = (s & 1) ? __byte_perm(hw, 0, 0x3232) : __byte_perm(hw, 0, 0x1010);
-            const __half2 h = *reinterpret_cast<const __half2*>(&hb);
+            const __half2 h =
+                __float2half2_rn(__uint_as_float((s & 1) ? ks[s >> 1] & 0xFFFF0000u : ks[s >> 1] << 16) * down);
             __half2 c[4];
             kv4_codes_f16(w[s], c);
             *reinterpret_cast<uint4*>(dst + (grp >> 1) * 8192 + sw128(r, (grp & 1) * 4 + t8)) =
@@ -344,14 +367,47 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&k_full[st]);
+          mbar_arrive(&kv_full[j & 3]);
           mbar_arrive(&raw_free[rs]);
         }
       } else {
-        if (j >= 2 && !mbar_wait_all(&v_free[st], ((j >> 1) - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL)) break;
-        uint8_t* dst = smem + SM::V + st * SM::VT;
+        // this warp's half of the groups, their scales as fp16 divided by 2^E: [slot][key] (two keys a lane)
+        const int part = dw >> 1;
+        __half* table = reinterpret_cast<__half*>(smem + SM::SCV) + dw * (G / 2) * 64;
+        {
+          uint32_t sc[2][G / 2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int key = 2 * lane + k;
+            const uint8_t* p = raw + (key >> 4) * F::REC + F::VS0 + F::scale(key & 15, part * (G / 2));
+            if constexpr (G == 4) {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+              sc[k][0] = w & 0xFFFFu;
+              sc[k][1] = w >> 16;
+            } else {
+              sc[k][0] = *reinterpret_cast<const uint16_t*>(p);
+            }
+#pragma unroll
+            for (int s = 0; s < G / 2; ++s) {
+              if (key >= left) sc[k][s] = 0;
+              if (sc[k][s] >= 0x7F80u) {                 // NaN: counts as zero here and is put back at the end
+                atomicMin(&nanv[part * (G / 2) + s], 64 * j + key);
+                sc[k][s] = 0;
+              }
+            }
+          }
+#pragma unroll
+          for (int s = 0; s < G / 2; ++s)
+            *reinterpret_cast<uint32_t*>(table + s * 64 + 2 * lane) =
+                pack_f16(__uint_as_float(sc[0][s] << 16) * down, __uint_as_float(sc[1][s] << 16) * down);
+          __syncwarp();
+        }
+        const int vt = j % KV4P_VST;
+        if (j >= KV4P_VST && !kv4_wait(&v_free[vt], (j / KV4P_VST - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL))
+          break;
+        uint8_t* dst = smem + SM::V + vt * SM::VT;
         // a thread: dims 4 q .. + 3 of G / 2 groups, of eight keys
-        const int oct = dt & 7, q = (dt >> 3) & 7, part = dt >> 6;
+        const int oct = lane & 7, q = (dw & 1) * 4 + (lane >> 3);
         uint32_t w[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -362,7 +418,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
 #pragma unroll
         for (int sl = 0; sl < G / 2; ++sl) {
           const int s = part * (G / 2) + sl, grp = (s & 1) * (G / 2) + s / 2;
-          const uint4 hs = *reinterpret_cast<const uint4*>(table + s * 64 + oct * 8);
+          const uint4 hs = *reinterpret_cast<const uint4*>(table + sl * 64 + oct * 8);
           const uint32_t hp[4] = {hs.x, hs.y, hs.z, hs.w};
           uint32_t o[4][4];
 #pragma unroll
@@ -381,18 +437,20 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&v_full[st]);
+          mbar_arrive(&kv_full[(j + 1) & 3]);
           mbar_arrive(&raw_free[rs]);
         }
       }
     }
-  } else if (warp == 16) {
-    if (lane == 0) {
+    if (!isv && lane == 0) mbar_arrive(&kv_full[nt & 3]);     // (no K comes with the last V)
+  } else {
+    A8_SETMAXNREG("dec", 80);
+    if (warp == 16 && lane == 0) {
       const uint8_t* src = kv4_rec(a.c, F::REC, crow, kvh, 0);
       int issued = 0;
       for (int j = 0; j < nt; ++j) {
         const int rs = j % KV4P_RAW;
-        if (j >= KV4P_RAW && !mbar_wait(&raw_free[rs], (j / KV4P_RAW - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL))
+        if (j >= KV4P_RAW && !kv4_wait1(&raw_free[rs], (j / KV4P_RAW - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL))
           break;
         const uint32_t bytes = min(4, a.c.nblk - 4 * j) * F::REC;
         mbar_arrive_expect_tx(&raw_full[rs], bytes);
@@ -401,42 +459,50 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       }
       // every requested copy has landed before the CTA can finish (bounded after an error)
       for (int j = max(0, issued - KV4P_RAW); j < issued; ++j)
-        mbar_wait(&raw_full[j % KV4P_RAW], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
+        kv4_wait1(&raw_full[j % KV4P_RAW], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
     }
-  } else {
-    if (lane == 0) {
-      const uint32_t idS = umma_idesc(128, 64, 0), idO = umma_idesc(128, HD, 0);
-      bool ok = mbar_wait(q_full, 0, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
+    if (warp == 17) {
+      // the whole warp walks the loop (ring positions and descriptors stay warp-uniform), one elected lane issues
+      constexpr uint32_t idS = umma_idesc(128, 64, 0), idO = umma_idesc(128, HD, 0);
+      const uint64_t dQ = umma_desc_sw128(smem + SM::Q), dK = umma_desc_sw128(smem + SM::K),
+                     dV = umma_desc_sw128(smem + SM::V);
+      bool ok = kv4_wait(q_full, 0, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
+      int vt = 0;
       for (int j = 0; ok && j <= nt; ++j) {
+        const int st = j & 1;
+        if (!(ok = kv4_wait(&kv_full[j & 3], (j >> 2) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
+        tc_fence_after();                                // (S of tile j - 2 was read before its P, which this waited for)
         if (j < nt) {
-          if (!(ok = mbar_wait(&k_full[j & 1], (j >> 1) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
-          // (softmax reads ev too: it is written before V's own tile, so wait for that tile as well)
-          if (!(ok = mbar_wait(&v_full[j & 1], (j >> 1) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
-          for (int x = 0; ok && x < ntx; ++x) {
-            if (j > 0) ok = mbar_wait(&s_free[x], (j - 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL);
-            if (!ok) break;
-            tc_fence_after();
+          if (elect_one()) {
+            for (int x = 0; x < ntx; ++x) {
+              const uint32_t d = tmem + x * 128 + st * 64;
+              const uint64_t da = dQ + x * (SM::QT >> 4), db = dK + st * (SM::KT >> 4);
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k)
-              umma_f16(tmem + x * 64, umma_desc_sw128(smem + SM::Q + x * SM::QT + (k >> 2) * 16384) + 2 * (k & 3),
-                       umma_desc_sw128(smem + SM::K + (j & 1) * SM::KT + (k >> 2) * 8192) + 2 * (k & 3), idS, k != 0);
-            umma_commit(&s_full[x]);
-            mbar_arrive(&s_full[x]);
+              for (int k = 0; k < HD / 16; ++k)
+                umma_f16(d, da + (k >> 2) * (16384 >> 4) + 2 * (k & 3), db + (k >> 2) * (8192 >> 4) + 2 * (k & 3), idS, k != 0);
+              umma_commit(&s_full[2 * x + st]);
+              mbar_arrive(&s_full[2 * x + st]);
+            }
+            umma_commit(&k_free[st]);
           }
-          umma_commit(&k_free[j & 1]);
+          __syncwarp();
         }
-        if (ok && j > 0) {
-          const int p = j - 1;
-          for (int x = 0; ok && x < ntx; ++x) {
-            if (!(ok = mbar_wait(&p_full[x], p & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
-            tc_fence_after();
+        if (j > 0) {
+          const int pst = st ^ 1, pph = ((j - 1) >> 1) & 1;
+          if (!(ok = kv4_wait(&p_full[pst], pph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t db = dV + vt * (SM::VT >> 4);
+            for (int x = 0; x < ntx; ++x) {
+              const uint32_t d = tmem + 256 + x * HD, ta = tmem + x * 128 + pst * 64;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16(tmem + 128 + x * HD, umma_desc_sw128(smem + SM::P + x * 16384) + 2 * k,
-                       umma_desc_sw128(smem + SM::V + (p & 1) * SM::VT) + 2 * k, idO, (p | k) != 0);
-            umma_commit(&p_free[x]);
+              for (int k = 0; k < 4; ++k) umma_f16_ts(d, ta + 8 * k, db + 2 * k, idO, (j > 1) | (k != 0));
+            }
+            umma_commit(&p_free[pst]);
+            umma_commit(&v_free[vt]);
           }
-          umma_commit(&v_free[p & 1]);
+          __syncwarp();
+          if (++vt == KV4P_VST) vt = 0;
         }
       }
     }
@@ -451,8 +517,10 @@ static int kv4_prefill_launch(Kv4AttnArgs& a, int nblocks, cudaStream_t s) {
   const void* fn = (const void*)k_kv4_prefill<HD>;
   static std::atomic<uint64_t> ready{0};
   if (!kv4_smem_ready(ready, fn, Kv4PreSmem<HD>::TOTAL)) return A8_ERR_CUDA;
+  const long long per = (long long)a.c.nkv * ((a.group + 3) / 4);
+  if (nblocks * per >= (1ll << 31)) return A8_ERR_SIZE;
   void* args[] = {&a};
-  return kv4_launch(fn, dim3(nblocks, a.c.nkv, (a.group + 3) / 4), KV4P_THREADS, Kv4PreSmem<HD>::TOTAL, args, s) ==
+  return kv4_launch(fn, dim3(unsigned(nblocks * per)), KV4P_THREADS, Kv4PreSmem<HD>::TOTAL, args, s) ==
                  cudaSuccess ? A8_OK : A8_ERR_CUDA;
 }
 
@@ -466,7 +534,7 @@ extern "C" int a8_kv4_prefill_attention(const A8KV4* c, int layer, const void* q
   Kv4AttnArgs a;
   int rc = kv4_attn_args(&a, c, layer, q, q_stride, nq, rows, scale, out, out_stride);
   if (rc) return rc;
-  if (blocks == nullptr || nblocks <= 0 || c->nkv > 65535) return A8_ERR_ARG;
+  if (blocks == nullptr || nblocks <= 0) return A8_ERR_ARG;
   a.blocks = blocks;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return c->hd == 64 ? kv4_prefill_launch<64>(a, nblocks, s) : kv4_prefill_launch<128>(a, nblocks, s);
