@@ -258,21 +258,11 @@ struct Kv4DecSmem {
   static_assert(PART <= RING && TOTAL <= 227 * 1024 && BARS % 8 == 0, "");
 };
 
-// mbar_wait_all / mbar_wait with the limit counted on the SM's clock: a read of the global timer between two tries costs
-// about a microsecond, which a wait in the middle of a tile cannot afford.
-constexpr long long KV4_WAIT_CYCLES = 4000000000ll;   // 2 s at 2 GHz
-__device__ __forceinline__ bool kv4_wait1(uint64_t* bar, uint32_t parity, int err, int where) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity))
-    if (clock64() - t0 > KV4_WAIT_CYCLES) {
-      set_error(err, where);
-      return false;
-    }
-  return true;
-}
-__device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, int err, int where) {
-  return __all_sync(0xffffffffu, kv4_wait1(bar, parity, err, where));
+// Two waits of a warp at once: the second barrier's state is on its way while the first one's is looked at.
+__device__ __forceinline__ bool kv4_wait2(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, int err, int where) {
+  const bool ra = mbar_try_wait(a, pa), rb = mbar_try_wait(b, pb);
+  if (__all_sync(0xffffffffu, ra && rb)) return true;
+  return mbar_wait_all(a, pa, err, where) && mbar_wait_all(b, pb, err, where);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -617,7 +607,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
         }
       }
     };
-    auto arrived = [&] { return kv4_wait(&full[slot], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_ATTN); };
+    auto arrived = [&] { return mbar_wait_all(&full[slot], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_ATTN); };
     auto step = [&] {
       if (++slot == NST) {
         slot = 0;
@@ -751,7 +741,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
       if (i < n) kv4_cursor_next<HD>(a, cc);
     }
     if (!ok)                                           // a copy did not arrive: wait (bounded) for what is in flight
-      for (int s = 0; s < NST; ++s) kv4_wait(&full[s], ph ^ (s < slot), ERR_TIMEOUT_FULL, KERNEL_ID_KV4_ATTN);
+      for (int s = 0; s < NST; ++s) mbar_wait_all(&full[s], ph ^ (s < slot), ERR_TIMEOUT_FULL, KERNEL_ID_KV4_ATTN);
   }
   __syncthreads();
 

@@ -7,7 +7,7 @@
 //   warps 8-11  K: codes -> fp16 [64 keys][hd], K-major, 128-byte swizzle
 //   warps 12-15 V: codes -> fp16 V^T [hd][64 keys]
 //   warp 16     bulk copies of the key tiles' records (a tile is four records, one copy)
-//   warp 17     MMA issue: S = Q K^T, O += P V
+//   warp 17     issue of S = Q K^T     warp 18  issue of O += P V     warp 19  each tile's exponents ek, E
 // fp16, not bf16: code * s has 8 + 3 significant bits, so K and V are exact in fp16's 11 where bf16 would round each to 8.
 // Its narrow range is met by powers of two: a tile's K is divided by 2^ek (its largest scale in [1, 2)), which the softmax
 // multiplies back into its logit scale; V by 2^E, the largest scale met so far, which joins the running maximum's factor
@@ -21,15 +21,11 @@ namespace a8 {
 constexpr int KERNEL_ID_KV4_PREFILL = 12;
 constexpr int KV4P_SOFT = 8, KV4P_DEQ = 4;               // softmax warps; warps of each of K and V
 constexpr int KV4P_THREADS = (KV4P_SOFT + 2 * KV4P_DEQ + 4) * 32;   // five warpgroups (the last: warps 16, 17 and two idle)
-// Registers a thread after the warpgroups' redistribution: 256 x 120 + 256 x 80 + 128 x 80, all of the 640 x 96 = 61,440
+// Registers a thread after the warpgroups' redistribution: 256 x 136 + 256 x 72 + 128 x 64, all of the 640 x 96 = 61,440
 // that the block is launched with.
 #define A8_SETMAXNREG(op, n) asm volatile("setmaxnreg." op ".sync.aligned.u32 %0;" ::"n"(n))
 constexpr int KV4P_RAW = 6;                              // raw key tiles in flight
 constexpr int KV4P_VST = 3;                              // V tiles at hand
-#ifndef PO
-#define PO 0
-#endif
-constexpr int KV4P_POLY = PO;
 constexpr float KV4P_BIAS = 6.f;                         // p = 2^(x - m + 6)
 
 template <int HD>
@@ -43,9 +39,9 @@ struct Kv4PreSmem {
   static constexpr int RAW = V + KV4P_VST * VT;
   static constexpr int RAWT = 4 * Kv4<HD>::REC;
   static constexpr int SCV = RAW + KV4P_RAW * RAWT;      // fp16 [4 warps][G / 2][64 keys]: V scales of the tile, divided
-  static constexpr int MISC = SCV + 4 * 64 * (HD / 64) * 2;  // int ek[8], ev[8], nanv[4]
-  static constexpr int BARS = MISC + 96;
-  static constexpr int TOTAL = BARS + 32 * 8 + 16 + 1024;
+  static constexpr int MISC = SCV + 4 * 64 * (HD / 64) * 2;  // int ek[16], ev[16], nanv[4]
+  static constexpr int BARS = MISC + 144;
+  static constexpr int TOTAL = BARS + 40 * 8 + 16 + 1024;
   static constexpr uint32_t COLS = 512;                  // TMEM: S of tile 0 and 1, two stages of 64 each (P takes
                                                          // the first half of its S); O (HD each)
   static_assert(TOTAL <= 227 * 1024, "");
@@ -62,22 +58,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
       "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-// 2^x for a pair, x <= 127 (below -126 as 2^-126), on the FMA units: x = i + f, |f| <= 1/2, 2^f by a degree-4 polynomial
-// fitted here for least relative error (2.6e-6), i added to its exponent.
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 magic = f2(12582912.f);                   // 1.5 x 2^23: the low bits of the sum are round(x)
-  const float2 t = fadd2(x, magic);
-  const float2 f = fsub2(x, fsub2(t, magic));
-  float2 p = ffma2(f2(0.009570068679749966f), f, f2(0.055917806923389435f));
-  p = ffma2(p, f, f2(0.240247443318367f));
-  p = ffma2(p, f, f2(0.6931218504905701f));
-  p = ffma2(p, f, f2(0.9999992847442627f));
-  return make_float2(__uint_as_float(__float_as_uint(t.x) * 0x800000u + __float_as_uint(p.x)),
-                     __uint_as_float(__float_as_uint(t.y) * 0x800000u + __float_as_uint(p.y)));
 }
 
 // D += A B with A (128 rows x 16 fp16, two a column) in tensor memory, B in shared memory
@@ -118,12 +98,12 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
   constexpr int G = F::G;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  int* ek = reinterpret_cast<int*>(smem + SM::MISC);     // by tile % 8
-  int* ev = ek + 8;
-  int* nanv = ev + 8;                                    // [4] first position whose V group is NaN
+  int* ek = reinterpret_cast<int*>(smem + SM::MISC);     // by tile % 16
+  int* ev = ek + 16;
+  int* nanv = ev + 16;                                   // [4] first position whose V group is NaN
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + SM::BARS);
-  uint64_t *raw_full = q_full + 1, *raw_free = raw_full + KV4P_RAW, *kv_full = raw_free + KV4P_RAW, *k_free = kv_full + 4,
-           *v_free = k_free + 2, *s_full = v_free + KV4P_VST, *p_full = s_full + 4, *p_free = p_full + 2;   // s_full: [tile][stage]
+  uint64_t *raw_full = q_full + 1, *raw_free = raw_full + KV4P_RAW, *e_full = raw_free + KV4P_RAW, *k_full = e_full + KV4P_RAW,
+           *k_free = k_full + 2, *v_full = k_free + 2, *v_free = v_full + KV4P_VST, *s_full = v_free + KV4P_VST, *p_full = s_full + 4, *p_free = p_full + 2;   // s_full: [tile][stage]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_free + 2);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -148,16 +128,20 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
     mbar_init(q_full, KV4P_SOFT);
     for (int s = 0; s < KV4P_RAW; ++s) {
       mbar_init(&raw_full[s], 1);
-      mbar_init(&raw_free[s], 2 * KV4P_DEQ);
+      mbar_init(&raw_free[s], 2 * KV4P_DEQ + 1);
+      mbar_init(&e_full[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], KV4P_DEQ);
       mbar_init(&k_free[s], 1);
       mbar_init(&p_full[s], 4 * ntx);
       mbar_init(&p_free[s], 1);
     }
-    for (int s = 0; s < KV4P_VST; ++s) mbar_init(&v_free[s], 1);
+    for (int s = 0; s < KV4P_VST; ++s) {
+      mbar_init(&v_full[s], KV4P_DEQ);
+      mbar_init(&v_free[s], 1);
+    }
     for (int s = 0; s < 4; ++s) {
-      mbar_init(&kv_full[s], 2 * KV4P_DEQ);              // K of tile j and V of tile j - 1
       mbar_init(&s_full[s], 2);                          // the MMAs' completion, and the issuer itself (for ek, ev)
     }
     fence_mbar_init();
@@ -170,7 +154,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
   const uint32_t tmem = *tmem_slot;
 
   if (warp < KV4P_SOFT) {
-    A8_SETMAXNREG("inc", 120);
+    A8_SETMAXNREG("inc", 136);
     // ---- softmax: thread = query vector (head 2 x + half, position pos0 + r)
     const int x = warp >> 2, row = (warp & 3) * 32 + lane, r = row & 63, hi = row >> 6;
     const int head = 2 * x + hi;
@@ -210,13 +194,13 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
     bool ok = true;
     for (int j = 0; x < ntx && j < nt; ++j) {
       const int b = 2 * x + (j & 1), ph = (j >> 1) & 1;
-      if (!(ok = kv4_wait(&s_full[b], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
+      if (!(ok = mbar_wait_all(&s_full[b], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
       tc_fence_after();
       float sv[64];
       tmem_ld32(tS + (j & 1) * 64, sv);
       tmem_ld32(tS + (j & 1) * 64 + 32, sv + 32);
-      const float f = qs * pow2_biased(ek[j & 7]);
-      const int Ej = ev[j & 7];
+      const float f = qs * pow2_biased(ek[j & 15]);
+      const int Ej = ev[j & 15];
       const int kmax = pos - 64 * j;                     // keys c <= kmax of this tile are causal for this row
       if (__any_sync(0xffffffffu, kmax < 63)) {
 #pragma unroll
@@ -238,7 +222,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
         if (j > 0) {
           // O is at rest once the previous tile's product is complete: scale it in place
           const float oa = al * (Ej > E ? pow2_biased(max(127 + E - Ej, 0)) : 1.f);
-          if (!(ok = kv4_wait(&p_free[(j - 1) & 1], ((j - 1) >> 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL))) break;
+          if (!(ok = mbar_wait_all(&p_free[(j - 1) & 1], ((j - 1) >> 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL))) break;
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
@@ -259,7 +243,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float2 z = ffma2(make_float2(sv[c + 2 * k], sv[c + 2 * k + 1]), f_2, mb);
-          const float2 p = k < KV4P_POLY ? exp2_fma(z) : make_float2(ex2(z.x), ex2(z.y));
+          const float2 p = make_float2(ex2(z.x), ex2(z.y));
           ls[k & 1] = fadd2(ls[k & 1], p);
           pk[c / 2 + k] = pack_f16(p.x, p.y);
         }
@@ -271,7 +255,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       if (lane == 0) mbar_arrive(&p_full[j & 1]);
     }
     if (x < ntx && ok) {
-      ok = kv4_wait(&p_free[(nt - 1) & 1], ((nt - 1) >> 1) & 1, ERR_TIMEOUT_ACCUM, KERNEL_ID_KV4_PREFILL);
+      ok = mbar_wait_all(&p_free[(nt - 1) & 1], ((nt - 1) >> 1) & 1, ERR_TIMEOUT_ACCUM, KERNEL_ID_KV4_PREFILL);
       tc_fence_after();
       if (ok) {
         const float inv = pow2_biased(E) / l;
@@ -292,48 +276,18 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       }
     }
   } else if (warp < KV4P_SOFT + 2 * KV4P_DEQ) {
-    A8_SETMAXNREG("dec", 80);
+    A8_SETMAXNREG("dec", 72);
     // ---- codes to fp16: 128 threads for K, 128 for V
     const bool isv = warp >= KV4P_SOFT + KV4P_DEQ;
     const int dw = (warp - KV4P_SOFT) & 3, dt = dw * 32 + lane;
-    int E = 1;                                           // V's largest exponent so far
-    if (isv && lane == 0) mbar_arrive(&kv_full[0]);      // (no V comes before the first K)
     for (int j = 0; j < nt; ++j) {
-      const int rs = j % KV4P_RAW, st = j & 1;
-      if (!kv4_wait(&raw_full[rs], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL)) break;
+      const int rs = j % KV4P_RAW, st = j & 1, rph = (j / KV4P_RAW) & 1;
+      if (!kv4_wait2(&raw_full[rs], rph, &e_full[rs], rph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL)) break;
       const uint8_t* raw = smem + SM::RAW + rs * SM::RAWT;
       const int left = klen - 64 * j;                    // positions of the tile that hold keys
-      // the exponent of the tile's largest scale (every warp finds it for itself: a lane takes 2 G of the 64 G scales)
-      auto largest = [&](int from) {
-        const uint8_t* p = raw + (lane >> 3) * F::REC + from + (lane & 7) * (4 * G);
-        uint32_t w[G], top = 0;
-        if constexpr (G == 4) {
-          const uint4 u = *reinterpret_cast<const uint4*>(p);
-          w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(p);
-          w[0] = u.x; w[1] = u.y;
-        }
-        // two positions: the i-th and (i + 1)-th of lane-in-quad t, G / 2 words each
-        const int t = (lane & 7) >> 1, i = (lane & 1) * 2, k0 = (lane >> 3) * 16 + 4 * i + t,
-                  k1 = (lane >> 3) * 16 + 4 * (i + 1) + (t ^ 3);
-#pragma unroll
-        for (int k = 0; k < G; ++k) {
-          uint32_t lo = w[k] & 0xFFFFu, hi = w[k] >> 16;
-          if ((k < G / 2 ? k0 : k1) >= left) lo = hi = 0;
-          top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));      // (NaN does not count)
-        }
-        return min(max(int(__reduce_max_sync(0xffffffffu, top) >> 7), 1), 253);
-      };
-      E = max(largest(F::VS0), E);
-      const int ex = isv ? E : largest(F::KS0);
-      const float down = pow2_biased_inv(ex);
-      if (!isv && dt == 0) {                             // (read by the softmax after k_full)
-        ek[j & 7] = ex;
-        ev[j & 7] = E;
-      }
+      const float down = pow2_biased_inv(isv ? ev[j & 15] : ek[j & 15]);
       if (!isv) {
-        if (j >= 2 && !kv4_wait(&k_free[st], ((j >> 1) - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL)) break;
+        if (j >= 2 && !mbar_wait_all(&k_free[st], ((j >> 1) - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL)) break;
         uint8_t* dst = smem + SM::K + st * SM::KT;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {                    // a thread: word t8 of a key, all groups
@@ -367,7 +321,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&kv_full[j & 3]);
+          mbar_arrive(&k_full[st]);
           mbar_arrive(&raw_free[rs]);
         }
       } else {
@@ -403,7 +357,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
           __syncwarp();
         }
         const int vt = j % KV4P_VST;
-        if (j >= KV4P_VST && !kv4_wait(&v_free[vt], (j / KV4P_VST - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL))
+        if (j >= KV4P_VST && !mbar_wait_all(&v_free[vt], (j / KV4P_VST - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL))
           break;
         uint8_t* dst = smem + SM::V + vt * SM::VT;
         // a thread: dims 4 q .. + 3 of G / 2 groups, of eight keys
@@ -437,20 +391,19 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&kv_full[(j + 1) & 3]);
+          mbar_arrive(&v_full[vt]);
           mbar_arrive(&raw_free[rs]);
         }
       }
     }
-    if (!isv && lane == 0) mbar_arrive(&kv_full[nt & 3]);     // (no K comes with the last V)
   } else {
-    A8_SETMAXNREG("dec", 80);
+    A8_SETMAXNREG("dec", 64);
     if (warp == 16 && lane == 0) {
       const uint8_t* src = kv4_rec(a.c, F::REC, crow, kvh, 0);
       int issued = 0;
       for (int j = 0; j < nt; ++j) {
         const int rs = j % KV4P_RAW;
-        if (j >= KV4P_RAW && !kv4_wait1(&raw_free[rs], (j / KV4P_RAW - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL))
+        if (j >= KV4P_RAW && !mbar_wait(&raw_free[rs], (j / KV4P_RAW - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL))
           break;
         const uint32_t bytes = min(4, a.c.nblk - 4 * j) * F::REC;
         mbar_arrive_expect_tx(&raw_full[rs], bytes);
@@ -459,51 +412,98 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       }
       // every requested copy has landed before the CTA can finish (bounded after an error)
       for (int j = max(0, issued - KV4P_RAW); j < issued; ++j)
-        kv4_wait1(&raw_full[j % KV4P_RAW], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
+        mbar_wait(&raw_full[j % KV4P_RAW], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
     }
+    // a whole warp walks each issue loop (ring positions and descriptors stay warp-uniform), one elected lane issues
     if (warp == 17) {
-      // the whole warp walks the loop (ring positions and descriptors stay warp-uniform), one elected lane issues
-      constexpr uint32_t idS = umma_idesc(128, 64, 0), idO = umma_idesc(128, HD, 0);
-      const uint64_t dQ = umma_desc_sw128(smem + SM::Q), dK = umma_desc_sw128(smem + SM::K),
-                     dV = umma_desc_sw128(smem + SM::V);
-      bool ok = kv4_wait(q_full, 0, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
-      int vt = 0;
-      for (int j = 0; ok && j <= nt; ++j) {
+      constexpr uint32_t idS = umma_idesc(128, 64, 0);
+      const uint64_t dQ = umma_desc_sw128(smem + SM::Q), dK = umma_desc_sw128(smem + SM::K);
+      bool ok = mbar_wait_all(q_full, 0, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
+      for (int j = 0; ok && j < nt; ++j) {
+        const int st = j & 1, ph = (j >> 1) & 1;
+        // K of this tile; the stage's last P (in the columns of S) has been multiplied
+        if (j < 2)
+          ok = mbar_wait_all(&k_full[st], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
+        else
+          ok = kv4_wait2(&k_full[st], ph, &p_free[st], ph ^ 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          for (int x = 0; x < ntx; ++x) {
+            const uint32_t d = tmem + x * 128 + st * 64;
+            const uint64_t da = dQ + x * (SM::QT >> 4), db = dK + st * (SM::KT >> 4);
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+              umma_f16(d, da + (k >> 2) * (16384 >> 4) + 2 * (k & 3), db + (k >> 2) * (8192 >> 4) + 2 * (k & 3), idS, k != 0);
+            umma_commit(&s_full[2 * x + st]);
+            mbar_arrive(&s_full[2 * x + st]);
+          }
+          umma_commit(&k_free[st]);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 18) {
+      constexpr uint32_t idO = umma_idesc(128, HD, 0);
+      const uint64_t dV = umma_desc_sw128(smem + SM::V);
+      int vt = 0, vph = 0;
+      for (int j = 0; j < nt; ++j) {
         const int st = j & 1;
-        if (!(ok = kv4_wait(&kv_full[j & 3], (j >> 2) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
-        tc_fence_after();                                // (S of tile j - 2 was read before its P, which this waited for)
-        if (j < nt) {
-          if (elect_one()) {
-            for (int x = 0; x < ntx; ++x) {
-              const uint32_t d = tmem + x * 128 + st * 64;
-              const uint64_t da = dQ + x * (SM::QT >> 4), db = dK + st * (SM::KT >> 4);
+        if (!kv4_wait2(&p_full[st], (j >> 1) & 1, &v_full[vt], vph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL)) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t db = dV + vt * (SM::VT >> 4);
+          for (int x = 0; x < ntx; ++x) {
+            const uint32_t d = tmem + 256 + x * HD, ta = tmem + x * 128 + st * 64;
 #pragma unroll
-              for (int k = 0; k < HD / 16; ++k)
-                umma_f16(d, da + (k >> 2) * (16384 >> 4) + 2 * (k & 3), db + (k >> 2) * (8192 >> 4) + 2 * (k & 3), idS, k != 0);
-              umma_commit(&s_full[2 * x + st]);
-              mbar_arrive(&s_full[2 * x + st]);
-            }
-            umma_commit(&k_free[st]);
+            for (int k = 0; k < 4; ++k) umma_f16_ts(d, ta + 8 * k, db + 2 * k, idO, (j > 0) | (k != 0));
           }
-          __syncwarp();
+          umma_commit(&p_free[st]);
+          umma_commit(&v_free[vt]);
         }
-        if (j > 0) {
-          const int pst = st ^ 1, pph = ((j - 1) >> 1) & 1;
-          if (!(ok = kv4_wait(&p_full[pst], pph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint64_t db = dV + vt * (SM::VT >> 4);
-            for (int x = 0; x < ntx; ++x) {
-              const uint32_t d = tmem + 256 + x * HD, ta = tmem + x * 128 + pst * 64;
+        __syncwarp();
+        if (++vt == KV4P_VST) {
+          vt = 0;
+          vph ^= 1;
+        }
+      }
+    } else if (warp == 19) {
+      // the exponents of each tile's largest scales (a lane takes 2 G of the 64 G); V's only grows
+      int E = 1;
+      for (int j = 0; j < nt; ++j) {
+        const int rs = j % KV4P_RAW;
+        if (!mbar_wait_all(&raw_full[rs], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL)) break;
+        const uint8_t* raw = smem + SM::RAW + rs * SM::RAWT;
+        const int left = klen - 64 * j;
+        auto largest = [&](int from) {
+          const uint8_t* p = raw + (lane >> 3) * F::REC + from + (lane & 7) * (4 * G);
+          uint32_t w[G], top = 0;
+          if constexpr (G == 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(p);
+            w[0] = u.x; w[1] = u.y;
+          }
+          // two positions: the i-th and (i + 1)-th of lane-in-quad t, G / 2 words each
+          const int t = (lane & 7) >> 1, i = (lane & 1) * 2, k0 = (lane >> 3) * 16 + 4 * i + t,
+                    k1 = (lane >> 3) * 16 + 4 * (i + 1) + (t ^ 3);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) umma_f16_ts(d, ta + 8 * k, db + 2 * k, idO, (j > 1) | (k != 0));
-            }
-            umma_commit(&p_free[pst]);
-            umma_commit(&v_free[vt]);
+          for (int k = 0; k < G; ++k) {
+            uint32_t lo = w[k] & 0xFFFFu, hi = w[k] >> 16;
+            if ((k < G / 2 ? k0 : k1) >= left) lo = hi = 0;
+            top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));      // (NaN does not count)
           }
-          __syncwarp();
-          if (++vt == KV4P_VST) vt = 0;
+          return min(max(int(__reduce_max_sync(0xffffffffu, top) >> 7), 1), 253);
+        };
+        E = max(largest(F::VS0), E);
+        const int ex = largest(F::KS0);
+        if (lane == 0) {
+          ek[j & 15] = ex;
+          ev[j & 15] = E;
+          mbar_arrive(&e_full[rs]);
+          mbar_arrive(&raw_free[rs]);
         }
+        __syncwarp();
       }
     }
   }
