@@ -66,35 +66,61 @@ struct Kv4StoreArgs {
   int ldq;
 };
 
-__device__ __forceinline__ void ld8f(const __nv_bfloat16* p, float* f) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y), c = unpack_bf16(u.z), d = unpack_bf16(u.w);
-  f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+// The 8 codes of this thread's dims (w: bf16 pairs; nibble n = dim n) and the scale of the group that they share with the
+// other three lanes of the aligned four. rint(x / s) without a division an element: x (1 / s) is off by under 2^-21 of
+// itself, and snapped to a multiple of 2^-10 it is on the right side of every border: a quotient that is not on the
+// border n + 1/2 is at least 2^-9.9 from it (x - (n + 1/2) s is a whole multiple of a 12-bit grid), one that is on it snaps
+// to it exactly.
+__device__ __forceinline__ uint32_t kv4_quant8(const uint32_t* w, uint32_t& scale_bits) {
+  // (as whole numbers the magnitudes order infinities and NaN above all)
+  uint32_t mm = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+  mm = __vmaxu2(mm, __shfl_xor_sync(0xffffffffu, mm, 1));
+  mm = __vmaxu2(mm, __shfl_xor_sync(0xffffffffu, mm, 2));
+  const uint32_t top = max(mm & 0xFFFFu, mm >> 16);
+  if (top >= 0x7F80u) {
+    scale_bits = 0x7FFFu;
+    return 0x88888888u;
+  }
+  const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(top << 16), 7.0f));
+  scale_bits = __bfloat16_as_ushort(sb);
+  float s = __bfloat162float(sb);
+  if (s == 0.f) return 0x88888888u;
+  float x[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 d = unpack_bf16(w[k]);
+    x[2 * k] = d.x;
+    x[2 * k + 1] = d.y;
+  }
+  if (s < 0x1p-100f) {
+    // a scale of few bits may be well below max|x| / 7: clamp; and keep 1 / s finite (both exact)
+    s *= 0x1p100f;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) x[n] = fminf(fmaxf(x[n] * 0x1p100f, -7.f * s), 7.f * s);
+  }
+  const float inv = __fdiv_rn(1.f, s);
+  uint32_t c = 0;
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const float y = fmaf(x[n], inv, 12288.f) - 12288.f;                     // 1.5 x 2^13: whole multiples of 2^-10
+    c |= (__float_as_uint(y + 12582920.f) & 15u) << (4 * n);                // 1.5 x 2^23 + 8: rint(y) + 8 in the low bits
+  }
+  return c;
 }
 
-// The 8 codes of this thread's dims (nibble n = dim n) and the scale of the group they share with the other three lanes
-// of the aligned four.
-__device__ __forceinline__ uint32_t kv4_quant8(const float* x, uint32_t& scale_bits) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int n = 0; n < 8; ++n) m = max(m, __float_as_uint(x[n]) & 0x7FFFFFFFu);   // (orders inf and NaN above all)
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  uint32_t w = 0x88888888u;
-  if (m >= 0x7F800000u) {
-    scale_bits = 0x7FFFu;
-    return w;
-  }
-  const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(m), 7.0f));
-  scale_bits = __bfloat16_as_ushort(sb);
-  const float s = __bfloat162float(sb);
-  if (s > 0.f) {
-    w = 0;
-#pragma unroll
-    for (int n = 0; n < 8; ++n)
-      w |= uint32_t(min(max(__float2int_rn(__fdiv_rn(x[n], s)), -7), 7) + 8) << (4 * n);
-  }
-  return w;
+// The (row, head, part of TPH) of this thread in the row-major sequence of all; false behind the last (the row is clamped).
+// The 64-bit division is the block's, the thread's is of a small number.
+template <int TPH>
+__device__ __forceinline__ bool kv4_item(int heads, int rows, int& row, int& head, int& sub) {
+  const unsigned per = (unsigned)heads * TPH;
+  const unsigned long long first = (unsigned long long)blockIdx.x * blockDim.x;
+  const unsigned long long r0 = first / per;
+  const unsigned t = unsigned(first - r0 * per) + threadIdx.x, up = t / per, in = t - up * per;
+  const unsigned long long r = r0 + up;
+  sub = in % TPH;
+  head = in / TPH;
+  row = int(min(r, (unsigned long long)rows - 1));
+  return r < (unsigned long long)rows;
 }
 
 // One thread: 8 dims of a head and the 8 dims hd / 2 further (a RoPE pair each) of one row's q, k or v head; the scale of
@@ -106,12 +132,13 @@ __global__ void __launch_bounds__(256) k_kv4_store(const Kv4StoreArgs a) {
   pdl_launch();
   pdl_wait();
   const int heads = a.nq + 2 * a.c.nkv;
-  const long long idx = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int sub = int(idx % TPH);
-  const long long rh = idx / TPH;
-  const int head = int(rh % heads);
-  const int row = int(min(rh / heads, (long long)a.rows - 1));
-  bool live = rh / heads < a.rows;
+  int row, head, sub;
+  bool live = kv4_item<TPH>(heads, a.rows, row, head, sub);
+  const int d0 = sub * 8;
+  const __nv_bfloat16* x = a.qkv + (size_t)row * a.ld + head * HD + d0;
+  uint32_t lo[4], hi[4];                                 // (on their way while the position is read)
+  *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(x);
+  *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(x + HD / 2);
   const int pos = a.pos[row];
   const int slot = a.slot != nullptr ? a.slot[row] : row;
   const int at = a.ring > 0 ? pos % a.ring : pos;
@@ -120,36 +147,26 @@ __global__ void __launch_bounds__(256) k_kv4_store(const Kv4StoreArgs a) {
     if (sub == 0 && head == 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_STORE, row);
     live = false;
   }
-  const int d0 = sub * 8;
-  float lo[8], hi[8];
+  if (live && a.cos != nullptr && head < a.nq + a.c.nkv) {
+    uint32_t cw[4], sw[4];
+    *reinterpret_cast<uint4*>(cw) = *reinterpret_cast<const uint4*>(a.cos + (size_t)pos * HD + d0);
+    *reinterpret_cast<uint4*>(sw) = *reinterpret_cast<const uint4*>(a.sin + (size_t)pos * HD + d0);
 #pragma unroll
-  for (int n = 0; n < 8; ++n) lo[n] = hi[n] = 0.f;
-  if (live) {
-    const __nv_bfloat16* x = a.qkv + (size_t)row * a.ld + head * HD;
-    ld8f(x + d0, lo);
-    ld8f(x + d0 + HD / 2, hi);
-    if (a.cos != nullptr && head < a.nq + a.c.nkv) {
-      float c[8], s[8];
-      ld8f(a.cos + (size_t)pos * HD + d0, c);
-      ld8f(a.sin + (size_t)pos * HD + d0, s);
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        // products of two bf16 are exact in fp32: the rotation is one fp32 rounding and one to bf16, what a bf16 cache
-        // would hold
-        const float u = lo[n], v = hi[n];
-        lo[n] = bf16r(u * c[n] - v * s[n]);
-        hi[n] = bf16r(v * c[n] + u * s[n]);
-      }
-    }
-    if (head < a.nq) {
-      __nv_bfloat16* y = a.q + (size_t)row * a.ldq + head * HD + d0;
-      *reinterpret_cast<uint4*>(y) = make_uint4(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]),
-                                                pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7]));
-      *reinterpret_cast<uint4*>(y + HD / 2) = make_uint4(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]),
-                                                         pack_bf16(hi[4], hi[5]), pack_bf16(hi[6], hi[7]));
+    for (int k = 0; k < 4; ++k) {
+      // products of two bf16 are exact in fp32: the rotation is one fp32 rounding and one to bf16, what a bf16 cache
+      // would hold
+      const float2 u = unpack_bf16(lo[k]), v = unpack_bf16(hi[k]), c = unpack_bf16(cw[k]), s = unpack_bf16(sw[k]);
+      lo[k] = pack_bf16(u.x * c.x - v.x * s.x, u.y * c.y - v.y * s.y);
+      hi[k] = pack_bf16(v.x * c.x + u.x * s.x, v.y * c.y + u.y * s.y);
     }
   }
-  // (every lane takes part in the group maximum)
+  if (live && head < a.nq) {
+    __nv_bfloat16* y = a.q + (size_t)row * a.ldq + head * HD + d0;
+    *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(lo);
+    *reinterpret_cast<uint4*>(y + HD / 2) = *reinterpret_cast<const uint4*>(hi);
+  }
+  // (a group's maximum takes every lane of its warp; warps of query heads alone are done)
+  if (!__any_sync(0xffffffffu, live && head >= a.nq)) return;
   uint32_t slo, shi;
   const uint32_t wlo = kv4_quant8(lo, slo), whi = kv4_quant8(hi, shi);
   if (!live || head < a.nq) return;
@@ -190,12 +207,8 @@ __global__ void __launch_bounds__(256) k_kv4_load(const Kv4LoadArgs a) {
   constexpr int TPH = HD / 16;
   pdl_launch();
   pdl_wait();
-  const long long idx = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int sub = int(idx % TPH);
-  const long long rh = idx / TPH;
-  const int h = int(rh % a.c.nkv);
-  if (rh / a.c.nkv >= a.rows) return;
-  const int row = int(rh / a.c.nkv);
+  int row, h, sub;
+  if (!kv4_item<TPH>(a.c.nkv, a.rows, row, h, sub)) return;
   const int pos = a.pos[row];
   const int slot = a.slot != nullptr ? a.slot[row] : row;
   if (pos < 0) return;
