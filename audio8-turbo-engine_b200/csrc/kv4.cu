@@ -193,12 +193,28 @@ struct Kv4LoadArgs {
   int ldk, ldv;
 };
 
-// bf16(code * s) of the 8 nibbles of w
-__device__ __forceinline__ uint4 kv4_deq8(uint32_t w, float s) {
-  float f[8];
+// Codes n of the two 16-bit halves of w as bf16: the nibble u is the low mantissa bits of 128 + u; less 136 is exact.
+template <int N>
+__device__ __forceinline__ uint32_t kv4_pair(uint32_t w) {
+  uint32_t d;
+  asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, 0x000F000F, 0x43004300, 0xEA;\n\tadd.rn.bf16x2 %0, t, %2;\n\t}"
+      : "=r"(d)
+      : "r"(w >> (4 * N)), "r"(0xC308C308u));
+  return d;
+}
+// bf16(code * s) of the 8 nibbles of w: a product of bf16 numbers rounded once
+__device__ __forceinline__ uint4 kv4_deq8(uint32_t w, uint32_t s_low) {
+  const uint32_t ss = __byte_perm(s_low, 0, 0x1010);
+  const __nv_bfloat162 s2 = *reinterpret_cast<const __nv_bfloat162*>(&ss);
+  const uint32_t c[4] = {kv4_pair<0>(w), kv4_pair<1>(w), kv4_pair<2>(w), kv4_pair<3>(w)};   // dims (n, n + 4)
+  uint32_t v[4];
 #pragma unroll
-  for (int n = 0; n < 8; ++n) f[n] = float(int((w >> (4 * n)) & 15u) - 8) * s;
-  return make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+  for (int n = 0; n < 4; ++n) {
+    const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&c[n]), s2);
+    v[n] = *reinterpret_cast<const uint32_t*>(&x);
+  }
+  return make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                    __byte_perm(v[2], v[3], 0x7632));
 }
 
 template <int HD>
@@ -218,20 +234,27 @@ __global__ void __launch_bounds__(256) k_kv4_load(const Kv4LoadArgs a) {
   }
   const int t8 = sub & 3, s0 = (sub >> 2) * 2, j = pos % KV4_BLK;
   const uint8_t* rec = kv4_rec(a.c, F::REC, slot, h, pos / KV4_BLK);
+  // both heads' words and scales are on their way before the first is used
+  uint2 w = make_uint2(0, 0);
+  uint32_t u0 = 0, u1 = 0, ks = 0, vs = 0;
   if (a.k != nullptr) {
-    const uint2 w = *reinterpret_cast<const uint2*>(rec + F::kword(j, t8, s0));
-    const float2 s = unpack_bf16(*reinterpret_cast<const uint32_t*>(rec + F::KS0 + F::scale(j, s0)));
-    __nv_bfloat16* y = a.k + (size_t)row * a.ldk + h * HD + sub * 8;
-    *reinterpret_cast<uint4*>(y) = kv4_deq8(w.x, s.x);
-    *reinterpret_cast<uint4*>(y + HD / 2) = kv4_deq8(w.y, s.y);
+    w = *reinterpret_cast<const uint2*>(rec + F::kword(j, t8, s0));
+    ks = *reinterpret_cast<const uint32_t*>(rec + F::KS0 + F::scale(j, s0));
   }
   if (a.v != nullptr) {
-    const uint32_t u0 = *reinterpret_cast<const uint32_t*>(rec + F::vhalf(j, 2 * t8, s0));
-    const uint32_t u1 = *reinterpret_cast<const uint32_t*>(rec + F::vhalf(j, 2 * t8 + 1, s0));
-    const float2 s = unpack_bf16(*reinterpret_cast<const uint32_t*>(rec + F::VS0 + F::scale(j, s0)));
+    u0 = *reinterpret_cast<const uint32_t*>(rec + F::vhalf(j, 2 * t8, s0));
+    u1 = *reinterpret_cast<const uint32_t*>(rec + F::vhalf(j, 2 * t8 + 1, s0));
+    vs = *reinterpret_cast<const uint32_t*>(rec + F::VS0 + F::scale(j, s0));
+  }
+  if (a.k != nullptr) {
+    __nv_bfloat16* y = a.k + (size_t)row * a.ldk + h * HD + sub * 8;
+    *reinterpret_cast<uint4*>(y) = kv4_deq8(w.x, ks);
+    *reinterpret_cast<uint4*>(y + HD / 2) = kv4_deq8(w.y, ks >> 16);
+  }
+  if (a.v != nullptr) {
     __nv_bfloat16* y = a.v + (size_t)row * a.ldv + h * HD + sub * 8;
-    *reinterpret_cast<uint4*>(y) = kv4_deq8((u0 & 0xFFFFu) | (u1 << 16), s.x);
-    *reinterpret_cast<uint4*>(y + HD / 2) = kv4_deq8((u0 >> 16) | (u1 & 0xFFFF0000u), s.y);
+    *reinterpret_cast<uint4*>(y) = kv4_deq8((u0 & 0xFFFFu) | (u1 << 16), vs);
+    *reinterpret_cast<uint4*>(y + HD / 2) = kv4_deq8((u0 >> 16) | (u1 & 0xFFFF0000u), vs >> 16);
   }
 }
 
@@ -282,15 +305,6 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-// Codes n of the two 16-bit halves of w as bf16: the nibble u is the low mantissa bits of 128 + u; less 136 is exact.
-template <int N>
-__device__ __forceinline__ uint32_t kv4_pair(uint32_t w) {
-  uint32_t d;
-  asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, 0x000F000F, 0x43004300, 0xEA;\n\tadd.rn.bf16x2 %0, t, %2;\n\t}"
-      : "=r"(d)
-      : "r"(w >> (4 * N)), "r"(0xC308C308u));
-  return d;
 }
 // The same codes as fp16 with an offset: nibbles 0 and 2 of a half as 1024 + u, 1 and 3 as 1024 + 16 u (mask with or).
 __device__ __forceinline__ uint32_t kv4_lo16(uint32_t w) {
