@@ -275,18 +275,19 @@ struct Kv4AttnArgs {
 };
 
 constexpr int KV4_CTAS = 148;         // one a SM
-constexpr int KV4_CTA_RECS = 48;      // fewer records than CTAs x this: fewer CTAs
+constexpr int KV4_STEP = 32;           // positions a warp takes at a time: two records
+constexpr int KV4_CTA_STEPS = 24;      // fewer steps than CTAs x this: fewer CTAs
 constexpr float KV4_LAZY = 8.f;       // a running maximum moves when a logit passes it by 2^8
 
 template <int HD, int NT>
 struct Kv4DecSmem {
   static constexpr int NW = HD == 64 ? 16 : NT == 1 ? 12 : 8;     // warps (each holds O [hd][8 NT] in registers)
-  static constexpr int NST = NW == 12 ? 6 : 8;                    // records in flight a warp
-  static constexpr int RING = NST * Kv4<HD>::REC;
+  static constexpr int NST = HD == 64 ? 4 : 3;                    // steps in flight a warp
+  static constexpr int RING = NST * 2 * Kv4<HD>::REC;
   static constexpr int PART = (8 * NT * HD + 16 * NT) * 4;        // bytes: O [8 NT][hd], (max, sum) [8 NT]
   static constexpr int HEADP = NW * RING;                         // first partials; the last ones go into the rings
-  static constexpr int PRE = HEADP + NW * PART;                   // prefix of the rows' records by thread
-  static constexpr int META = PRE + (NW * 32 + 4) * 4;            // int [2 NW][4]: unit, its first and end record, run
+  static constexpr int PRE = HEADP + NW * PART;                   // prefix of the rows' steps by thread
+  static constexpr int META = PRE + (NW * 32 + 4) * 4;            // int [2 NW][4]: unit, its first and end step, run
   static constexpr int RUNS = META + 2 * NW * 4 * 4;              // int [2 NW][2]: a unit's pieces [from, to)
   static constexpr int WGT = RUNS + 2 * NW * 2 * 4;               // float [2 NW][8 NT]: a piece's weight in its unit
   static constexpr int BARS = WGT + 2 * NW * 8 * NT * 4;
@@ -342,18 +343,18 @@ __device__ __forceinline__ int kv4_row(const Kv4AttnArgs& a, int r, int& crow) {
   return crow >= 0 && crow < a.c.cache_rows ? n : 0;
 }
 
-// A place in the records of all units (row-major, then kv head): row r, head h, record blk of nb; len keys.
+// A place in the steps of all units (row-major, then kv head): row r, head h, step blk of nb; len keys.
 struct Kv4Cursor {
   int r, h, blk, nb, len;
-  const uint8_t* at;            // the record
+  const uint8_t* at;            // the step's first record
 };
 
 template <int HD>
 __device__ __forceinline__ void kv4_cursor_unit(const Kv4AttnArgs& a, Kv4Cursor& c, int crow) {
-  c.nb = (c.len + KV4_BLK - 1) / KV4_BLK;
-  c.at = kv4_rec(a.c, Kv4<HD>::REC, crow, c.h, c.blk);
+  c.nb = (c.len + KV4_STEP - 1) / KV4_STEP;
+  c.at = kv4_rec(a.c, Kv4<HD>::REC, crow, c.h, 2 * c.blk);
 }
-// On to the next unit's first record (there is one).
+// On to the next unit's first step (there is one).
 template <int HD>
 __device__ __forceinline__ void kv4_cursor_next(const Kv4AttnArgs& a, Kv4Cursor& c) {
   int crow;
@@ -371,8 +372,8 @@ __device__ __forceinline__ void kv4_cursor_next(const Kv4AttnArgs& a, Kv4Cursor&
   kv4_cursor_unit<HD>(a, c, crow);
 }
 
-// The records of all rows and kv heads form one sequence; CTA b of G takes the b-th of G equal parts of it, its warps
-// equal parts of that: the work is even whatever the lengths. A warp runs through its records alone (its own ring of bulk
+// The steps (32 positions, two records) of all rows and kv heads form one sequence; CTA b of G takes the b-th of G equal parts of it, its warps
+// equal parts of that: the work is even whatever the lengths. A warp runs through its steps alone (its own ring of bulk
 // copies, no barrier with the others) and writes the units that lie wholly in its part; what it has of the unit it begins
 // and the unit it ends within goes to shared memory, where the CTA joins its warps' pieces, and units that span CTAs are
 // joined, in order, by the CTA that comes last.
@@ -398,13 +399,13 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   if (tid < 2 * NW) meta[4 * tid] = -1;
   pdl_wait();
 
-  // ---- how many records every row has: a prefix by thread (rows in equal runs), and zeros into rows without keys
+  // ---- how many steps every row has: a prefix by thread (rows in equal runs), and zeros into rows without keys
   const int run = (a.rows + NTHR - 1) / NTHR;
   int mine = 0;
   for (int r = tid * run; r < min(a.rows, (tid + 1) * run); ++r) {
     int crow;
     const int n = kv4_row(a, r, crow);
-    mine += (n + KV4_BLK - 1) / KV4_BLK;
+    mine += (n + KV4_STEP - 1) / KV4_STEP;
     if (n == 0 && r % gridDim.x == blockIdx.x) {
       if (a.lens[r] > 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_ATTN, r);
       uint4* o = reinterpret_cast<uint4*>(a.out + (size_t)r * a.out_stride);
@@ -419,31 +420,33 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   }
   if (lane == 31) s_sum[warp] = inc;
   __syncthreads();
-  int below = 0, total = 0;
-  for (int w = 0; w < NW; ++w) {
-    if (w < warp) below += s_sum[w];
-    total += s_sum[w];
+  int sums = lane < NW ? s_sum[lane] : 0;
+#pragma unroll
+  for (int k = 1; k < 32; k <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, sums, k);
+    if (lane >= k) sums += up;
   }
-  pre[tid] = below + inc - mine;
+  const int total = __shfl_sync(0xffffffffu, sums, 31), upto = __shfl_sync(0xffffffffu, sums, warp);
+  pre[tid] = upto - s_sum[warp] + inc - mine;
   if (tid == 0) pre[NTHR] = total;
   __syncthreads();
-  const int T = total * a.c.nkv;                       // records of all units
-  const int ctas = min((int)gridDim.x, (T + KV4_CTA_RECS - 1) / KV4_CTA_RECS);
+  const int T = total * a.c.nkv;                       // steps of all units
+  const int ctas = min((int)gridDim.x, (T + KV4_CTA_STEPS - 1) / KV4_CTA_STEPS);
   if ((int)blockIdx.x >= ctas) return;
-  // the row that holds record x: its first record (at) and its records a head (nb)
+  // the row that holds step x: its first step (at) and its steps a head (nb)
   auto locate = [&](int x, int& at, int& nb) {
-    int lo = 0, hi = NTHR - 1;                         // the last thread whose rows begin at or before x
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (pre[mid] * a.c.nkv <= x) lo = mid; else hi = mid - 1;
-    }
+    // the last thread whose rows begin at or before x, the warp looking together: every NW-th, then the NW of one
+    uint32_t le = __ballot_sync(0xffffffffu, pre[lane * NW] * a.c.nkv <= x);
+    int lo = (31 - __clz(le)) * NW;
+    le = __ballot_sync(0xffffffffu, lane < NW && pre[lo + min(lane, NW - 1)] * a.c.nkv <= x);
+    lo += 31 - __clz(le);
     int r = lo * run;
     at = pre[lo] * a.c.nkv;
     nb = pre[lo + 1] - pre[lo];
     if (run > 1)
       for (;; ++r) {
         int crow;
-        nb = (kv4_row(a, r, crow) + KV4_BLK - 1) / KV4_BLK;
+        nb = (kv4_row(a, r, crow) + KV4_STEP - 1) / KV4_STEP;
         if (at + nb * a.c.nkv > x) break;
         at += nb * a.c.nkv;
       }
@@ -479,18 +482,19 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     int issued = 0;
     auto issue = [&](int s) {
       if (lane == 0) {
-        mbar_arrive_expect_tx(&full[s], F::REC);
-        bulk_load(ring + s * F::REC, pc.at, F::REC, &full[s]);
+        const uint32_t bytes = (pc.len - pc.blk * KV4_STEP > KV4_BLK ? 2 : 1) * F::REC;
+        mbar_arrive_expect_tx(&full[s], bytes);
+        bulk_load(ring + s * 2 * F::REC, pc.at, bytes, &full[s]);
       }
       ++issued;
-      pc.at += F::REC;
+      pc.at += 2 * F::REC;
       if (++pc.blk == pc.nb && issued < n) kv4_cursor_next<HD>(a, pc);
     };
     for (int s = 0; s < NST && s < n; ++s) issue(s);
 
     uint32_t qa[G][2][2 * NT];
     float o[NT][G][2][4], m[NT], l[NT], qs[NT], off[NT][G];
-    int slot = 0, ph = 0;                              // ring position of the next record
+    int slot = 0, ph = 0;                              // ring position of the next step
     bool ok = true;
     // this lane's places in a record: K words of its key in the first half (the second: 8 positions on), scales, and V
     // words of its even and odd positions
@@ -543,12 +547,13 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
       }
     };
     // the running maximum m (in logits of base 2) moves only when a logit passes it by 2^8: p stays below 2^8
-    auto raise = [&](const float2 (&v)[NT][2]) {
+    auto raise = [&](const float2 (&v)[2][NT][2]) {
       bool over = false;
       float mx[NT];
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
-        mx[u] = fmaxf(fmaxf(v[u][0].x, v[u][0].y), fmaxf(v[u][1].x, v[u][1].y)) * qs[u];
+        mx[u] = fmaxf(fmaxf(fmaxf(v[0][u][0].x, v[0][u][0].y), fmaxf(v[0][u][1].x, v[0][u][1].y)),
+                      fmaxf(fmaxf(v[1][u][0].x, v[1][u][0].y), fmaxf(v[1][u][1].x, v[1][u][1].y))) * qs[u];
         over = over || mx[u] > m[u] + KV4_LAZY;
       }
       if (__any_sync(0xffffffffu, over)) {
@@ -573,9 +578,8 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
         }
       }
     };
-    // O^T += V^T P^T of a record; CUT: only its first `left` positions count
-    auto values = [&](auto cut, const uint8_t* rec, float2 (&v)[NT][2], int left) {
-      constexpr bool CUT = decltype(cut)::value;
+    // O^T += V^T P^T of a record's first `keys` positions
+    auto values = [&](const uint8_t* rec, float2 (&v)[NT][2], int keys) {
 #pragma unroll
       for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -595,10 +599,10 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
         const uint4 y = *reinterpret_cast<const uint4*>(rec + sc0 + F::VS0);
         vs[0][0] = y.x; vs[1][0] = y.y; vs[2][0] = y.z; vs[3][0] = y.w;
       }
-      if constexpr (CUT) {
+      if (keys < KV4_BLK) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (4 * k + ((k & 1) ? t ^ 3 : t) >= left)
+          if (4 * k + ((k & 1) ? t ^ 3 : t) >= keys)
 #pragma unroll
             for (int s = 0; s < G / 2; ++s) vs[k][s] = 0u;
       }
@@ -643,7 +647,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     };
 
     for (int i = 0; i < n && ok;) {
-      // ---- a segment: the warp's records of one unit. The query heads as fp16: scaled by a power of two so that the
+      // ---- a segment: the warp's steps of one unit. The query heads as fp16: scaled by a power of two so that the
       // largest is in [2^7, 2^8) (exact down to 2^-18 of it), every other dim divided by 16 against its 16 u, and what
       // the offsets of the codes add up to in each group
       const int first = cc.blk, seg = min(cc.nb - cc.blk, n - i);
@@ -686,43 +690,30 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
           for (int k = 0; k < 2; ++k) o[u][s][k][0] = o[u][s][k][1] = o[u][s][k][2] = o[u][s][k][3] = 0.f;
         }
       }
-      // the scores of a record are formed while the values of the one before are gathered: two independent streams
-      const int left = cc.len - (first + seg - 1) * KV4_BLK;           // keys of the segment's last record
-      if (!(ok = arrived())) break;
-      const uint8_t* rec = ring + slot * F::REC;
-      float2 v[NT][2];
-      scores(rec, v);
-      int here = slot;
-      step();
-      for (int j = 1; j < seg; ++j) {
-        raise(v);
+      int keys = cc.len - first * KV4_STEP;              // of the unit from this step on
+      for (int j = 0; j < seg; ++j, keys -= KV4_STEP) {
         if (!(ok = arrived())) break;
-        const uint8_t* next = ring + slot * F::REC;
-        float2 w[NT][2];
-        scores(next, w);
-        values(std::false_type(), rec, v, KV4_BLK);
-        __syncwarp();
-        if (issued < n) issue(here);
-        here = slot;
-        step();
-        rec = next;
+        const uint8_t* rec = ring + slot * 2 * F::REC;
+        float2 v[2][NT][2];
+        scores(rec, v[0]);
+        scores(rec + F::REC, v[1]);
+        if (keys < KV4_STEP) {
+          // past the row's end: whatever the records hold there (their scales may be NaN) counts for nothing
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          v[u][0] = w[u][0];
-          v[u][1] = w[u][1];
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (r * KV4_BLK + 4 * k + ((k & 1) ? t ^ 3 : t) >= keys)
+#pragma unroll
+                for (int u = 0; u < NT; ++u) ((k & 1) ? v[r][u][k >> 1].y : v[r][u][k >> 1].x) = -INFINITY;
         }
+        raise(v);
+        values(rec, v[0], keys);
+        values(rec + F::REC, v[1], keys - KV4_BLK);
+        __syncwarp();
+        if (issued < n) issue(slot);
+        step();
       }
-      if (!ok) break;
-      // past the row's end: whatever the record holds there (its scales may be NaN) counts for nothing
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (4 * k + ((k & 1) ? t ^ 3 : t) >= left)
-#pragma unroll
-          for (int u = 0; u < NT; ++u) ((k & 1) ? v[u][k >> 1].y : v[u][k >> 1].x) = -INFINITY;
-      raise(v);
-      values(std::true_type(), rec, v, left);
-      __syncwarp();
-      if (issued < n) issue(here);
       if (!ok) break;
       // ---- the segment's result: the unit's, or a piece of it
       i += seg;
@@ -762,7 +753,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
       if (!whole && lane == 0) {
         int* e = meta + 4 * (2 * warp + piece);
         e[0] = cc.r * a.c.nkv + cc.h;
-        e[1] = w0 + i - cc.blk;                        // the unit's first record, and its end
+        e[1] = w0 + i - cc.blk;                        // the unit's first step, and its end
         e[2] = e[1] + cc.nb;
       }
       if (i < n) kv4_cursor_next<HD>(a, cc);
@@ -780,19 +771,33 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   };
   constexpr int ML = 8 * NT * HD;                      // (max, sum) behind a piece's O
   if (warp == 0) {
-    const int u = lane < 2 * NW ? meta[4 * lane] : -1;
-    const uint32_t valid = __ballot_sync(0xffffffffu, u >= 0), before = (1u << lane) - 1;
-    const int prev = (valid & before) ? 31 - __clz(valid & before) : lane;
-    const int pu = __shfl_sync(0xffffffffu, u, prev);
-    const bool starts = u >= 0 && (prev == lane || pu != u);
-    const uint32_t heads = __ballot_sync(0xffffffffu, starts);
-    if (lane < 2 * NW) meta[4 * lane + 3] = __popc(heads & (before | (1u << lane))) - 1;
-    if (starts) {
-      const uint32_t later = heads & ~(before | (1u << lane));
-      runs[2 * __popc(heads & before)] = lane;
-      runs[2 * __popc(heads & before) + 1] = later ? __ffs(later) - 1 : 2 * NW;
+    static_assert(2 * NW <= 64, "");
+    uint64_t valid = 0, heads = 0;
+    bool starts[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int e = lane + 32 * k;
+      valid |= uint64_t(__ballot_sync(0xffffffffu, e < 2 * NW && meta[4 * min(e, 2 * NW - 1)] >= 0)) << (32 * k);
     }
-    if (lane == 0) s_runs = __popc(heads);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int e = lane + 32 * k;
+      const uint64_t before = valid & ((1ull << e) - 1);
+      starts[k] = (valid >> e & 1) && (before == 0 || meta[4 * (63 - __clzll(before))] != meta[4 * e]);
+      heads |= uint64_t(__ballot_sync(0xffffffffu, starts[k])) << (32 * k);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int e = lane + 32 * k;
+      if (valid >> e & 1) meta[4 * e + 3] = __popcll(heads & (2ull * (1ull << e) - 1)) - 1;
+      if (starts[k]) {
+        const uint64_t later = heads & ~(2ull * (1ull << e) - 1);
+        const int r = __popcll(heads & ((1ull << e) - 1));
+        runs[2 * r] = e;
+        runs[2 * r + 1] = later ? __ffsll(later) - 1 : 2 * NW;
+      }
+    }
+    if (lane == 0) s_runs = __popcll(heads);
   }
   __syncthreads();
   const int nruns = s_runs;
@@ -1059,10 +1064,10 @@ static int kv4_attn_args(Kv4AttnArgs* a, const A8KV4* c, int layer, const void* 
   return A8_OK;
 }
 
-// CTAs of a decode call: one an SM, fewer when the rows cannot hold enough records.
+// CTAs of a decode call: one an SM, fewer when the rows cannot hold enough steps.
 static int kv4_ctas(const A8KV4* c, int rows, int max_len) {
-  const long long recs = (long long)rows * c->nkv * ((max_len + KV4_BLK - 1) / KV4_BLK);
-  return (int)std::min<long long>(KV4_CTAS, (recs + KV4_CTA_RECS - 1) / KV4_CTA_RECS);
+  const long long steps = (long long)rows * c->nkv * ((max_len + KV4_STEP - 1) / KV4_STEP);
+  return (int)std::min<long long>(KV4_CTAS, (steps + KV4_CTA_STEPS - 1) / KV4_CTA_STEPS);
 }
 static int kv4_part(const A8KV4* c, int nq) { return (nq / c->nkv * (c->hd + 2) + 3) / 4 * 4; }
 
@@ -1093,8 +1098,8 @@ extern "C" int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_
   int rc = kv4_attn_args(&a, c, layer, q, q_stride, nq, rows, scale, out, out_stride);
   if (rc) return rc;
   if (lens == nullptr || max_len <= 0 || max_len > c->cache_len) return A8_ERR_ARG;
-  // the records of all rows are counted in 32 bits
-  if (rows > (1 << 24) || (long long)rows * c->nkv * ((max_len + KV4_BLK - 1) / KV4_BLK) >= (1ll << 31)) return A8_ERR_SIZE;
+  // the steps of all rows are counted in 32 bits
+  if (rows > (1 << 24) || (long long)rows * c->nkv * ((max_len + KV4_STEP - 1) / KV4_STEP) >= (1ll << 31)) return A8_ERR_SIZE;
   const int ctas = kv4_ctas(c, rows, max_len);
   a.part = kv4_part(c, nq);
   if (ws == nullptr || ws_floats < 2ll * ctas * a.part || counters == nullptr || n_counters < (long long)rows * c->nkv)
