@@ -281,15 +281,20 @@ constexpr float KV4_LAZY = 8.f;       // a running maximum moves when a logit pa
 
 template <int HD, int NT>
 struct Kv4DecSmem {
-  static constexpr int NW = HD == 64 ? 16 : NT == 1 ? 12 : 8;     // warps (each holds O [hd][8 NT] in registers)
-  static constexpr int NST = HD == 64 ? 4 : 3;                    // steps in flight a warp
+#ifndef KB
+#define KB 12
+#define KBS 3
+#endif
+  static constexpr int NW = HD == 64 ? 16 : NT == 1 ? KB : 8;     // warps (each holds O [hd][8 NT] in registers)
+  static constexpr int NST = HD == 64 ? 4 : NT == 1 ? KBS : 3;                    // steps in flight a warp
   static constexpr int RING = NST * 2 * Kv4<HD>::REC;
   static constexpr int PART = (8 * NT * HD + 16 * NT) * 4;        // bytes: O [8 NT][hd], (max, sum) [8 NT]
   static constexpr int HEADP = NW * RING;                         // first partials; the last ones go into the rings
   static constexpr int PRE = HEADP + NW * PART;                   // prefix of the rows' steps by thread
-  static constexpr int META = PRE + (NW * 32 + 4) * 4;            // int [2 NW][4]: unit, its first and end step, run
-  static constexpr int RUNS = META + 2 * NW * 4 * 4;              // int [2 NW][2]: a unit's pieces [from, to)
-  static constexpr int WGT = RUNS + 2 * NW * 2 * 4;               // float [2 NW][8 NT]: a piece's weight in its unit
+  static constexpr int META = PRE + (NW * 32 + 4) * 4;            // int [2 NW][3]: a piece's unit, its first and end step
+  static constexpr int RUNS = META + 2 * NW * 4 * 4;              // int [2 NW] x 4: a unit's pieces [from, to); the pieces in
+                                                                  // order; their runs
+  static constexpr int WGT = RUNS + 2 * NW * 4 * 4;               // float [2 NW][8 NT]: a piece's weight in its unit
   static constexpr int BARS = WGT + 2 * NW * 8 * NT * 4;
   static constexpr int TOTAL = BARS + NW * NST * 8 + 16;
   static_assert(PART <= RING && TOTAL <= 227 * 1024 && BARS % 8 == 0, "");
@@ -388,7 +393,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   extern __shared__ __align__(128) uint8_t smem[];
   int* pre = reinterpret_cast<int*>(smem + SM::PRE);
   int* meta = reinterpret_cast<int*>(smem + SM::META);
-  __shared__ int s_sum[32], s_runs, s_last[2];
+  __shared__ int s_sum[32], s_runs, s_pieces, s_last[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::BARS) + warp * NST;
   uint8_t* ring = smem + warp * SM::RING;
@@ -402,16 +407,22 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   // ---- how many steps every row has: a prefix by thread (rows in equal runs), and zeros into rows without keys
   const int run = (a.rows + NTHR - 1) / NTHR;
   int mine = 0;
+  bool none = false;
+#pragma unroll 4
   for (int r = tid * run; r < min(a.rows, (tid + 1) * run); ++r) {
     int crow;
     const int n = kv4_row(a, r, crow);
     mine += (n + KV4_STEP - 1) / KV4_STEP;
-    if (n == 0 && r % gridDim.x == blockIdx.x) {
+    none = none || n == 0;
+  }
+  if (none)
+    for (int r = tid * run; r < min(a.rows, (tid + 1) * run); ++r) {
+      int crow;
+      if (r % gridDim.x != blockIdx.x || kv4_row(a, r, crow) != 0) continue;
       if (a.lens[r] > 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_ATTN, r);
       uint4* o = reinterpret_cast<uint4*>(a.out + (size_t)r * a.out_stride);
       for (int i = 0; i < a.nq * HD / 8; ++i) o[i] = make_uint4(0, 0, 0, 0);
     }
-  }
   int inc = mine;
 #pragma unroll
   for (int k = 1; k < 32; k <<= 1) {
@@ -764,7 +775,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   __syncthreads();
 
   // ---- join the warps' pieces of each unit, in key order: the runs of pieces of one unit, each piece's weight
-  int* runs = reinterpret_cast<int*>(smem + SM::RUNS);
+  int *runs = reinterpret_cast<int*>(smem + SM::RUNS), *list = runs + 4 * NW, *rof = list + 2 * NW;
   float* wgt = reinterpret_cast<float*>(smem + SM::WGT);
   auto piece_at = [&](int e) {
     return reinterpret_cast<const float*>((e & 1) ? smem + (e >> 1) * SM::RING : smem + SM::HEADP + (e >> 1) * SM::PART);
@@ -789,46 +800,70 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int e = lane + 32 * k;
-      if (valid >> e & 1) meta[4 * e + 3] = __popcll(heads & (2ull * (1ull << e) - 1)) - 1;
+      const uint64_t below = (1ull << e) - 1;
+      const int at = __popcll(valid & below);
+      if (valid >> e & 1) {
+        list[at] = e;
+        rof[at] = __popcll(heads & (2 * below + 1)) - 1;
+      }
       if (starts[k]) {
-        const uint64_t later = heads & ~(2ull * (1ull << e) - 1);
-        const int r = __popcll(heads & ((1ull << e) - 1));
-        runs[2 * r] = e;
-        runs[2 * r + 1] = later ? __ffsll(later) - 1 : 2 * NW;
+        const uint64_t later = heads & ~(2 * below + 1);
+        const int r = __popcll(heads & below);
+        runs[2 * r] = at;
+        runs[2 * r + 1] = later ? __popcll(valid & ((1ull << (__ffsll(later) - 1)) - 1)) : __popcll(valid);
       }
     }
-    if (lane == 0) s_runs = __popcll(heads);
+    if (lane == 0) {
+      s_runs = __popcll(heads);
+      s_pieces = __popcll(valid);
+    }
   }
   __syncthreads();
   const int nruns = s_runs;
-  for (int i = tid; i < 2 * NW * a.group; i += NTHR) {
-    const int e = i / a.group, qh = i % a.group;
-    if (meta[4 * e] < 0) continue;
-    const int k = meta[4 * e + 3];
+  for (int i = tid; i < s_pieces * a.group; i += NTHR) {
+    const int p = i / a.group, qh = i % a.group, from = runs[2 * rof[p]], to = runs[2 * rof[p] + 1];
     float M = -INFINITY;
-    for (int p = runs[2 * k]; p < runs[2 * k + 1]; ++p)
-      if (meta[4 * p] >= 0) M = fmaxf(M, piece_at(p)[ML + 2 * qh]);
-    wgt[e * 8 * NT + qh] = ex2(piece_at(e)[ML + 2 * qh] - M);
+#pragma unroll 4
+    for (int e = from; e < to; ++e) M = fmaxf(M, piece_at(list[e])[ML + 2 * qh]);
+    wgt[p * 8 * NT + qh] = ex2(piece_at(list[p])[ML + 2 * qh] - M);
   }
   __syncthreads();
   auto cta_of = [&](int x) { return int(((long long)(x + 1) * ctas - 1) / T); };    // by equal shares
   const int nel = a.group * HD / 4;                    // float4 elements of a unit
-  for (int i = tid; i < nruns * nel; i += NTHR) {
-    const int k = i / nel, el = i % nel, qh = el / (HD / 4), from = runs[2 * k], to = runs[2 * k + 1];
-    const int u = meta[4 * from], us = meta[4 * from + 1], ue = meta[4 * from + 2];
+  // few elements: 2 or 4 neighbouring lanes share one, each every 2nd or 4th piece of it
+  const int share_ = nruns * nel * 4 <= NTHR ? 4 : nruns * nel * 2 <= NTHR ? 2 : 1, part_ = tid & (share_ - 1);
+  for (int i0 = 0; i0 < nruns * nel; i0 += NTHR / share_) {
+    const int i = i0 + tid / share_;
+    const bool live = i < nruns * nel;
+    const int k = live ? i / nel : 0, el = live ? i % nel : 0, qh = el / (HD / 4), from = runs[2 * k], to = runs[2 * k + 1];
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     float L = 0.f, M = -INFINITY;
-    for (int e = from; e < to; ++e)
-      if (meta[4 * e] >= 0) {
-        const float f = wgt[e * 8 * NT + qh];
-        const float4 y = reinterpret_cast<const float4*>(piece_at(e))[el];
+    if (live) {
+#pragma unroll 4
+      for (int p = from + part_; p < to; p += share_) {
+        const float* src = piece_at(list[p]);
+        const float f = wgt[p * 8 * NT + qh];
+        const float4 y = reinterpret_cast<const float4*>(src)[el];
+        const float2 ml = *reinterpret_cast<const float2*>(src + ML + 2 * qh);
         x.x += f * y.x;
         x.y += f * y.y;
         x.z += f * y.z;
         x.w += f * y.w;
-        L += f * piece_at(e)[ML + 2 * qh + 1];
-        M = fmaxf(M, piece_at(e)[ML + 2 * qh]);
+        L += f * ml.y;
+        M = fmaxf(M, ml.x);
       }
+    }
+    for (int d = 1; d < share_; d <<= 1) {
+      x.x += __shfl_xor_sync(0xffffffffu, x.x, d);
+      x.y += __shfl_xor_sync(0xffffffffu, x.y, d);
+      x.z += __shfl_xor_sync(0xffffffffu, x.z, d);
+      x.w += __shfl_xor_sync(0xffffffffu, x.w, d);
+      L += __shfl_xor_sync(0xffffffffu, L, d);
+      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    }
+    if (!live || part_ != 0) continue;
+    const int* e = meta + 4 * list[from];
+    const int u = e[0], us = e[1], ue = e[2];
     if (us >= b0 && ue <= b1) {
       const float inv = 1.f / L;
       *reinterpret_cast<uint2*>(a.out + (size_t)(u / a.c.nkv) * a.out_stride + (u % a.c.nkv * a.group) * HD + 4 * el) =
@@ -840,7 +875,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     }
   }
   // only the first and the last run can belong to a unit that other CTAs share
-  int cut_from[2] = {nruns > 0 ? runs[0] : -1, nruns > 1 ? runs[2 * nruns - 2] : -1};
+  int cut_from[2] = {nruns > 0 ? list[runs[0]] : -1, nruns > 1 ? list[runs[2 * nruns - 2]] : -1};
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     if (cut_from[k] >= 0 && meta[4 * cut_from[k] + 1] >= b0 && meta[4 * cut_from[k] + 2] <= b1) cut_from[k] = -1;
