@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     };
     for (int s = 0; s < NST && s < n; ++s) issue(s);
 
-    uint32_t qa[G][2][2 * NT];
+    uint32_t qa[G][2][4];                              // A operands; with one tile of heads rows 8-15 repeat rows 0-7
     float o[NT][G][2][4], m[NT], l[NT], qs[NT], off[NT][G];
     int slot = 0, ph = 0;                              // ring position of the next step
     bool ok = true;
@@ -541,13 +541,9 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
 #pragma unroll
         for (int s = 0; s < G; ++s) {
           float acc[4];
-          const uint32_t a0[4] = {qa[s][0][0], NT == 2 ? qa[s][0][1] : 0u, qa[s][0][NT],
-                                  NT == 2 ? qa[s][0][2 * NT - 1] : 0u};
-          const uint32_t a1[4] = {qa[s][1][0], NT == 2 ? qa[s][1][1] : 0u, qa[s][1][NT],
-                                  NT == 2 ? qa[s][1][2 * NT - 1] : 0u};
-          mma_f16_first(acc, a0, kv4_lo16(w[s]), kv4_hi16(w[s]));
+          mma_f16_first(acc, qa[s][0], kv4_lo16(w[s]), kv4_hi16(w[s]));
           const uint32_t w8 = w[s] >> 8;
-          mma_f16(acc, a1, kv4_lo16(w8), kv4_hi16(w8));
+          mma_f16(acc, qa[s][1], kv4_lo16(w8), kv4_hi16(w8));
           const float2 sc = sf2(ks[2 * nb][s >> 1], ks[2 * nb + 1][s >> 1], s);
 #pragma unroll
           for (int u = 0; u < NT; ++u) {
@@ -589,8 +585,8 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
         }
       }
     };
-    // O^T += V^T P^T of a record's first `keys` positions
-    auto values = [&](const uint8_t* rec, float2 (&v)[NT][2], int keys) {
+    // O^T += V^T P^T of a record; CUT: only its first `keys` positions count
+    auto values = [&](auto cut, const uint8_t* rec, float2 (&v)[NT][2], int keys) {
 #pragma unroll
       for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -610,7 +606,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
         const uint4 y = *reinterpret_cast<const uint4*>(rec + sc0 + F::VS0);
         vs[0][0] = y.x; vs[1][0] = y.y; vs[2][0] = y.z; vs[3][0] = y.w;
       }
-      if (keys < KV4_BLK) {
+      if constexpr (decltype(cut)::value) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (4 * k + ((k & 1) ? t ^ 3 : t) >= keys)
@@ -687,12 +683,15 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
           const float2 d01 = unpack_bf16(x[s].x), d23 = unpack_bf16(x[s].y), d45 = unpack_bf16(x[s].z),
                        d67 = unpack_bf16(x[s].w);
           // dims (n, n + 4) of the word's eight
-          qa[s][0][u] = pack_f16(d01.x * up, d45.x * up);
-          qa[s][0][NT + u] = pack_f16(d01.y * up * 0.0625f, d45.y * up * 0.0625f);
-          qa[s][1][u] = pack_f16(d23.x * up, d67.x * up);
-          qa[s][1][NT + u] = pack_f16(d23.y * up * 0.0625f, d67.y * up * 0.0625f);
-          const float2 e0 = unpack_f16(qa[s][0][u]), e1 = unpack_f16(qa[s][1][u]), h0 = unpack_f16(qa[s][0][NT + u]),
-                       h1 = unpack_f16(qa[s][1][NT + u]);
+#pragma unroll
+          for (int w = u; w < 2; w += NT) {
+            qa[s][0][w] = pack_f16(d01.x * up, d45.x * up);
+            qa[s][0][2 + w] = pack_f16(d01.y * up * 0.0625f, d45.y * up * 0.0625f);
+            qa[s][1][w] = pack_f16(d23.x * up, d67.x * up);
+            qa[s][1][2 + w] = pack_f16(d23.y * up * 0.0625f, d67.y * up * 0.0625f);
+          }
+          const float2 e0 = unpack_f16(qa[s][0][u]), e1 = unpack_f16(qa[s][1][u]), h0 = unpack_f16(qa[s][0][2 + u]),
+                       h1 = unpack_f16(qa[s][1][2 + u]);
           float f = KV4_OFF_LO * ((e0.x + e0.y) + (e1.x + e1.y)) + KV4_OFF_HI * ((h0.x + h0.y) + (h1.x + h1.y));
           f += __shfl_xor_sync(0xffffffffu, f, 1);
           f += __shfl_xor_sync(0xffffffffu, f, 2);
@@ -701,15 +700,15 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
           for (int k = 0; k < 2; ++k) o[u][s][k][0] = o[u][s][k][1] = o[u][s][k][2] = o[u][s][k][3] = 0.f;
         }
       }
-      int keys = cc.len - first * KV4_STEP;              // of the unit from this step on
-      for (int j = 0; j < seg; ++j, keys -= KV4_STEP) {
-        if (!(ok = arrived())) break;
+      // (only the last step can hold positions past the row's end; the others are spared the masks)
+      auto one = [&](auto cut, int keys) {
+        if (!(ok = arrived())) return;
         const uint8_t* rec = ring + slot * 2 * F::REC;
         float2 v[2][NT][2];
         scores(rec, v[0]);
         scores(rec + F::REC, v[1]);
-        if (keys < KV4_STEP) {
-          // past the row's end: whatever the records hold there (their scales may be NaN) counts for nothing
+        if constexpr (decltype(cut)::value) {
+          // whatever the records hold there (their scales may be NaN) counts for nothing
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -719,12 +718,14 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
                 for (int u = 0; u < NT; ++u) ((k & 1) ? v[r][u][k >> 1].y : v[r][u][k >> 1].x) = -INFINITY;
         }
         raise(v);
-        values(rec, v[0], keys);
-        values(rec + F::REC, v[1], keys - KV4_BLK);
+        values(cut, rec, v[0], keys);
+        values(cut, rec + F::REC, v[1], keys - KV4_BLK);
         __syncwarp();
         if (issued < n) issue(slot);
         step();
-      }
+      };
+      for (int j = 1; ok && j < seg; ++j) one(std::false_type(), KV4_STEP);
+      if (ok) one(std::true_type(), cc.len - (first + seg - 1) * KV4_STEP);
       if (!ok) break;
       // ---- the segment's result: the unit's, or a piece of it
       i += seg;
