@@ -13,7 +13,9 @@ import torch
 
 from . import _lib as L
 
-BF16 = torch.bfloat16
+BF16, I32 = torch.bfloat16, torch.int32
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def _need(ok, what):
@@ -45,30 +47,39 @@ class KV4Cache:
     def nbytes(self) -> int:
         return self.buf.numel()
 
-    # ---- argument checks (host side, nothing launched by a refused call)
+    # ---- argument checks: on the host, before anything is launched, and kept lean (a decode step's kernel takes a few
+    # microseconds, a check a tenth of one; the C entry points check shapes, strides and alignment again)
     def _rows(self, t, rows, width, what):
-        shape = t.shape
-        if not (len(shape) == 2 and t.dtype is BF16 and t.device == self.dev and shape[0] >= rows and shape[1] >= width):
-            _need(False, f"{what}: bf16 rows of at least {width} on {self.dev}, at least {rows} of them")
-        ld, one = t.stride()
-        _need(one == 1, f"{what}: contiguous rows")
+        """Row stride of bf16 rows [>= rows, >= width]."""
+        shape, (ld, one) = t.shape, t.stride() if t.dim() == 2 else (0, 0)
+        if one != 1 or t.dtype is not BF16 or t.device != self.dev or shape[0] < rows or shape[1] < width:
+            _need(False, f"{what}: bf16 [at least {rows}, at least {width}] on {self.dev}, rows contiguous")
         # (the row stride of a single row means nothing: torch may give it any value)
         return ld if shape[0] > 1 else max(ld, shape[1])
 
+    def _heads(self, t, rows, what):
+        """Row stride of bf16 [>= rows, nkv, hd] with contiguous heads."""
+        _need(t.dtype is BF16 and t.device == self.dev and t.dim() == 3 and t.shape[0] >= rows
+              and t.shape[1:] == (self.nkv, self.hd) and t.stride(2) == 1
+              and (self.nkv == 1 or t.stride(1) == self.hd),
+              f"{what}: bf16 [at least {rows}, {self.nkv}, {self.hd}] on {self.dev}, heads contiguous")
+        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), self.nkv * self.hd)
+
     def _ints(self, t, n, what):
-        if not (t.dtype is torch.int32 and t.device == self.dev and t.is_contiguous() and t.numel() >= n):
+        if t.dtype is not I32 or t.device != self.dev or not t.is_contiguous() or t.numel() < n:
             _need(False, f"{what}: {n} contiguous int32 on {self.dev}")
         return t.data_ptr()
 
     def _call(self, fn, *args):
-        # (kept lean: a decode step is a few microseconds on the GPU)
+        """fn(cache, *args, the current stream of the cache's device)."""
         dev = self.dev.index
-        _need(dev is not None, "the cache is not on a GPU (there is no CPU fallback)")
-        if dev == torch._C._cuda_getDevice():
-            rc = fn(self._ref, *args, torch._C._cuda_getCurrentRawStream(dev))
+        if dev is None:
+            _need(False, "the cache is not on a GPU (there is no CPU fallback)")
+        if dev == _current_device():
+            rc = fn(self._ref, *args, _current_stream(dev))
         else:
             with torch.cuda.device(dev):
-                rc = fn(self._ref, *args, torch._C._cuda_getCurrentRawStream(dev))
+                rc = fn(self._ref, *args, _current_stream(dev))
         if rc:
             L.check(rc, fn.__name__)
 
@@ -78,46 +89,52 @@ class KV4Cache:
         rows slot (int32, None: the row index); with cos / sin [npos, hd] q and k are rotated (rotate_half). Returns the
         query heads [rows, nq hd]: `q` if given (it may be qkv), else a new tensor (None with nq = 0); padding rows of it
         are not written."""
-        rows, w = pos.numel(), (nq + 2 * self.nkv) * self.hd
-        ld = self._rows(qkv, rows, w, "qkv")
-        npos = 0
-        if cos is not None:
-            _need(sin is not None and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == self.hd
-                  and cos.dtype == sin.dtype == BF16 and cos.is_contiguous() and sin.is_contiguous()
-                  and cos.device == sin.device == self.dev, f"cos, sin: two contiguous bf16 [npos, {self.hd}] tables")
+        rows, hd = pos.numel(), self.hd
+        ld = self._rows(qkv, rows, (nq + 2 * self.nkv) * hd, "qkv")
+        ppos = self._ints(pos, rows, "pos")
+        pslot = None if slot is None else self._ints(slot, rows, "slot")
+        npos = pcos = psin = None
+        if cos is not None and sin is not None:
             npos = cos.shape[0]
+            if (cos.dtype is not BF16 or sin.dtype is not BF16 or cos.shape != (npos, hd) or sin.shape != (npos, hd)
+                    or not cos.is_contiguous() or not sin.is_contiguous() or cos.device != self.dev
+                    or sin.device != self.dev):
+                _need(False, f"cos, sin: two contiguous bf16 [npos, {hd}] tables on {self.dev}")
+            pcos, psin = cos.data_ptr(), sin.data_ptr()
         else:
-            _need(sin is None, "sin without cos")
-        if nq > 0 and q is None:
-            q = torch.empty(rows, nq * self.hd, dtype=BF16, device=self.dev)
-        ldq = self._rows(q, rows, nq * self.hd, "q") if nq > 0 else 0
+            _need(cos is None and sin is None, "cos and sin come together")
+        ldq = pq = None
+        if nq > 0:
+            if q is None:
+                ldq = nq * hd
+                q = torch.empty(rows, ldq, dtype=BF16, device=self.dev)
+            else:
+                ldq = self._rows(q, rows, nq * hd, "q")
+            pq = q.data_ptr()
         if rows:
-            self._call(self._lib.a8_kv4_store, layer, qkv.data_ptr(), ld, nq, None if cos is None else cos.data_ptr(),
-                       None if sin is None else sin.data_ptr(), npos, self._ints(pos, rows, "pos"),
-                       None if slot is None else self._ints(slot, rows, "slot"), rows, ring,
-                       q.data_ptr() if nq > 0 else None, ldq)
+            self._call(self._lib.a8_kv4_store, layer, qkv.data_ptr(), ld, nq, pcos, psin, npos or 0, ppos, pslot, rows,
+                       ring, pq, ldq or 0)
         return q if nq > 0 else None
 
     def load(self, pos, slot=None, *, layer: int = 0, k=None, v=None):
         """(k, v) bf16 [rows, nkv, hd] at positions pos of cache rows slot (None: the row index): code * scale, rounded
-        once. Given tensors are written in place; rows with a negative position are left as they are (zero in new
-        tensors only by chance)."""
+        once. Given tensors are written in place; rows with a negative position are left as they are (undefined in new
+        tensors)."""
         rows = pos.numel()
-        new = lambda: torch.empty(rows, self.nkv, self.hd, dtype=BF16, device=self.dev)
-        k, v = new() if k is None else k, new() if v is None else v
-        ld = [self._heads(t, rows, n) for t, n in ((k, "k"), (v, "v"))]
+        ppos = self._ints(pos, rows, "pos")
+        pslot = None if slot is None else self._ints(slot, rows, "slot")
+        ldk = ldv = self.nkv * self.hd
+        if k is None:
+            k = torch.empty(rows, self.nkv, self.hd, dtype=BF16, device=self.dev)
+        else:
+            ldk = self._heads(k, rows, "k")
+        if v is None:
+            v = torch.empty(rows, self.nkv, self.hd, dtype=BF16, device=self.dev)
+        else:
+            ldv = self._heads(v, rows, "v")
         if rows:
-            self._call(self._lib.a8_kv4_load, layer, self._ints(pos, rows, "pos"),
-                       None if slot is None else self._ints(slot, rows, "slot"), rows, k.data_ptr(), ld[0],
-                       v.data_ptr(), ld[1])
+            self._call(self._lib.a8_kv4_load, layer, ppos, pslot, rows, k.data_ptr(), ldk, v.data_ptr(), ldv)
         return k, v
-
-    def _heads(self, t, rows, what):
-        _need(t.dtype == BF16 and t.device == self.dev and t.dim() == 3 and t.shape[0] >= rows
-              and t.shape[1:] == (self.nkv, self.hd) and t.stride(2) == 1
-              and (self.nkv == 1 or t.stride(1) == self.hd),
-              f"{what}: bf16 [at least {rows}, {self.nkv}, {self.hd}] on {self.dev}, heads contiguous")
-        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), self.nkv * self.hd)
 
     def workspace(self, nq: int, rows: int, max_len: int):
         """A workspace (partials, tickets) for `attention` calls up to these sizes; one call at a time uses it."""
@@ -131,12 +148,13 @@ class KV4Cache:
         # Calls on one stream run one after another and share a workspace; every other stream has its own. A captured
         # call gets one of its own inside the graph's memory (cleared by the graph): replays of two graphs may overlap.
         dev = self.dev.index
-        _need(dev is not None, "the cache is not on a GPU (there is no CPU fallback)")
-        if torch._C._cuda_isCurrentStreamCapturing():
-            return self.workspace(nq, rows, max_len)
-        key = torch._C._cuda_getCurrentRawStream(dev)
+        if dev is None:
+            _need(False, "the cache is not on a GPU (there is no CPU fallback)")
+        key = _current_stream(dev)
         have = self._ws.get(key)
-        if have is None or nq > have[0] or rows > have[1] or max_len > have[2]:
+        if have is None or nq > have[0] or rows > have[1] or max_len > have[2] or _capturing():
+            if _capturing():
+                return self.workspace(nq, rows, max_len)
             if have is not None:
                 nq, rows, max_len = max(nq, have[0]), max(rows, have[1]), max(max_len, have[2])
             with torch.cuda.device(self.dev):
@@ -147,31 +165,36 @@ class KV4Cache:
         """Decode attention: q bf16 [rows, nq hd], row r over keys [0, min(lens[r], max_len)) of cache row rowmap[r]
         (None: r); an empty row gives zeros. max_len bounds every row's keys (0: cache_len). Returns bf16 [rows, nq hd].
         ws: a `workspace()` of the caller's (None: the stream's own)."""
-        rows, nq = q.shape[0], q.shape[1] // self.hd
-        _need(q.shape[1] % self.hd == 0, f"q: heads of {self.hd}")
+        nq, ldq, ldo, out = self._queries(q, out)
+        rows = q.shape[0]
         max_len = max_len or self.cache_len
-        if out is None:
-            out = torch.empty(rows, nq * self.hd, dtype=BF16, device=self.dev)
-        ldq, ldo = self._rows(q, rows, nq * self.hd, "q"), self._rows(out, rows, nq * self.hd, "out")
         plens = self._ints(lens, rows, "lens")           # (the tensors stay referenced until the launch)
         pmap = None if rowmap is None else self._ints(rowmap, rows, "rowmap")
         if rows:
             w, t = ws if ws is not None else self._workspace(nq, rows, max_len)
-            self._call(self._lib.a8_kv4_attention, layer, q.data_ptr(), ldq, nq, plens, pmap, rows, max_len, float(scale),
+            self._call(self._lib.a8_kv4_attention, layer, q.data_ptr(), ldq, nq, plens, pmap, rows, max_len, scale,
                        out.data_ptr(), ldo, w.data_ptr(), w.numel(), t.data_ptr(), t.numel())
         return out
+
+    def _queries(self, q, out):
+        """(nq, row stride of q, of out, out) of q [rows, nq hd]."""
+        rows, width = q.shape if q.dim() == 2 else (0, -1)
+        if width < 0 or width % self.hd:
+            _need(False, f"q: [rows, heads of {self.hd}]")
+        ldq = self._rows(q, rows, width, "q")
+        if out is None:
+            return width // self.hd, ldq, width, torch.empty(rows, width, dtype=BF16, device=self.dev)
+        return width // self.hd, ldq, self._rows(out, rows, width, "out"), out
 
     def prefill_attention(self, q, blocks, *, layer: int = 0, scale: float = 0.0, out=None):
         """Packed causal attention: q bf16 [rows, nq hd], blocks int32 [n, 4] = (q0, n, slot, pos0) on the device (the
         rows of `FastEngine.query_blocks`). Rows that no block covers are left as they are. Returns bf16 [rows, nq hd]."""
-        rows, nq = q.shape[0], q.shape[1] // self.hd
-        _need(q.shape[1] % self.hd == 0, f"q: heads of {self.hd}")
+        nq, ldq, ldo, out = self._queries(q, out)
+        rows = q.shape[0]
         _need(blocks.dim() == 2 and blocks.shape[1] == 4, "blocks: int32 [n, 4]")
-        if out is None:
-            out = torch.empty(rows, nq * self.hd, dtype=BF16, device=self.dev)
-        ldq, ldo = self._rows(q, rows, nq * self.hd, "q"), self._rows(out, rows, nq * self.hd, "out")
-        if rows and blocks.shape[0]:
-            self._call(self._lib.a8_kv4_prefill_attention, layer, q.data_ptr(), ldq, nq,
-                       self._ints(blocks, blocks.numel(), "blocks"), blocks.shape[0], rows, float(scale),
+        n = blocks.shape[0]
+        pblocks = self._ints(blocks, 4 * n, "blocks")
+        if rows and n:
+            self._call(self._lib.a8_kv4_prefill_attention, layer, q.data_ptr(), ldq, nq, pblocks, n, rows, scale,
                        out.data_ptr(), ldo)
         return out
