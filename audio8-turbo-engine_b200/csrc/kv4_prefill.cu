@@ -21,7 +21,7 @@ namespace a8 {
 constexpr int KERNEL_ID_KV4_PREFILL = 12;
 constexpr int KV4P_SOFT = 8, KV4P_DEQ = 4;               // softmax warps; warps of each of K and V
 constexpr int KV4P_THREADS = (KV4P_SOFT + 2 * KV4P_DEQ + 4) * 32;   // five warpgroups (the last: warps 16, 17 and two idle)
-// Registers a thread after the warpgroups' redistribution: 256 x 136 + 256 x 72 + 128 x 64, all of the 640 x 96 = 61,440
+// Registers a thread after the warpgroups' redistribution: 256 x 144 + 256 x 64 + 128 x 64, all of the 640 x 96 = 61,440
 // that the block is launched with.
 #define A8_SETMAXNREG(op, n) asm volatile("setmaxnreg." op ".sync.aligned.u32 %0;" ::"n"(n))
 constexpr int KV4P_RAW = 6;                              // raw key tiles in flight
@@ -38,8 +38,9 @@ struct Kv4PreSmem {
   static constexpr int VT = HD * 128;
   static constexpr int RAW = V + KV4P_VST * VT;
   static constexpr int RAWT = 4 * Kv4<HD>::REC;
-  static constexpr int SCV = RAW + KV4P_RAW * RAWT;      // fp16 [4 warps][G / 2][64 keys]: V scales of the tile, divided
-  static constexpr int MISC = SCV + 4 * 64 * (HD / 64) * 2;  // int ek[16], ev[16], nanv[4]
+  static constexpr int SC = RAW + KV4P_RAW * RAWT;       // a raw tile's scales as fp16, divided: K [64 keys][G], V [G][64 keys]
+  static constexpr int SCT = 2 * 64 * (HD / 32) * 2;
+  static constexpr int MISC = SC + KV4P_RAW * SCT;       // int ek[16], ev[16], nanv[4]
   static constexpr int BARS = MISC + 144;
   static constexpr int TOTAL = BARS + 40 * 8 + 16 + 1024;
   static constexpr uint32_t COLS = 512;                  // TMEM: S of tile 0 and 1, two stages of 64 each (P takes
@@ -58,6 +59,28 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
       "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// 64 columns at once
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) {
+  uint32_t r[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+      "%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,"
+      "%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // D += A B with A (128 rows x 16 fp16, two a column) in tensor memory, B in shared memory
@@ -154,7 +177,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
   const uint32_t tmem = *tmem_slot;
 
   if (warp < KV4P_SOFT) {
-    A8_SETMAXNREG("inc", 136);
+    A8_SETMAXNREG("inc", 144);
     // ---- softmax: thread = query vector (head 2 x + half, position pos0 + r)
     const int x = warp >> 2, row = (warp & 3) * 32 + lane, r = row & 63, hi = row >> 6;
     const int head = 2 * x + hi;
@@ -197,8 +220,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       if (!(ok = mbar_wait_all(&s_full[b], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
       tc_fence_after();
       float sv[64];
-      tmem_ld32(tS + (j & 1) * 64, sv);
-      tmem_ld32(tS + (j & 1) * 64 + 32, sv + 32);
+      tmem_ld64(tS + (j & 1) * 64, sv);
       const float f = qs * pow2_biased(ek[j & 15]);
       const int Ej = ev[j & 15];
       const int kmax = pos - 64 * j;                     // keys c <= kmax of this tile are causal for this row
@@ -206,50 +228,62 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
 #pragma unroll
         for (int c = 0; c < 64; ++c) sv[c] = c <= kmax ? sv[c] : -INFINITY;
       }
-      float m4[4] = {sv[0], sv[1], sv[2], sv[3]};
+      // The weights are formed against the maximum at hand; only where their sum says that one may pass fp16's range (or in
+      // the first tile, or when E grows) is the tile's own maximum looked for, the running maximum moved where a logit
+      // passes it by 2^8, and the weights formed again.
+      bool full = __any_sync(0xffffffffu, j == 0 || Ej > E);
+      uint32_t pk[32];
+      float sum;
+      for (;;) {
+        if (full) {
+          float m4[4] = {sv[0], sv[1], sv[2], sv[3]};
 #pragma unroll
-      for (int c = 4; c < 60; c += 8)
+          for (int c = 4; c < 60; c += 8)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) m4[k] = fmaxf(fmaxf(m4[k], sv[c + k]), sv[c + 4 + k]);
+            for (int k = 0; k < 4; ++k) m4[k] = fmaxf(fmaxf(m4[k], sv[c + k]), sv[c + 4 + k]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], sv[60 + k]);
-      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
-      if (__any_sync(0xffffffffu, mx > m + 8.f || Ej > E)) {
-        const float nm = mx > m + 8.f ? mx : m;
-        const float al = m == -INFINITY ? 0.f : ex2(m - nm);
-        l *= al;
-        m = nm;
-        if (j > 0) {
-          // O is at rest once the previous tile's product is complete: scale it in place
-          const float oa = al * (Ej > E ? pow2_biased(max(127 + E - Ej, 0)) : 1.f);
-          if (!(ok = mbar_wait_all(&p_free[(j - 1) & 1], ((j - 1) >> 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL))) break;
-          tc_fence_after();
+          for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], sv[60 + k]);
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
+          const float nm = mx > m + 8.f ? mx : m;
+          const float al = m == -INFINITY ? 0.f : ex2(m - nm);
+          l *= al;
+          m = nm;
+          if (j > 0) {
+            // O is at rest once the previous tile's product is complete: scale it in place
+            const float oa = al * (Ej > E ? pow2_biased(max(127 + E - Ej, 0)) : 1.f);
+            if (!(ok = mbar_wait_all(&p_free[(j - 1) & 1], ((j - 1) >> 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL)))
+              break;
+            tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            float ov[32];
-            tmem_ld32(tO + c, ov);
+            for (int c = 0; c < HD; c += 32) {
+              float ov[32];
+              tmem_ld32(tO + c, ov);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) ov[k] *= oa;
-            tmem_st32(tO + c, ov);
+              for (int k = 0; k < 32; ++k) ov[k] *= oa;
+              tmem_st32(tO + c, ov);
+            }
+          }
+          E = max(E, Ej);
+        }
+        const float2 f_2 = f2(f), mb = f2(KV4P_BIAS - m);
+        float2 ls[2] = {f2(0.f), f2(0.f)};
+#pragma unroll
+        for (int c = 0; c < 64; c += 8) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 z = ffma2(make_float2(sv[c + 2 * k], sv[c + 2 * k + 1]), f_2, mb);
+            const float2 p = make_float2(ex2(z.x), ex2(z.y));
+            ls[k & 1] = fadd2(ls[k & 1], p);
+            pk[c / 2 + k] = pack_f16(p.x, p.y);
           }
         }
-        E = max(E, Ej);
+        sum = (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
+        if (full || !__any_sync(0xffffffffu, sum > 32768.f)) break;
+        full = true;
       }
-      const float2 f_2 = f2(f), mb = f2(KV4P_BIAS - m);
-      float2 ls[2] = {f2(0.f), f2(0.f)};
-      uint32_t pk[32];
-#pragma unroll
-      for (int c = 0; c < 64; c += 8) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 z = ffma2(make_float2(sv[c + 2 * k], sv[c + 2 * k + 1]), f_2, mb);
-          const float2 p = make_float2(ex2(z.x), ex2(z.y));
-          ls[k & 1] = fadd2(ls[k & 1], p);
-          pk[c / 2 + k] = pack_f16(p.x, p.y);
-        }
-      }
+      if (!ok) break;
       tmem_st32(tS + (j & 1) * 64, reinterpret_cast<const float*>(pk));
-      l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
+      l += sum;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[j & 1]);
@@ -276,7 +310,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       }
     }
   } else if (warp < KV4P_SOFT + 2 * KV4P_DEQ) {
-    A8_SETMAXNREG("dec", 72);
+    A8_SETMAXNREG("dec", 64);
     // ---- codes to fp16: 128 threads for K, 128 for V
     const bool isv = warp >= KV4P_SOFT + KV4P_DEQ;
     const int dw = (warp - KV4P_SOFT) & 3, dt = dw * 32 + lane;
@@ -284,8 +318,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       const int rs = j % KV4P_RAW, st = j & 1, rph = (j / KV4P_RAW) & 1;
       if (!kv4_wait2(&raw_full[rs], rph, &e_full[rs], rph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL)) break;
       const uint8_t* raw = smem + SM::RAW + rs * SM::RAWT;
-      const int left = klen - 64 * j;                    // positions of the tile that hold keys
-      const float down = pow2_biased_inv(isv ? ev[j & 15] : ek[j & 15]);
+      const __half* table = reinterpret_cast<const __half*>(smem + SM::SC + rs * SM::SCT) + (isv ? 64 * G : 0);
       if (!isv) {
         if (j >= 2 && !mbar_wait_all(&k_free[st], ((j >> 1) - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL)) break;
         uint8_t* dst = smem + SM::K + st * SM::KT;
@@ -297,21 +330,18 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
           if constexpr (G == 4) {
             const uint4 u = *reinterpret_cast<const uint4*>(src);
             w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-            const uint2 v = *reinterpret_cast<const uint2*>(raw + (r >> 4) * F::REC + F::KS0 + F::scale(r & 15, 0));
+            const uint2 v = *reinterpret_cast<const uint2*>(table + r * G);
             ks[0] = v.x; ks[1] = v.y;
           } else {
             const uint2 u = *reinterpret_cast<const uint2*>(src);
             w[0] = u.x; w[1] = u.y;
-            ks[0] = *reinterpret_cast<const uint32_t*>(raw + (r >> 4) * F::REC + F::KS0 + F::scale(r & 15, 0));
+            ks[0] = *reinterpret_cast<const uint32_t*>(table + r * G);
           }
-          if (r >= left)
-#pragma unroll
-            for (int s = 0; s < G / 2; ++s) ks[s] = 0;
 #pragma unroll
           for (int s = 0; s < G; ++s) {
             const int grp = (s & 1) * (G / 2) + s / 2;
-            const __half2 h =
-                __float2half2_rn(__uint_as_float((s & 1) ? ks[s >> 1] & 0xFFFF0000u : ks[s >> 1] << 16) * down);
+            const uint32_t hb = __byte_perm(ks[s >> 1], 0, (s & 1) ? 0x3232 : 0x1010);
+            const __half2 h = *reinterpret_cast<const __half2*>(&hb);
             __half2 c[4];
             kv4_codes_f16(w[s], c);
             *reinterpret_cast<uint4*>(dst + (grp >> 1) * 8192 + sw128(r, (grp & 1) * 4 + t8)) =
@@ -325,37 +355,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
           mbar_arrive(&raw_free[rs]);
         }
       } else {
-        // this warp's half of the groups, their scales as fp16 divided by 2^E: [slot][key] (two keys a lane)
-        const int part = dw >> 1;
-        __half* table = reinterpret_cast<__half*>(smem + SM::SCV) + dw * (G / 2) * 64;
-        {
-          uint32_t sc[2][G / 2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int key = 2 * lane + k;
-            const uint8_t* p = raw + (key >> 4) * F::REC + F::VS0 + F::scale(key & 15, part * (G / 2));
-            if constexpr (G == 4) {
-              const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-              sc[k][0] = w & 0xFFFFu;
-              sc[k][1] = w >> 16;
-            } else {
-              sc[k][0] = *reinterpret_cast<const uint16_t*>(p);
-            }
-#pragma unroll
-            for (int s = 0; s < G / 2; ++s) {
-              if (key >= left) sc[k][s] = 0;
-              if (sc[k][s] >= 0x7F80u) {                 // NaN: counts as zero here and is put back at the end
-                atomicMin(&nanv[part * (G / 2) + s], 64 * j + key);
-                sc[k][s] = 0;
-              }
-            }
-          }
-#pragma unroll
-          for (int s = 0; s < G / 2; ++s)
-            *reinterpret_cast<uint32_t*>(table + s * 64 + 2 * lane) =
-                pack_f16(__uint_as_float(sc[0][s] << 16) * down, __uint_as_float(sc[1][s] << 16) * down);
-          __syncwarp();
-        }
+        const int part = dw >> 1;                        // this warp's half of the groups
         const int vt = j % KV4P_VST;
         if (j >= KV4P_VST && !mbar_wait_all(&v_free[vt], (j / KV4P_VST - 1) & 1, ERR_TIMEOUT_EMPTY, KERNEL_ID_KV4_PREFILL))
           break;
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
 #pragma unroll
         for (int sl = 0; sl < G / 2; ++sl) {
           const int s = part * (G / 2) + sl, grp = (s & 1) * (G / 2) + s / 2;
-          const uint4 hs = *reinterpret_cast<const uint4*>(table + sl * 64 + oct * 8);
+          const uint4 hs = *reinterpret_cast<const uint4*>(table + s * 64 + oct * 8);
           const uint32_t hp[4] = {hs.x, hs.y, hs.z, hs.w};
           uint32_t o[4][4];
 #pragma unroll
@@ -497,6 +497,36 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
         };
         E = max(largest(F::VS0), E);
         const int ex = largest(F::KS0);
+        // the scales as fp16, K's divided by 2^ek, V's by 2^E (two positions a lane); none behind the last key
+        __half* tk = reinterpret_cast<__half*>(smem + SM::SC + rs * SM::SCT);
+        __half* tv = tk + 64 * G;
+        const float dk = pow2_biased_inv(ex), dv = pow2_biased_inv(E);
+        float vsc[2][G];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int key = 2 * lane + k;
+          const uint8_t* p = raw + (key >> 4) * F::REC + F::scale(key & 15, 0);
+          uint32_t kw[G / 2], vw[G / 2], h[G / 2];
+#pragma unroll
+          for (int i = 0; i < G / 2; ++i) {
+            kw[i] = key < left ? *reinterpret_cast<const uint32_t*>(p + F::KS0 + 4 * i) : 0u;
+            vw[i] = key < left ? *reinterpret_cast<const uint32_t*>(p + F::VS0 + 4 * i) : 0u;
+            h[i] = pack_f16(__uint_as_float(kw[i] << 16) * dk, __uint_as_float(kw[i] & 0xFFFF0000u) * dk);
+            *reinterpret_cast<uint32_t*>(tk + key * G + 2 * i) = h[i];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t sc = e ? vw[i] & 0xFFFF0000u : vw[i] << 16;
+              if (sc >= 0x7F800000u) {                   // NaN: counts as zero here and is put back at the end
+                atomicMin(&nanv[2 * i + e], 64 * j + key);
+                sc = 0;
+              }
+              vsc[k][2 * i + e] = __uint_as_float(sc) * dv;
+            }
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < G; ++s) *reinterpret_cast<uint32_t*>(tv + s * 64 + 2 * lane) = pack_f16(vsc[0][s], vsc[1][s]);
+        __syncwarp();
         if (lane == 0) {
           ek[j & 15] = ex;
           ev[j & 15] = E;
