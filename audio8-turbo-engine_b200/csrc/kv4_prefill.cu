@@ -467,65 +467,85 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
         }
       }
     } else if (warp == 19) {
-      // the exponents of each tile's largest scales (a lane takes 2 G of the 64 G); V's only grows
+      // The exponents of each tile's largest scales (V's only grows), and the scales as fp16, K's divided by 2^ek, V's by
+      // 2^E: two positions a lane. (One warp for the other eight: it shares its scheduler with as many of them as any.)
+      const int k0 = 2 * lane, off[2] = {(k0 >> 4) * F::REC + F::scale(k0 & 15, 0),
+                                         (k0 >> 4) * F::REC + F::scale((k0 + 1) & 15, 0)};
+      auto largest = [](const uint32_t (&w)[2][G / 2]) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i) m = __vmaxu2(m, __vmaxu2(w[0][i], w[1][i]));
+        return __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
+      };
+      auto without_nan = [](const uint32_t (&w)[2][G / 2], uint32_t (&o)[2][G / 2]) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < G / 2; ++i)
+            o[k][i] = ((w[k][i] & 0xFFFFu) < 0x7F80u ? w[k][i] & 0xFFFFu : 0u) | (w[k][i] < 0x7F800000u ? w[k][i] & 0xFFFF0000u : 0u);
+      };
       int E = 1;
       for (int j = 0; j < nt; ++j) {
         const int rs = j % KV4P_RAW;
         if (!mbar_wait_all(&raw_full[rs], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL)) break;
         const uint8_t* raw = smem + SM::RAW + rs * SM::RAWT;
         const int left = klen - 64 * j;
-        auto largest = [&](int from) {
-          const uint8_t* p = raw + (lane >> 3) * F::REC + from + (lane & 7) * (4 * G);
-          uint32_t w[G], top = 0;
-          if constexpr (G == 4) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-          } else {
-            const uint2 u = *reinterpret_cast<const uint2*>(p);
-            w[0] = u.x; w[1] = u.y;
-          }
-          // two positions: the i-th and (i + 1)-th of lane-in-quad t, G / 2 words each
-          const int t = (lane & 7) >> 1, i = (lane & 1) * 2, k0 = (lane >> 3) * 16 + 4 * i + t,
-                    k1 = (lane >> 3) * 16 + 4 * (i + 1) + (t ^ 3);
+        uint32_t kw[2][G / 2], vw[2][G / 2];
 #pragma unroll
-          for (int k = 0; k < G; ++k) {
-            uint32_t lo = w[k] & 0xFFFFu, hi = w[k] >> 16;
-            if ((k < G / 2 ? k0 : k1) >= left) lo = hi = 0;
-            top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));      // (NaN does not count)
+        for (int k = 0; k < 2; ++k) {
+          if constexpr (G == 4) {
+            const uint2 x = *reinterpret_cast<const uint2*>(raw + F::KS0 + off[k]);
+            kw[k][0] = x.x; kw[k][1] = x.y;
+            const uint2 y = *reinterpret_cast<const uint2*>(raw + F::VS0 + off[k]);
+            vw[k][0] = y.x; vw[k][1] = y.y;
+          } else {
+            kw[k][0] = *reinterpret_cast<const uint32_t*>(raw + F::KS0 + off[k]);
+            vw[k][0] = *reinterpret_cast<const uint32_t*>(raw + F::VS0 + off[k]);
           }
-          return min(max(int(__reduce_max_sync(0xffffffffu, top) >> 7), 1), 253);
-        };
-        E = max(largest(F::VS0), E);
-        const int ex = largest(F::KS0);
-        // the scales as fp16, K's divided by 2^ek, V's by 2^E (two positions a lane); none behind the last key
+          if (k0 + k >= left)                            // behind the last key: whatever the record holds there
+#pragma unroll
+            for (int i = 0; i < G / 2; ++i) kw[k][i] = vw[k][i] = 0;
+        }
+        uint32_t topk = largest(kw), topv = largest(vw);
+        if (topk >= 0x7F80u) {                           // a NaN scale of K stays NaN but does not count
+          uint32_t x[2][G / 2];
+          without_nan(kw, x);
+          topk = largest(x);
+        }
+        if (topv >= 0x7F80u) {                           // one of V counts as zero here and is put back at the end
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < G / 2; ++i) {
+              if ((vw[k][i] & 0xFFFFu) >= 0x7F80u) atomicMin(&nanv[2 * i], 64 * j + k0 + k);
+              if (vw[k][i] >= 0x7F800000u) atomicMin(&nanv[2 * i + 1], 64 * j + k0 + k);
+            }
+          uint32_t x[2][G / 2];
+          without_nan(vw, x);
+#pragma unroll
+          for (int i = 0; i < G / 2; ++i) {
+            vw[0][i] = x[0][i];
+            vw[1][i] = x[1][i];
+          }
+          topv = largest(vw);
+        }
+        const int ex = min(max(int(topk >> 7), 1), 253);
+        E = max(E, min(int(topv >> 7), 253));
         __half* tk = reinterpret_cast<__half*>(smem + SM::SC + rs * SM::SCT);
         __half* tv = tk + 64 * G;
         const float dk = pow2_biased_inv(ex), dv = pow2_biased_inv(E);
-        float vsc[2][G];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int key = 2 * lane + k;
-          const uint8_t* p = raw + (key >> 4) * F::REC + F::scale(key & 15, 0);
-          uint32_t kw[G / 2], vw[G / 2], h[G / 2];
+        for (int i = 0; i < G / 2; ++i) {
+          float2 v[2];
 #pragma unroll
-          for (int i = 0; i < G / 2; ++i) {
-            kw[i] = key < left ? *reinterpret_cast<const uint32_t*>(p + F::KS0 + 4 * i) : 0u;
-            vw[i] = key < left ? *reinterpret_cast<const uint32_t*>(p + F::VS0 + 4 * i) : 0u;
-            h[i] = pack_f16(__uint_as_float(kw[i] << 16) * dk, __uint_as_float(kw[i] & 0xFFFF0000u) * dk);
-            *reinterpret_cast<uint32_t*>(tk + key * G + 2 * i) = h[i];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              uint32_t sc = e ? vw[i] & 0xFFFF0000u : vw[i] << 16;
-              if (sc >= 0x7F800000u) {                   // NaN: counts as zero here and is put back at the end
-                atomicMin(&nanv[2 * i + e], 64 * j + key);
-                sc = 0;
-              }
-              vsc[k][2 * i + e] = __uint_as_float(sc) * dv;
-            }
+          for (int k = 0; k < 2; ++k) {
+            const float2 x = unpack_bf16(kw[k][i]), y = unpack_bf16(vw[k][i]);
+            *reinterpret_cast<uint32_t*>(tk + (k0 + k) * G + 2 * i) = pack_f16(x.x * dk, x.y * dk);
+            v[k] = make_float2(y.x * dv, y.y * dv);
           }
+          *reinterpret_cast<uint32_t*>(tv + 2 * i * 64 + k0) = pack_f16(v[0].x, v[1].x);
+          *reinterpret_cast<uint32_t*>(tv + (2 * i + 1) * 64 + k0) = pack_f16(v[0].y, v[1].y);
         }
-#pragma unroll
-        for (int s = 0; s < G; ++s) *reinterpret_cast<uint32_t*>(tv + s * 64 + 2 * lane) = pack_f16(vsc[0][s], vsc[1][s]);
         __syncwarp();
         if (lane == 0) {
           ek[j & 15] = ex;
