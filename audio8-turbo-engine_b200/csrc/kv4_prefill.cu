@@ -126,8 +126,9 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
   int* nanv = ev + 16;                                   // [4] first position whose V group is NaN
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + SM::BARS);
   uint64_t *raw_full = q_full + 1, *raw_free = raw_full + KV4P_RAW, *e_full = raw_free + KV4P_RAW, *k_full = e_full + KV4P_RAW,
-           *k_free = k_full + 2, *v_full = k_free + 2, *v_free = v_full + KV4P_VST, *s_full = v_free + KV4P_VST, *p_full = s_full + 4, *p_free = p_full + 2;   // s_full: [tile][stage]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_free + 2);
+           *k_free = k_full + 2, *v_full = k_free + 2, *v_free = v_full + KV4P_VST, *s_full = v_free + KV4P_VST, *p_full = s_full + 4,
+           *p_free = p_full + 4;                         // the last three: [tile][stage]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_free + 4);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch();
@@ -157,8 +158,6 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], KV4P_DEQ);
       mbar_init(&k_free[s], 1);
-      mbar_init(&p_full[s], 4 * ntx);
-      mbar_init(&p_free[s], 1);
     }
     for (int s = 0; s < KV4P_VST; ++s) {
       mbar_init(&v_full[s], KV4P_DEQ);
@@ -166,6 +165,8 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&s_full[s], 2);                          // the MMAs' completion, and the issuer itself (for ek, ev)
+      mbar_init(&p_full[s], 4);
+      mbar_init(&p_free[s], 1);
     }
     fence_mbar_init();
     for (int g = 0; g < 4; ++g) nanv[g] = 0x7FFFFFFF;
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
           if (j > 0) {
             // O is at rest once the previous tile's product is complete: scale it in place
             const float oa = al * (Ej > E ? pow2_biased(max(127 + E - Ej, 0)) : 1.f);
-            if (!(ok = mbar_wait_all(&p_free[(j - 1) & 1], ((j - 1) >> 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL)))
+            if (!(ok = mbar_wait_all(&p_free[b ^ 1], ((j - 1) >> 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL)))
               break;
             tc_fence_after();
 #pragma unroll 1
@@ -286,10 +287,10 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       l += sum;
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[j & 1]);
+      if (lane == 0) mbar_arrive(&p_full[b]);
     }
     if (x < ntx && ok) {
-      ok = mbar_wait_all(&p_free[(nt - 1) & 1], ((nt - 1) >> 1) & 1, ERR_TIMEOUT_ACCUM, KERNEL_ID_KV4_PREFILL);
+      ok = mbar_wait_all(&p_free[2 * x + ((nt - 1) & 1)], ((nt - 1) >> 1) & 1, ERR_TIMEOUT_ACCUM, KERNEL_ID_KV4_PREFILL);
       tc_fence_after();
       if (ok) {
         const float inv = pow2_biased(E) / l;
@@ -422,14 +423,12 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       for (int j = 0; ok && j < nt; ++j) {
         const int st = j & 1, ph = (j >> 1) & 1;
         // K of this tile; the stage's last P (in the columns of S) has been multiplied
-        if (j < 2)
-          ok = mbar_wait_all(&k_full[st], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
-        else
-          ok = kv4_wait2(&k_full[st], ph, &p_free[st], ph ^ 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          for (int x = 0; x < ntx; ++x) {
+        for (int x = 0; x < ntx; ++x) {
+          ok = j < 2 ? mbar_wait_all(&k_full[st], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL)
+                     : kv4_wait2(&k_full[st], ph, &p_free[2 * x + st], ph ^ 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
             const uint32_t d = tmem + x * 128 + st * 64;
             const uint64_t da = dQ + x * (SM::QT >> 4), db = dK + st * (SM::KT >> 4);
 #pragma unroll
@@ -437,10 +436,10 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
               umma_f16(d, da + (k >> 2) * (16384 >> 4) + 2 * (k & 3), db + (k >> 2) * (8192 >> 4) + 2 * (k & 3), idS, k != 0);
             umma_commit(&s_full[2 * x + st]);
             mbar_arrive(&s_full[2 * x + st]);
+            if (x == ntx - 1) umma_commit(&k_free[st]);
           }
-          umma_commit(&k_free[st]);
+          __syncwarp();
         }
-        __syncwarp();
       }
     } else if (warp == 18) {
       constexpr uint32_t idO = umma_idesc(128, HD, 0);
@@ -448,19 +447,22 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       int vt = 0, vph = 0;
       for (int j = 0; j < nt; ++j) {
         const int st = j & 1;
-        if (!kv4_wait2(&p_full[st], (j >> 1) & 1, &v_full[vt], vph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL)) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t db = dV + vt * (SM::VT >> 4);
-          for (int x = 0; x < ntx; ++x) {
+        bool ok = true;
+        for (int x = 0; x < ntx; ++x) {
+          ok = kv4_wait2(&p_full[2 * x + st], (j >> 1) & 1, &v_full[vt], vph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t db = dV + vt * (SM::VT >> 4);
             const uint32_t d = tmem + 256 + x * HD, ta = tmem + x * 128 + st * 64;
 #pragma unroll
             for (int k = 0; k < 4; ++k) umma_f16_ts(d, ta + 8 * k, db + 2 * k, idO, (j > 0) | (k != 0));
+            umma_commit(&p_free[2 * x + st]);
+            if (x == ntx - 1) umma_commit(&v_free[vt]);
           }
-          umma_commit(&p_free[st]);
-          umma_commit(&v_free[vt]);
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
         if (++vt == KV4P_VST) {
           vt = 0;
           vph ^= 1;
