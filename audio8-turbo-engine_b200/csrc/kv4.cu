@@ -1033,6 +1033,7 @@ extern "C" int a8_kv4_store(const A8KV4* c, int layer, const void* qkv, int ld, 
   if (ld < heads * c->hd || (nq > 0 && ldq < (long long)nq * c->hd) || ring > c->cache_len) return A8_ERR_ARG;
   if (kv4_misaligned(qkv, ld) || (nq > 0 && kv4_misaligned(q, ldq)) || kv4_misaligned(cos, 0) || kv4_misaligned(sin, 0))
     return A8_ERR_ALIGN;
+  if (nq > 0 && q == qkv && ldq != ld) return A8_ERR_ARG;     // (in place: every thread rewrites what it read)
   Kv4StoreArgs a;
   a.c = kv4_view(c, layer);
   a.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv);
@@ -1133,7 +1134,8 @@ extern "C" int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_
   Kv4AttnArgs a;
   int rc = kv4_attn_args(&a, c, layer, q, q_stride, nq, rows, scale, out, out_stride);
   if (rc) return rc;
-  if (lens == nullptr || max_len <= 0 || max_len > c->cache_len) return A8_ERR_ARG;
+  // (in place: a unit's result is written after its last read of the queries it stands in)
+  if (lens == nullptr || max_len <= 0 || max_len > c->cache_len || (out == q && out_stride != q_stride)) return A8_ERR_ARG;
   // the steps of all rows are counted in 32 bits
   if (rows > (1 << 24) || (long long)rows * c->nkv * ((max_len + KV4_STEP - 1) / KV4_STEP) >= (1ll << 31)) return A8_ERR_SIZE;
   const int ctas = kv4_ctas(c, rows, max_len);

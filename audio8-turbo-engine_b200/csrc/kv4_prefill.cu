@@ -131,7 +131,6 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_free + 4);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  pdl_launch();
   pdl_wait();
   // the last blocks first, all their heads together: they attend the most keys of a prompt
   const int hq = (a.group + 3) / 4, per = a.c.nkv * hq;
@@ -176,6 +175,9 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // Only now may the next kernel's CTAs come: one that took tensor memory on this SM first, and then waited for this grid,
+  // would leave none for this CTA.
+  pdl_launch();
 
   if (warp < KV4P_SOFT) {
     A8_SETMAXNREG("inc", 144);
@@ -586,7 +588,8 @@ extern "C" int a8_kv4_prefill_attention(const A8KV4* c, int layer, const void* q
   Kv4AttnArgs a;
   int rc = kv4_attn_args(&a, c, layer, q, q_stride, nq, rows, scale, out, out_stride);
   if (rc) return rc;
-  if (blocks == nullptr || nblocks <= 0) return A8_ERR_ARG;
+  // (in place: a CTA reads the queries of its rows and heads before it writes their results)
+  if (blocks == nullptr || nblocks <= 0 || (out == q && out_stride != q_stride)) return A8_ERR_ARG;
   a.blocks = blocks;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return c->hd == 64 ? kv4_prefill_launch<64>(a, nblocks, s) : kv4_prefill_launch<128>(a, nblocks, s);

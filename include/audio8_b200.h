@@ -155,8 +155,8 @@ long long a8_kv4_bytes(const A8KV4* c);
 /* Write packed rows: qkv bf16 [rows, ld], row r = [q (nq heads) | k (nkv) | v (nkv)] of hd (what a8_gemm with
  * A8_EPI_BF16 and a bias gives), at position pos[r] of cache row slot[r] (NULL: r); with ring > 0 the cache position is
  * pos % ring. cos / sin bf16 [npos, hd] rotate_half tables (both halves alike) rotate q and k at pos in fp32, rounded once
- * to bf16; NULL: no rotation. q_out [rows, ldq] receives the query heads (it may be qkv itself with ldq = ld); nq = 0: k
- * and v only, q_out unused. A row with pos < 0 is padding: nothing of it is read or written. A row whose cache row,
+ * to bf16; NULL: no rotation. q_out [rows, ldq] receives the query heads (it may be qkv itself with ldq = ld, else it does
+ * not overlap it); nq = 0: k and v only, q_out unused. A row with pos < 0 is padding: nothing of it is written. A row whose cache row,
  * cache position or table row is out of range is not written and records ERR_BOUNDS (a8_get_error). Rows of one call that
  * share a cache row and position leave either row's codes or scales there (finite values; give a position once). Pointers
  * 16-byte aligned, ld and ldq multiples of 8. The counterpart of A8_EPI_ROPE for this cache. */
@@ -175,17 +175,20 @@ int a8_kv4_attention_workspace(const A8KV4* c, int nq, int rows, int max_len, lo
 /* a8_attention over the 4-bit cache, one query token a row: out[r, h, :] = softmax(scale q[r, h] . K[:L_r]) V[:L_r] over
  * cache row rowmap[r] (NULL: r), kv head h / (nq / nkv), L_r = min(lens[r], max_len). q / out bf16 [rows, stride] (16-byte
  * aligned, strides multiples of 8), nq / nkv from 1 to 16. L_r <= 0 gives zeros. A row whose cache row is out of range
- * gives zeros and records ERR_BOUNDS. scale <= 0: hd^-0.5. counters: n_counters ints, zero before the first call (a call
- * leaves them zero); ws and counters belong to one call at a time. The order of every sum depends only on the lens of the
- * call, so equal calls give equal bits. */
+ * gives zeros and records ERR_BOUNDS. scale <= 0: hd^-0.5. out may be q (of the same stride), else it does not overlap
+ * it. counters: n_counters ints, zero before the first call (a call leaves them zero; after a recorded timeout, zero them again); ws (16-byte aligned) and counters
+ * belong to one call at a time. The order of every sum depends only on the shape, lens, cache rows and max_len of a call, so
+ * equal calls give equal bits. */
 int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* lens, const int* rowmap,
                      int rows, int max_len, float scale, void* out, int out_stride, float* ws, long long ws_floats,
                      int* counters, int n_counters, a8_stream_t stream);
 
 /* a8_prefill_attention over the 4-bit cache: blocks int32 [nblocks][4] = (q0, n, slot, pos0) as there (n <= 64; rows
  * q0 .. q0 + n - 1 at positions pos0 .. of cache row slot, each attending keys [0, its position], stored beforehand); a
- * block with n <= 0 is skipped and rows of out that no block covers are left as they are. A block whose rows, cache row or
- * positions are out of range writes nothing and records ERR_BOUNDS. hd 64 or 128, nq / nkv from 1 to 16. */
+ * block with n <= 0 is skipped and rows of out that no block covers are left as they are; a row is in one block at most. A
+ * block whose rows, cache row or positions are out of range writes nothing and records ERR_BOUNDS. hd 64 or 128, nq / nkv
+ * from 1 to 16; out may be q (of the same stride). Codes times scales are exact in the fp16 that the products take, except
+ * for values below 2^-14 of the largest in their 64-key tile (or, of V, in an earlier one): those are held to 2^-24 of it. */
 int a8_kv4_prefill_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* blocks,
                              int nblocks, int rows, float scale, void* out, int out_stride, a8_stream_t stream);
 

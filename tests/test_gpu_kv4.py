@@ -511,3 +511,178 @@ def test_a_layer_prompt_then_decode(kv4, nq, nkv, hd):
         kv = {s: torch.stack(v) for s, v in hist.items()}
         assert same(qd, qo)
         check_rows(od, qo, kv, [(0, 1, 2, at[0]), (1, 1, 0, at[1])], nq, nkv, hd)
+
+
+# ------------------------------------------------------------------------------------------------- many shapes
+def gpu_reference(q, kv, row_keys, nq, nkv, hd):
+    """check_rows' reference and bound on the GPU in 64 bits, one query row at a time: row_keys (cache row, keys) each."""
+    out = torch.zeros(len(row_keys), nq, hd, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(out)
+    qd = q.double().view(-1, nkv, nq // nkv, hd)
+    for r, (row, n) in enumerate(row_keys):
+        if n <= 0:
+            continue
+        k, v = kv[row][:n, 0].transpose(0, 1), kv[row][:n, 1].transpose(0, 1)          # [nkv, n, hd]
+        z = qd[r] @ k.transpose(1, 2) * hd ** -0.5
+        w = torch.softmax(z, -1)
+        o, pv = w @ v, w @ v.abs()
+        logit = (qd[r].abs() @ k.abs().transpose(1, 2) * hd ** -0.5).amax(-1, keepdim=True) * 2.0 ** -18
+        out[r] = o.reshape(nq, hd)
+        tol[r] = (2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -10 + 2 * logit) * pv + 1e-30).reshape(nq, hd)
+    return out, tol
+
+
+def random_case(seed):
+    g = torch.Generator().manual_seed(seed)
+    pick = lambda xs: xs[int(torch.randint(0, len(xs), (1,), generator=g))]
+    nq, nkv, hd = pick([(14, 2, 64), (8, 8, 128), (12, 3, 128), (16, 1, 64), (10, 1, 128), (3, 3, 64), (5, 1, 64)])
+    rows = pick([1, 2, 5, 40, 300, 700, 1537])
+    top = pick([1, 33, 64, 200, 900, 2500]) if rows < 300 else pick([1, 40, 130])
+    kind = pick(["even", "any", "one long", "mostly empty"])
+    lens = torch.randint(0, top + 1, (rows,), generator=g)
+    if kind == "even":
+        lens[:] = top
+    elif kind == "one long":
+        lens = lens.clamp(max=3)
+        lens[rows // 2] = top
+    elif kind == "mostly empty":
+        lens[torch.rand(rows, generator=g) < 0.9] = 0
+    return nq, nkv, hd, rows, top, lens.tolist(), g
+
+
+@pytest.mark.parametrize("seed", range(36))
+def test_attention_random_shapes(kv4, seed):
+    nq, nkv, hd, rows, top, lens, g = random_case(seed)
+    CR = min(rows, 11)
+    c, kv = filled(kv4, seed, {r: top for r in range(CR)}, CR, nkv, hd, top + seed % 40)
+    kv = {r: x.cuda() for r, x in kv.items()}
+    q = rnd(seed + 7000, rows, nq * hd, scale=1.5).cuda()
+    rowmap = torch.randint(0, CR, (rows,), generator=g).tolist()
+    got = c.attention(q, i32(lens), i32(rowmap), max_len=top).double().view(rows, nq, hd)
+    no_error(kv4)
+    want, tol = gpu_reference(q, kv, list(zip(rowmap, lens)), nq, nkv, hd)
+    d = (got - want).abs()
+    assert bool((d <= tol).all()), (nq, nkv, hd, rows, top, float((d - tol).max()))
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_prefill_random_shapes(kv4, seed):
+    from audio8_b200.engine import FastEngine
+    nq, nkv, hd, rows, top, lens, g = random_case(seed + 100)
+    parts, slot = [], 0
+    for n in [x for x in lens if x > 0][:9]:
+        parts.append((slot, int(torch.randint(0, 300, (1,), generator=g)), n))
+        slot += 1
+    if not parts:
+        parts = [(0, 5, 70)]
+    S = max(a + n for _, a, n in parts)
+    c, kv = filled(kv4, seed, {s: a + n for s, a, n in parts}, len(parts), nkv, hd, S)
+    kv = {r: x.cuda() for r, x in kv.items()}
+    pos = [p for _, a, n in parts for p in range(a, a + n)]
+    sl = [s for s, _, n in parts for _ in range(n)]
+    q = rnd(seed + 9000, len(pos), nq * hd, scale=1.5).cuda()
+    blocks = FastEngine.query_blocks(pos, sl)
+    blocks = torch.from_numpy(blocks)[torch.randperm(len(blocks), generator=g)].contiguous().cuda()
+    got = c.prefill_attention(q, blocks).double().view(len(pos), nq, hd)
+    no_error(kv4)
+    take = torch.randperm(len(pos), generator=g)[:150].tolist()
+    want, tol = gpu_reference(q[take], kv, [(sl[r], pos[r] + 1) for r in take], nq, nkv, hd)
+    d = (got[take] - want).abs()
+    assert bool((d <= tol).all()), (nq, nkv, hd, parts, float((d - tol).max()))
+    # in place
+    same_place = q.clone()
+    assert c.prefill_attention(same_place, blocks, out=same_place).data_ptr() == same_place.data_ptr()
+    assert torch.equal(same_place.double().view(len(pos), nq, hd), got)
+
+
+def test_prefill_nan_reaches_its_own_rows_only(kv4):
+    """A NaN among the values at position 70 makes the 32 dims of its group NaN for rows from 70 on, one among the keys at
+    position 90 whole rows from 90 on; earlier rows of the same tiles are untouched."""
+    nq, nkv, hd, n = 4, 2, 128, 130
+    x = rnd(123, n, 2, nkv, hd)
+    q = rnd(124, n, nq * hd).cuda()
+    pos = torch.arange(n, dtype=I32).cuda()
+    from audio8_b200.engine import FastEngine
+    blocks = torch.from_numpy(FastEngine.query_blocks(list(range(n)), [0] * n)).cuda()
+
+    def run(y):
+        c = garbage(kv4.KV4Cache(1, nkv, hd, n))
+        c.store(y.reshape(n, -1).cuda(), pos, torch.zeros(n, dtype=I32).cuda())
+        return c.prefill_attention(q, blocks).view(n, nq, 4, 32).cpu()
+    clean = run(x)
+    y = x.clone()
+    y[70, 1, 1, 40] = float("nan")
+    y[90, 0, 0, 3] = float("nan")
+    got = run(y)
+    no_error(kv4)
+    nan = torch.zeros(n, nq, 4, 32, dtype=torch.bool)
+    nan[70:, 2:, 1] = True                               # kv head 1: query heads 2, 3; dims 32..63
+    nan[90:, :2] = True                                  # kv head 0
+    assert torch.equal(got.isnan(), nan)
+    assert torch.equal(got[~nan], clean[~nan])
+
+
+def test_prefill_wide_scales(kv4):
+    """Keys and values from 2^-90 to 2^20 and values rising by tiles (the exponent that V is divided by grows)."""
+    from audio8_b200.engine import FastEngine
+    nq, nkv, hd, n = 2, 1, 64, 300
+    x = rnd(130, n, 2, nkv, hd)
+    x[:, 1] *= (2.0 ** torch.linspace(-90, 20, n)).to(BF)[:, None, None]
+    x[:, 0] *= (2.0 ** torch.linspace(-60, 0, n)).to(BF)[:, None, None]
+    c = garbage(kv4.KV4Cache(1, nkv, hd, n))
+    c.store(x.reshape(n, -1).cuda(), torch.arange(n, dtype=I32).cuda(), torch.zeros(n, dtype=I32).cuda())
+    q = rnd(131, n, nq * hd, scale=2.0)
+    out = c.prefill_attention(q.cuda(), torch.from_numpy(FastEngine.query_blocks(list(range(n)), [0] * n)).cuda())
+    no_error(kv4)
+    got, qd, kv = out.cpu().double().view(n, nq, hd), q.double().view(n, nq, hd), R.values(x)
+    for h in range(nq):
+        o, tol = R.attention(qd[:, h], kv[:, 0, 0], kv[:, 1, 0], 0, hd ** -0.5)
+        # (the exponents fp16 operands are divided by come from whole tiles: the bound of kv4_ref.prompt_slack)
+        tol = tol + R.prompt_slack(qd[:, h], kv[:, 0, 0], kv[:, 1, 0], 0, hd ** -0.5)
+        d = (got[:, h] - o).abs()
+        assert bool((d <= tol).all()), (h, float((d - tol).max()))
+
+
+def test_attention_in_place(kv4):
+    for nq, nkv, hd, lens in ((14, 2, 64, [5000, 3, 0, 70]), (8, 8, 128, [128] * 40), (16, 1, 64, [9000])):
+        c, _ = filled(kv4, 9, {0: max(lens)}, 1, nkv, hd, max(lens))
+        q = rnd(150, len(lens), nq * hd).cuda()
+        rowmap = torch.zeros(len(lens), dtype=I32, device="cuda")
+        want = c.attention(q, i32(lens), rowmap)
+        place = q.clone()
+        c.attention(place, i32(lens), rowmap, out=place)
+        no_error(kv4)
+        assert torch.equal(place, want)
+
+
+def test_prompt_attention_between_gemms(kv4):
+    """Many CTAs of the prompt attention between GEMMs that hold tensor memory, over and over in one stream and captured:
+    each result is the first one's."""
+    from audio8_b200.engine import FastEngine
+    L = kv4._lib
+    nq, nkv, hd, n, dim = 14, 2, 64, 1900, 256
+    c, _ = filled(kv4, 8, {0: n}, 1, nkv, hd, n)
+    q = rnd(140, n, nq * hd).cuda()
+    blocks = torch.from_numpy(FastEngine.query_blocks(list(range(n)), [0] * n)).cuda()
+    w = rnd(141, dim, nq * hd, scale=0.03).cuda()
+    y = torch.empty(n, dim, dtype=BF, device="cuda")
+    o = torch.empty_like(q)
+
+    def chain():
+        for _ in range(4):
+            c.prefill_attention(q, blocks, out=o)
+            e = L.A8Epilogue(kind=L.EPI_BF16)
+            L.call("a8_gemm", L.ptr(o), nq * hd, L.ptr(w), dim, nq * hd, n, L.ptr(y), dim, C.byref(e), 0,
+                   L.stream_handle())
+    chain()
+    no_error(kv4)
+    first_o, first_y = o.clone(), y.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        chain()
+    for _ in range(10):
+        o.zero_()
+        y.zero_()
+        g.replay()
+    no_error(kv4)
+    assert torch.equal(o, first_o) and torch.equal(y, first_y)

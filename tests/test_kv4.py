@@ -198,3 +198,14 @@ def test_record_layout_is_a_permutation():
                     b = base + ((t * 4 + i) * G + slot(g)) * 2
                     seen |= set(range(b, b + 2))
         assert len(seen) == 18 * hd and max(seen) == 18 * hd - 1
+
+
+def test_overlapping_outputs_refused(L):
+    lib, N = L.load(), None
+    d = C.byref(desc(L))
+    # store: q may be qkv itself only with its stride
+    assert lib.a8_kv4_store(d, 0, p(), 18 * 64 + 64, 14, N, N, 0, p(4096), N, 4, 0, p(), 14 * 64, N) == ARG
+    # attention: in place only with the same stride
+    assert lib.a8_kv4_attention(d, 0, p(), 896, 14, p(4096), N, 4, 100, 0.0, p(), 960, p(8192), 1 << 40, p(8192), 1 << 30,
+                                N) == ARG
+    assert lib.a8_kv4_prefill_attention(d, 0, p(), 896, 14, p(4096), 1, 4, 0.0, p(), 960, N) == ARG
