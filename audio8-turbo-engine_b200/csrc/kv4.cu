@@ -312,23 +312,15 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// The same codes as fp16 with an offset: nibbles 0 and 2 of a half as 1024 + u, 1 and 3 as 1024 + 16 u (mask with or).
-__device__ __forceinline__ uint32_t kv4_lo16(uint32_t w) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(d) : "r"(w));
-  return d;
-}
-__device__ __forceinline__ uint32_t kv4_hi16(uint32_t w) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, 0x00F000F0, 0x64006400, 0xEA;" : "=r"(d) : "r"(w));
-  return d;
-}
 __device__ __forceinline__ void kv4_mma_bf16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-constexpr float KV4_OFF_LO = 1032.f, KV4_OFF_HI = 1152.f;   // code 0 in the two forms: 1024 + 8, 1024 + 16 x 8
+// As they stand, nibbles 0 and 2 of a half are the fp16 subnormals u 2^-24, 1 and 3 (in bits 4-7) 16 u 2^-24: exact operands
+// of a product, one mask each.
+constexpr uint32_t KV4_LO = 0x000F000Fu, KV4_HI = 0x00F000F0u;
+constexpr float KV4_OFF_LO = 8.f * 0x1p-24f, KV4_OFF_HI = 128.f * 0x1p-24f;     // code 0 in the two forms
 // d = a b (+ c): fp16 products of one 16-dim step
 __device__ __forceinline__ void mma_f16_first(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
@@ -541,9 +533,9 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
 #pragma unroll
         for (int s = 0; s < G; ++s) {
           float acc[4];
-          mma_f16_first(acc, qa[s][0], kv4_lo16(w[s]), kv4_hi16(w[s]));
+          mma_f16_first(acc, qa[s][0], w[s] & KV4_LO, w[s] & KV4_HI);
           const uint32_t w8 = w[s] >> 8;
-          mma_f16(acc, qa[s][1], kv4_lo16(w8), kv4_hi16(w8));
+          mma_f16(acc, qa[s][1], w8 & KV4_LO, w8 & KV4_HI);
           const float2 sc = sf2(ks[2 * nb][s >> 1], ks[2 * nb + 1][s >> 1], s);
 #pragma unroll
           for (int u = 0; u < NT; ++u) {
@@ -677,7 +669,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const uint32_t ex = max(top >> 7, 8u);
         const float up = __uint_as_float((261u - ex) << 23);
-        qs[u] = a.scale_log2 * __uint_as_float((ex - 7u) << 23);
+        qs[u] = a.scale_log2 * __uint_as_float((ex - 7u) << 23) * 0x1p24f;
 #pragma unroll
         for (int s = 0; s < G; ++s) {
           const float2 d01 = unpack_bf16(x[s].x), d23 = unpack_bf16(x[s].y), d45 = unpack_bf16(x[s].z),

@@ -94,6 +94,17 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
       : "memory");
 }
 
+// Codes of the two 16-bit halves of w as fp16 with an offset: nibbles 0 and 2 of a half as 1024 + u, 1 and 3 as 1024 + 16 u (mask with or).
+__device__ __forceinline__ uint32_t kv4_lo16(uint32_t w) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(d) : "r"(w));
+  return d;
+}
+__device__ __forceinline__ uint32_t kv4_hi16(uint32_t w) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, 0x00F000F0, 0x64006400, 0xEA;" : "=r"(d) : "r"(w));
+  return d;
+}
 // The pairs (n, n + 4) of a word's (or of a key pair's) codes, n = 0..3, as fp16 whole numbers.
 __device__ __forceinline__ void kv4_codes_f16(uint32_t w, __half2* c) {
   const __half2 off = __half2half2(__ushort_as_half(0xE408));                     // -1032

@@ -32,13 +32,22 @@ def values(x):
     return (c * s[..., None]).flatten(-2)
 
 
+def logit_error(q, k):
+    """[m, n]: what q.k (before the softmax scale) may be off by, as `attention` derives it; batch dimensions allowed."""
+    gq = q.abs().unflatten(-1, (-1, GROUP)).sum(-1)
+    gk = k.abs().unflatten(-1, (-1, GROUP)).amax(-1) / 6.9
+    return 2.0 ** -18 * (q.abs() @ k.abs().transpose(-1, -2)) + 2.0 ** -13 * (gq @ gk.transpose(-1, -2))
+
+
 def attention(q, k, v, first, scale):
     """(out, err) [m, hd] float64: row i of q [m, hd] over keys [0, first + i] of k / v [n, hd], and a bound of what a
     kernel with fp32 sums and bf16 softmax weights may be off by. A rounding to bf16 is off by at most 2^-8 of its value:
-    one on every weight (together at most 2^-8 sum p|v| / sum p), one on the output (2^-8 |out|). An fp32 logit is off by
-    at most 2^-18 scale sum_d |q_d k_d| (a sum of at most 128 exact products, 16 at a time: fewer than 32 roundings of
-    2^-23), which moves a weight by as much of itself, in the numerator and in the sum below; the fp32 sums over keys by
-    at most n 2^-23, taken as 2^-10 (far above it at the lengths tested)."""
+    one on every weight (together at most 2^-8 sum p|v| / sum p), one on the output (2^-8 |out|). A logit sums, over the
+    32-dim groups, s q.code: at most 128 exact products, 16 at a time, fewer than 32 roundings of 2^-23 of the sum so far:
+    2^-18 scale sum_d |q_d k_d|. A kernel may hold the codes as code + 8 and take 8 sum q off afterwards; a group's sum of
+    32 products of up to 15 |q_d| is then off by at most 40 roundings of 2^-23 of it, 2^-13 s sum_d |q_d|, with
+    s <= max|k| / 6.9 over the group. A logit's error moves a weight by as much of itself, in the numerator and in the sum
+    below; the fp32 sums over keys add at most n 2^-23, taken as 2^-10 (far above it at the lengths tested)."""
     m, n = q.shape[0], k.shape[0]
     z = q @ k.T * scale
     far = torch.arange(n)[None, :] > first + torch.arange(m)[:, None]
@@ -46,7 +55,7 @@ def attention(q, k, v, first, scale):
     p = torch.softmax(z, -1)
     out = p @ v
     pv = p @ v.abs()
-    logit = ((q.abs() @ k.abs().T * scale).masked_fill(far, 0).amax(-1, keepdim=True)) * 2.0 ** -18
+    logit = logit_error(q, k).mul(scale).masked_fill(far, 0).amax(-1, keepdim=True)
     return out, 2.0 ** -8 * out.abs() + (2.0 ** -8 + 2.0 ** -10 + 2 * logit) * pv + 1e-30
 
 

@@ -526,7 +526,7 @@ def gpu_reference(q, kv, row_keys, nq, nkv, hd):
         z = qd[r] @ k.transpose(1, 2) * hd ** -0.5
         w = torch.softmax(z, -1)
         o, pv = w @ v, w @ v.abs()
-        logit = (qd[r].abs() @ k.abs().transpose(1, 2) * hd ** -0.5).amax(-1, keepdim=True) * 2.0 ** -18
+        logit = (R.logit_error(qd[r], k) * hd ** -0.5).amax(-1, keepdim=True)
         out[r] = o.reshape(nq, hd)
         tol[r] = (2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -10 + 2 * logit) * pv + 1e-30).reshape(nq, hd)
     return out, tol
