@@ -312,15 +312,29 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// As they stand, nibbles 0 and 2 of a half are the fp16 subnormals u 2^-24, 1 and 3 (in bits 4-7) 16 u 2^-24: exact operands
+// of a product, one mask each.
+constexpr uint32_t KV4_LO = 0x000F000Fu, KV4_HI = 0x00F000F0u;
+constexpr float KV4_OFF_LO = 8.f * 0x1p-24f, KV4_OFF_HI = 128.f * 0x1p-24f;     // code 0 in the two forms
+// The codes n of the two 16-bit halves of w (n = 0, 2: w >> 4 n; n = 1, 3: w >> 4 (n - 1)) as bf16, times 2^-6: the masked
+// bits are the bf16 subnormals u 2^-133 and 16 u 2^-133, one fused multiply-add (exact) makes them (u - 8) 2^-6.
+__device__ __forceinline__ uint32_t kv4_code_lo(uint32_t w) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(w & KV4_LO), "r"(0x7F007F00u), "r"(0xBE00BE00u));   // x 2^127, - 2^-3
+  return d;
+}
+__device__ __forceinline__ uint32_t kv4_code_hi(uint32_t w) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(w & KV4_HI), "r"(0x7D007D00u), "r"(0xBE00BE00u));   // x 2^123, - 2^-3
+  return d;
+}
+constexpr float KV4_O_UNIT = 64.f;    // what O is held in
+
 __device__ __forceinline__ void kv4_mma_bf16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// As they stand, nibbles 0 and 2 of a half are the fp16 subnormals u 2^-24, 1 and 3 (in bits 4-7) 16 u 2^-24: exact operands
-// of a product, one mask each.
-constexpr uint32_t KV4_LO = 0x000F000Fu, KV4_HI = 0x00F000F0u;
-constexpr float KV4_OFF_LO = 8.f * 0x1p-24f, KV4_OFF_HI = 128.f * 0x1p-24f;     // code 0 in the two forms
 // d = a b (+ c): fp16 products of one 16-dim step
 __device__ __forceinline__ void mma_f16_first(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
@@ -628,8 +642,8 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
           b[u][0] = pack_bf16(p0.x, p0.y);
           b[u][1] = pack_bf16(p1.x, p1.y);
         }
-        const uint32_t lo[4] = {kv4_pair<0>(u01), kv4_pair<1>(u01), kv4_pair<0>(u23), kv4_pair<1>(u23)};
-        const uint32_t hi[4] = {kv4_pair<2>(u01), kv4_pair<3>(u01), kv4_pair<2>(u23), kv4_pair<3>(u23)};
+        const uint32_t lo[4] = {kv4_code_lo(u01), kv4_code_hi(u01), kv4_code_lo(u23), kv4_code_hi(u23)};
+        const uint32_t hi[4] = {kv4_code_lo(u01 >> 8), kv4_code_hi(u01 >> 8), kv4_code_lo(u23 >> 8), kv4_code_hi(u23 >> 8)};
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
           kv4_mma_bf16(o[u][s][0], lo, b[u][0], b[u][1]);
@@ -737,7 +751,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
         for (int e = 0; e < 2; ++e) {
           const int qh = 2 * t + e + 8 * u;
           if (qh >= a.group) continue;
-          const float inv = 1.f / (e ? l1 : l0);
+          const float inv = KV4_O_UNIT / (e ? l1 : l0);
 #pragma unroll
           for (int s = 0; s < G; ++s) {
             const int d = 32 * ((s & 1) * (G / 2) + s / 2) + 4 * g;
@@ -858,7 +872,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     const int* e = meta + 4 * list[from];
     const int u = e[0], us = e[1], ue = e[2];
     if (us >= b0 && ue <= b1) {
-      const float inv = 1.f / L;
+      const float inv = KV4_O_UNIT / L;
       *reinterpret_cast<uint2*>(a.out + (size_t)(u / a.c.nkv) * a.out_stride + (u % a.c.nkv * a.group) * HD + 4 * el) =
           make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
     } else {                                           // cut: in the unit's first CTA place 1, in later ones place 0
@@ -943,7 +957,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
         x.w += f * y.w;
         L += f * redm[sp * nel + el].y;
       }
-      const float inv = 1.f / L;
+      const float inv = KV4_O_UNIT / L;
       *reinterpret_cast<uint2*>(a.out + (size_t)(u / a.c.nkv) * a.out_stride + (u % a.c.nkv * a.group) * HD + 4 * el) =
           make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
     }
