@@ -64,11 +64,15 @@ int stack_forward(const A8StackDesc& d, const A8StackRun& r, cudaStream_t s) {
   A8_TRY(a8_rmsnorm(r.x, r.ldx, nullptr, 0, d.ln1, h, D, R, D, d.eps, st));
   CUtensorMap mk, mv;
   const long long total = (long long)d.layers * d.cache_rows * d.nkv * d.cache_len;
-  A8_TRY(attn_maps(&mk, &mv, d.kc, d.vc, total, d.hd));
+  const bool four = d.kv4 != nullptr;           // the caches in 4 bits
+  const A8KV4 kv4 = {d.kv4, d.layers, d.cache_rows, d.nkv, d.hd, d.cache_len};
+  if (four && NQKV > d.inter) return A8_ERR_SIZE;
+  if (four && d.ring > 0 && r.nblocks > 0) return A8_ERR_ARG;   // (the prompt form reads position p at p)
+  if (!four) A8_TRY(attn_maps(&mk, &mv, d.kc, d.vc, total, d.hd));
   const int max_len = r.max_len > 0 ? r.max_len : d.cache_len;
   // packed prefill rows with a query-block table go to the tensor-core prefill attention
-  const bool packed = r.blocks != nullptr && r.nblocks > 0 && d.hd == 64 && d.nq / d.nkv <= 8;
-  const int ms = packed ? 1 : attn_splits(R, d.nkv, max_len);
+  const bool packed = r.blocks != nullptr && r.nblocks > 0 && (four || (d.hd == 64 && d.nq / d.nkv <= 8));
+  const int ms = packed || four ? 1 : attn_splits(R, d.nkv, max_len);
   if (ms > 1 && (sc.attn_ws == nullptr || sc.attn_ws_floats < attn_ws_floats(R, d.nkv, ms, d.hd) ||
                  sc.attn_counters == nullptr || sc.n_attn_counters < R * d.nkv))
     return A8_ERR_SIZE;
@@ -89,14 +93,14 @@ int stack_forward(const A8StackDesc& d, const A8StackRun& r, cudaStream_t s) {
   for (int l = 0; l < d.layers; ++l) {
     const bool in_h = !fuse || l == 0;          // the layer's normed input is already in h
     A8Epilogue e = {};
-    e.kind = A8_EPI_ROPE;
+    e.kind = four ? A8_EPI_BF16 : A8_EPI_ROPE;
     e.bias = d.bqkv != nullptr ? at<__nv_bfloat16>(d.bqkv, l * bstride(d, 1)) : nullptr;
     e.cos = d.cos;
     e.sin = d.sin;
     e.pos = r.pos;
     e.slot = r.slot;
-    e.kc = reinterpret_cast<__nv_bfloat16*>(d.kc) + (size_t)l * d.cache_rows * d.nkv * d.cache_len * d.hd;
-    e.vc = reinterpret_cast<__nv_bfloat16*>(d.vc) + (size_t)l * d.cache_rows * d.nkv * d.cache_len * d.hd;
+    if (!four) e.kc = reinterpret_cast<__nv_bfloat16*>(d.kc) + (size_t)l * d.cache_rows * d.nkv * d.cache_len * d.hd;
+    if (!four) e.vc = reinterpret_cast<__nv_bfloat16*>(d.vc) + (size_t)l * d.cache_rows * d.nkv * d.cache_len * d.hd;
     e.nq = d.nq;
     e.nkv = d.nkv;
     e.hd = d.hd;
@@ -104,7 +108,11 @@ int stack_forward(const A8StackDesc& d, const A8StackRun& r, cudaStream_t s) {
     e.cache_len = d.cache_len;
     if (!in_h) normed(e, at<__nv_bfloat16>(d.ln1, l * bstride(d, 5)));
     A8_TRY(gemm(in_h ? (const void*)h : r.x, in_h ? D : r.ldx, at<__nv_bfloat16>(d.wqkv, l * bstride(d, 0)), NQKV, D,
-                R, q, QW, e, sc, s));
+                R, four ? m : q, four ? NQKV : QW, e, sc, s));
+    // (the tables hold every position the caller gives, as in the RoPE epilogue; the MLP's rows are free until then)
+    if (four)
+      A8_TRY(a8_kv4_store(&kv4, l, m, NQKV, d.nq, d.cos, d.sin, 1 << 30, r.pos, r.slot, R, d.ring > 0 ? d.ring : 0, q, QW,
+                          st));
     AttnArgs aa = {};
     aa.q = q;
     aa.q_stride = QW;
@@ -123,7 +131,12 @@ int stack_forward(const A8StackDesc& d, const A8StackRun& r, cudaStream_t s) {
     aa.ws = sc.attn_ws;
     aa.counters = sc.attn_counters;
     aa.rows = R;
-    if (packed) {
+    if (four && packed) {
+      A8_TRY(a8_kv4_prefill_attention(&kv4, l, q, QW, d.nq, r.blocks, r.nblocks, R, 0.f, o, QW, st));
+    } else if (four) {
+      A8_TRY(kv4_attention(&kv4, l, q, QW, d.nq, aa.lens, aa.lens_add, r.rowmap, R, std::min(max_len, aa.lens_max), 0.f, o,
+                           QW, sc.attn_ws, sc.attn_ws_floats, sc.attn_counters, sc.n_attn_counters, s));
+    } else if (packed) {
       PattnArgs pa = {};
       pa.blocks = r.blocks;
       pa.nq = d.nq;

@@ -263,7 +263,8 @@ struct Kv4AttnArgs {
   Kv4View c;
   const __nv_bfloat16* q;
   int q_stride, nq, group;
-  const int *lens, *rowmap;   // decode: keys of row r; cache row of row r (null: r)
+  const int *lens, *rowmap;   // decode: keys of row r: lens[r] + lens_add; cache row of row r (null: r)
+  int lens_add;
   const int* blocks;          // packed prompts: [nblocks][4] = (q0, n, slot, pos0)
   int rows, max_len;
   float scale_log2;
@@ -350,7 +351,7 @@ __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0
 // Row r's keys and cache row; (0, -) for a row that attends nothing.
 __device__ __forceinline__ int kv4_row(const Kv4AttnArgs& a, int r, int& crow) {
   crow = a.rowmap != nullptr ? a.rowmap[r] : r;
-  const int n = max(0, min(a.lens[r], a.max_len));
+  const int n = max(0, min(a.lens[r] + a.lens_add, a.max_len));
   return crow >= 0 && crow < a.c.cache_rows ? n : 0;
 }
 
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     for (int r = tid * run; r < min(a.rows, (tid + 1) * run); ++r) {
       int crow;
       if (r % gridDim.x != blockIdx.x || kv4_row(a, r, crow) != 0) continue;
-      if (a.lens[r] > 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_ATTN, r);
+      if (a.lens[r] + a.lens_add > 0) set_error(ERR_BOUNDS, KERNEL_ID_KV4_ATTN, r);
       uint4* o = reinterpret_cast<uint4*>(a.out + (size_t)r * a.out_stride);
       for (int i = 0; i < a.nq * HD / 8; ++i) o[i] = make_uint4(0, 0, 0, 0);
     }
@@ -1134,9 +1135,10 @@ static int kv4_attn_launch(Kv4AttnArgs& a, int ctas, cudaStream_t s) {
   return kv4_launch(fn, dim3(ctas), SM::NW * 32, SM::TOTAL, args, s) == cudaSuccess ? A8_OK : A8_ERR_CUDA;
 }
 
-extern "C" int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* lens,
-                                const int* rowmap, int rows, int max_len, float scale, void* out, int out_stride,
-                                float* ws, long long ws_floats, int* counters, int n_counters, a8_stream_t stream) {
+// a8_kv4_attention with row r's keys counted from lens[r] + lens_add (a stack gives its positions and 1).
+static int kv4_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* lens, int lens_add,
+                         const int* rowmap, int rows, int max_len, float scale, void* out, int out_stride, float* ws,
+                         long long ws_floats, int* counters, int n_counters, cudaStream_t s) {
   Kv4AttnArgs a;
   int rc = kv4_attn_args(&a, c, layer, q, q_stride, nq, rows, scale, out, out_stride);
   if (rc) return rc;
@@ -1150,11 +1152,18 @@ extern "C" int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_
     return A8_ERR_SIZE;
   if (reinterpret_cast<uintptr_t>(ws) & 15) return A8_ERR_ALIGN;
   a.lens = lens;
+  a.lens_add = lens_add;
   a.rowmap = rowmap;
   a.max_len = max_len;
   a.ws = ws;
   a.counters = counters;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (a.group <= 8) return c->hd == 64 ? kv4_attn_launch<64, 1>(a, ctas, s) : kv4_attn_launch<128, 1>(a, ctas, s);
   return c->hd == 64 ? kv4_attn_launch<64, 2>(a, ctas, s) : kv4_attn_launch<128, 2>(a, ctas, s);
+}
+
+extern "C" int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* lens,
+                                const int* rowmap, int rows, int max_len, float scale, void* out, int out_stride,
+                                float* ws, long long ws_floats, int* counters, int n_counters, a8_stream_t stream) {
+  return kv4_attention(c, layer, q, q_stride, nq, lens, 0, rowmap, rows, max_len, scale, out, out_stride, ws, ws_floats,
+                       counters, n_counters, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -24,6 +24,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
+from .kv4 import KV4Cache
 from .snapstore import SnapStore, ref_fp
 
 BF16 = torch.bfloat16
@@ -63,7 +64,7 @@ class PackedStack:
     """One transformer stack's packed weights, caches and RoPE tables on the device + its A8StackDesc."""
 
     def __init__(self, layers, norm, nq, nkv, hd, eps, rope_base, cache_rows, cache_len, max_pos, dev, ring=0,
-                 layer_scale=False):
+                 layer_scale=False, kv_bits=16):
         def w(t):
             return t.detach().to(torch.float32)
         wq, bq, wo, w13, w2, l1, l2 = [], [], [], [], [], [], []
@@ -89,8 +90,17 @@ class PackedStack:
         c, s = rope_tables(rope_base, hd, max_pos)
         self.cos, self.sin = c.to(dev), s.to(dev)
         nl = len(layers)
-        self.kc = torch.zeros(nl, cache_rows, nkv, cache_len, hd, dtype=BF16, device=dev)
-        self.vc = torch.zeros_like(self.kc)
+        # keys and values in bf16, or in 4 bits (kv4.KV4Cache)
+        self.kc = self.vc = self.kv4 = None
+        if kv_bits == 4:
+            if (nq + 2 * nkv) * hd > self.w2.shape[2]:
+                raise L.A8Error(f"a 4-bit cache needs an MLP of at least {(nq + 2 * nkv) * hd} columns")
+            self.kv4 = KV4Cache(cache_rows, nkv, hd, cache_len, dev, layers=nl)
+        elif kv_bits == 16:
+            self.kc = torch.zeros(nl, cache_rows, nkv, cache_len, hd, dtype=BF16, device=dev)
+            self.vc = torch.zeros_like(self.kc)
+        else:
+            raise L.A8Error(f"a cache of {kv_bits} bits (16 or 4)")
         self.nq, self.nkv, self.hd, self.eps = nq, nkv, hd, float(eps)
         self.dim = self.wo.shape[1]
         self.inter = self.w2.shape[2]
@@ -99,18 +109,21 @@ class PackedStack:
             layers=nl, dim=self.dim, nq=nq, nkv=nkv, hd=hd, inter=self.inter, eps=self.eps, wqkv=L.ptr(self.wqkv),
             bqkv=L.ptr(self.bqkv), wo=L.ptr(self.wo), w13=L.ptr(self.w13), w2=L.ptr(self.w2), ln1=L.ptr(self.ln1),
             ln2=L.ptr(self.ln2), norm=L.ptr(self.norm), cos=L.ptr(self.cos), sin=L.ptr(self.sin), kc=L.ptr(self.kc),
-            vc=L.ptr(self.vc), cache_rows=cache_rows, cache_len=cache_len, ring=self.ring)
+            vc=L.ptr(self.vc), cache_rows=cache_rows, cache_len=cache_len, ring=self.ring,
+            kv4=None if self.kv4 is None else L.ptr(self.kv4.buf))
 
 
 class Scratch:
     """Activation buffers and the attention's split workspace for up to `rows` token rows of stacks up to `dim` /
     `inter` wide."""
 
-    def __init__(self, rows, dim, qdim, inter, nkv, hd, max_len, dev):
+    def __init__(self, rows, dim, qdim, inter, nkv, hd, max_len, dev, kv4=None):
         mk = lambda n: torch.zeros(rows, n, dtype=BF16, device=dev)
         self.h, self.q, self.o, self.a, self.mlp = mk(dim), mk(qdim), mk(qdim), mk(dim), mk(inter)
         n = C.c_longlong()
         L.check(L.load().a8_attention_workspace(rows, nkv, hd, max_len, C.byref(n), None), "attention workspace")
+        if kv4 is not None:                 # (the 4-bit cache's attention also runs on it)
+            n.value = max(n.value, kv4.workspace(qdim // hd, rows, max_len)[0].numel())
         self.attn_ws = torch.zeros(max(1, n.value), dtype=torch.float32, device=dev)
         self.attn_counters = torch.zeros(rows * nkv, dtype=torch.int32, device=dev)
         self.ssq = torch.zeros(8, rows, dtype=torch.float32, device=dev)
@@ -161,7 +174,8 @@ class FastEngine:
         self.pf_rows = min(self.prefill_tokens, int(os.environ.get("TTS_PREFILL_ROWS", "2048")))
         self.SCR = B
         self.slow = PackedStack(model.layers, model.norm, c.n_head, c.n_local_heads, c.head_dim, c.norm_eps,
-                                c.rope_base, cache_rows=B + 1, cache_len=self.S, max_pos=self.S, dev=dev)
+                                c.rope_base, cache_rows=B + 1, cache_len=self.S, max_pos=self.S, dev=dev,
+                                kv_bits=int(os.environ.get("TTS_KV_BITS", "16")))
         self.fast = PackedStack(model.fast_layers, model.fast_norm, c.fast_n_head, c.fast_n_local_heads,
                                 c.fast_head_dim, c.norm_eps, c.rope_base, cache_rows=B, cache_len=self.ncg,
                                 max_pos=self.ncg, dev=dev)
@@ -219,7 +233,7 @@ class FastEngine:
         self.f_slot0 = (torch.arange(2 * B, dtype=i32, device=dev) // 2).contiguous()
         rows = max(2 * B, self.pf_rows)
         self.scratch = Scratch(rows, H, self.slow.nq * self.slow.hd, self.slow.inter, self.slow.nkv, self.slow.hd,
-                               self.S, dev)
+                               self.S, dev, self.slow.kv4)
         self.pf_pos = torch.zeros(self.pf_rows, dtype=i32, device=dev)
         self.pf_slot = torch.zeros(self.pf_rows, dtype=i32, device=dev)
         self.pf_last = torch.zeros(self.pf_rows, dtype=i32, device=dev)
@@ -524,6 +538,17 @@ class FastEngine:
         as one blob [K / V, kv head, layer, Lp, hd] that a8_state_rows snapshots from the scratch row and loads into
         slots."""
         st = self.slow
+        if st.kv4 is not None:
+            # whole records (16 positions, K and V): the last may hold positions past Lp, which the slot's own overwrite
+            rec = 18 * st.hd
+            row = -(-st.cache_len // 16) * rec
+            size = -(-Lp // 16) * rec
+            segs = [L.A8StateSeg(base=st.kv4.buf.data_ptr() + h * row, slot_stride=st.nkv * row, chunk_bytes=size,
+                                 chunk_stride=st.cache_rows * st.nkv * row, nchunks=st.layers,
+                                 blob_off=h * st.layers * size) for h in range(st.nkv)]
+            raw = bytes((L.A8StateSeg * len(segs))(*segs))
+            return (torch.frombuffer(bytearray(raw), dtype=torch.uint8).to(self.dev), len(segs),
+                    st.nkv * st.layers * size)
         es = 2
         per_pos = st.hd * es
         segs, off = [], 0

@@ -310,6 +310,10 @@ typedef struct A8StackDesc {
   void* kc;             /* bf16 [layers, cache_rows, nkv, cache_len, hd] */
   void* vc;
   int cache_rows, cache_len, ring;   /* ring 0: positions stored at pos, else at pos % ring */
+  void* kv4;            /* the caches in 4 bits instead (A8KV4 with these layers, cache_rows, nkv, hd, cache_len; kc and vc
+                           are unused then), or NULL. The q, k and v rows pass through scratch.mlp, so
+                           (nq + 2 nkv) hd <= inter; scratch.attn_ws and attn_counters hold a8_kv4_attention's workspace.
+                           No query blocks with a ring */
 } A8StackDesc;
 
 typedef struct A8StackRun {
