@@ -66,6 +66,9 @@ struct Kv4StoreArgs {
   int ldq;
 };
 
+// Bound: at many rows by memory with the quantiser's instructions right behind it (16,381 rows of 48 heads, hd 128: 354 MB in
+// 73 us, 4.8 TB/s); a tick's 192 rows by the launch, 2.4 us. Warps of query heads alone skip the quantiser.
+
 // The 8 codes of this thread's dims (w: bf16 pairs; nibble n = dim n) and the scale of the group that they share with the
 // other three lanes of the aligned four. rint(x / s) without a division an element: x (1 / s) is off by under 2^-21 of
 // itself, and snapped to a multiple of 2^-10 it is on the right side of every border: a quotient that is not on the
@@ -217,6 +220,8 @@ __device__ __forceinline__ uint4 kv4_deq8(uint32_t w, uint32_t s_low) {
                     __byte_perm(v[2], v[3], 0x7632));
 }
 
+// The inverse map, one thread the same 8 + 8 dims of a row's K and V head: bound by memory (65,533 rows x 8 heads, hd 128:
+// 344 MB in 57 us, 6.1 TB/s, 0.93 of a copy's rate); streaming stores and more rows a thread changed nothing.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv4_load(const Kv4LoadArgs a) {
   using F = Kv4<HD>;
@@ -277,17 +282,22 @@ struct Kv4AttnArgs {
 
 constexpr int KV4_CTAS = 148;         // one a SM
 constexpr int KV4_STEP = 32;           // positions a warp takes at a time: two records
-constexpr int KV4_CTA_STEPS = 24;      // fewer steps than CTAs x this: fewer CTAs
+// Fewer steps than CTAs x this: fewer CTAs, so that short work is joined within a CTA. Measured with 12, 16, 24, 36, 48: one
+// row of 733 keys (two heads of 23 steps) 12.8, 12.9, 9.9, 9.9, 11.3 us; 192 rows x 8 heads of 1 to 128 keys 15.9, 16.0, 16.0,
+// 16.8, 19.6; long ones the same.
+constexpr int KV4_CTA_STEPS = 24;
+constexpr int KV4_WHOLE = 8;          // a unit of at most so many steps is not cut between warps
 constexpr float KV4_LAZY = 8.f;       // a running maximum moves when a logit passes it by 2^8
 
 template <int HD, int NT>
 struct Kv4DecSmem {
-#ifndef KB
-#define KB 12
-#define KBS 3
-#endif
-  static constexpr int NW = HD == 64 ? 16 : NT == 1 ? KB : 8;     // warps (each holds O [hd][8 NT] in registers)
-  static constexpr int NST = HD == 64 ? 4 : NT == 1 ? KBS : 3;                    // steps in flight a warp
+  // Warps: as many as their registers (O [hd][8 NT], the queries, a record's scores) leave without spilling in the loop.
+  // hd 64, 192 rows of 1 to 2,047 keys: 16 warps (128 registers) 22 us, 20, 24 and 28 no better. hd 128, 3 rows x 8 heads of
+  // 40,009 to 131,071 keys: 8 warps 106 us, 10 123 (the SM's quarters are uneven), 12 101, 14 121 and 16 114 (spills).
+  static constexpr int NW = HD == 64 ? 16 : NT == 1 ? 12 : 8;
+  // Steps in flight a warp: 148 SMs x 16 x 4 x 2.3 KB or 12 x 3 x 4.6 KB are 22 to 24 MB, well above what 6.5 TB/s times
+  // the latency of a load (about 1 us) asks for; what shared memory holds beside the partials.
+  static constexpr int NST = HD == 64 ? 4 : 3;
   static constexpr int RING = NST * 2 * Kv4<HD>::REC;
   static constexpr int PART = (8 * NT * HD + 16 * NT) * 4;        // bytes: O [8 NT][hd], (max, sum) [8 NT]
   static constexpr int HEADP = NW * RING;                         // first partials; the last ones go into the rings
@@ -384,14 +394,25 @@ __device__ __forceinline__ void kv4_cursor_next(const Kv4AttnArgs& a, Kv4Cursor&
   kv4_cursor_unit<HD>(a, c, crow);
 }
 
-// The steps (32 positions, two records) of all rows and kv heads form one sequence; CTA b of G takes the b-th of G equal parts of it, its warps
-// equal parts of that: the work is even whatever the lengths. A warp runs through its steps alone (its own ring of bulk
-// copies, no barrier with the others) and writes the units that lie wholly in its part; what it has of the unit it begins
-// and the unit it ends within goes to shared memory, where the CTA joins its warps' pieces, and units that span CTAs are
-// joined, in order, by the CTA that comes last.
+// The steps (32 positions, two records) of all rows and kv heads form one sequence; CTA b of G takes the b-th of G equal
+// parts of it, its warps equal parts of that: the work is even whatever the lengths. A warp runs through its steps alone
+// (its own ring of bulk copies, no barrier with the others) and writes the units (a row's kv head) that lie wholly in its
+// part; what it has of the unit it begins and the unit it ends within goes to shared memory, where the CTA joins its warps'
+// pieces, and units that span CTAs are joined, in order, by the CTA that comes last.
 //   S = Q K^T (M: the query heads of the kv head, N: 8 keys), O^T = V^T P^T (M: 16 dims, K: 16 keys): the accumulator
-//   layout of S is the B operand of the second product. Scales: S gathers s_k(key, group) q.code per group in fp32; P is
-//   multiplied by s_v(key, group) in fp32 before its rounding to bf16.
+//   layout of S is the B operand of the second product, no exchange between lanes. Codes are operands as they stand: K's
+//   nibbles are masked to fp16 subnormals u 2^-24 (code + 8 = u: 8 times the query's sum is taken off each group's product
+//   in fp32, then it is scaled by s_k); V's become bf16 by a mask and a fused multiply-add; P is multiplied by s_v in fp32
+//   before its rounding to bf16. The query is fp16, scaled by a power of two (8 bits in 11).
+//   Running maximum per head, moved only when a logit passes it by 2^8 (then O and the sum are rescaled); sums and O fp32.
+// Why mma.sync and not tcgen05: up to 16 query heads share a kv head, a 128-row tile would be an eighth full at best, and
+// its operands would have to be written to shared memory as 16-bit values; here they never leave registers.
+// Bound: at long lengths by the instructions that unpack and scale and by their latency at four (three) warps a scheduler,
+// not by memory: hd 64 takes about 240 warp instructions a record (ALU 100, FMA 85), half of all issue slots of the
+// call below. 3 rows x 8 heads of 40,009 to 131,071 keys, hd 128: 407 MB in 101 us, 4.0 TB/s; 1,408 rows x 2 heads of 97 to
+// 911 keys, hd 64: 106 MB in 41 us, 2.6 TB/s. Short ones by latency: launch 2.5 us, lengths and the split 2.5, first
+// records and queries 1.5, joining 2.5, a cut unit's join 3 to 5: 192 rows of 1 to 2,047 keys 22 us, one row of 733 keys
+// 9.8, 192 rows x 8 heads of 1 to 128 keys (hd 128) 14.8.
 template <int HD, int NT>
 __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(const Kv4AttnArgs a) {
   using F = Kv4<HD>;
@@ -400,7 +421,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   extern __shared__ __align__(128) uint8_t smem[];
   int* pre = reinterpret_cast<int*>(smem + SM::PRE);
   int* meta = reinterpret_cast<int*>(smem + SM::META);
-  __shared__ int s_sum[32], s_runs, s_pieces, s_last[2];
+  __shared__ int s_sum[32], s_runs, s_pieces, s_last[2], s_split[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::BARS) + warp * NST;
   uint8_t* ring = smem + warp * SM::RING;
@@ -448,8 +469,8 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   pre[tid] = upto - s_sum[warp] + inc - mine;
   if (tid == 0) pre[NTHR] = total;
   __syncthreads();
-  const int T = total * a.c.nkv;                       // steps of all units
-  const int ctas = min((int)gridDim.x, (T + KV4_CTA_STEPS - 1) / KV4_CTA_STEPS);
+  int T = total * a.c.nkv;                             // steps of all units
+  int ctas = min((int)gridDim.x, (T + KV4_CTA_STEPS - 1) / KV4_CTA_STEPS);
   if ((int)blockIdx.x >= ctas) return;
   // the row that holds step x: its first step (at) and its steps a head (nb)
   auto locate = [&](int x, int& at, int& nb) {
@@ -470,20 +491,38 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
       }
     return r;
   };
-  // where CTA b's part begins: an equal share, moved to the nearer end of a unit that is small against it (a cut unit
-  // costs a pass through global memory and a ticket, about 4 us)
+  // Where CTA b's part begins: an equal share, moved to the nearer end of a unit that is small against it (at most half a
+  // share). A cut unit costs a pass through global memory and a ticket, 3 to 5 us, an uneven share less: measured at 192
+  // rows of 1 to 2,047 keys, 1,408 rows of 97 to 911 and 192 rows x 8 heads of 1 to 128: never moved 23.6, 45.1 and
+  // 20.7 us; up to an eighth of a share 24.0, 41.7, 20.1; a quarter 22.5, 41.7, 16.0; half 22.1, 41.6, 15.9.
+  // Then warp w's: the CTA's part in equal shares, moved likewise where units are few steps (joining a unit's pieces costs
+  // about 2.5 us, a step too many in a warp 0.5): 192 rows x 8 heads of 1 to 128 keys 15.9 us cut, 14.6 whole.
+  // (No part is empty: places a share apart move by at most a quarter of one.)
   const int share = T / ctas;
-  auto begin = [&](int b) {
-    const int x = int((long long)T * b / ctas);
-    if (b == 0 || b == ctas) return x;
+  auto moved = [&](int x, int most) {
     int at, nb;
     locate(x, at, nb);
     const int in = (x - at) % nb;
-    return 4 * nb > share ? x : 2 * in < nb ? x - in : x - in + nb;
+    return nb > most ? x : 2 * in < nb ? x - in : x - in + nb;
   };
-  const int b0 = begin(blockIdx.x), b1 = begin(blockIdx.x + 1);
-  const int w0 = b0 + int((long long)(b1 - b0) * warp / NW), w1 = b0 + int((long long)(b1 - b0) * (warp + 1) / NW);
+  auto begin = [&](int b) {
+    const int x = int((long long)T * b / ctas);
+    return b == 0 || b == ctas ? x : moved(x, share / 2);
+  };
+  int b0 = begin(blockIdx.x), b1 = begin(blockIdx.x + 1);
+  int w0 = b0 + int((long long)(b1 - b0) * warp / NW), w1 = b0 + int((long long)(b1 - b0) * (warp + 1) / NW);
+  if (T <= (long long)KV4_WHOLE * a.rows * a.c.nkv) {
+    if (warp > 0) w0 = max(b0, moved(w0, KV4_WHOLE));
+    if (warp < NW - 1) w1 = min(b1, moved(w1, KV4_WHOLE));
+  }
+  if (tid == 0) {                                      // (not in registers until the join)
+    s_split[0] = b0;
+    s_split[1] = b1;
+    s_split[2] = T;
+    s_split[3] = ctas;
+  }
   const int n = w1 - w0;
+  bool pieces = false;                                 // of units that other warps share
 
   if (n > 0) {
     // ---- where the warp's part begins
@@ -743,6 +782,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
         l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
       }
       const bool whole = seg == cc.nb;
+      pieces = pieces || !whole;
       const int piece = i == seg ? 0 : 1;              // the warp's first segment, or a later one (then its last)
       float* part = reinterpret_cast<float*>(piece == 0 ? smem + SM::HEADP + warp * SM::PART : ring);
 #pragma unroll
@@ -780,7 +820,11 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     if (!ok)                                           // a copy did not arrive: wait (bounded) for what is in flight
       for (int s = 0; s < NST; ++s) mbar_wait_all(&full[s], ph ^ (s < slot), ERR_TIMEOUT_FULL, KERNEL_ID_KV4_ATTN);
   }
-  __syncthreads();
+  if (!__syncthreads_or(pieces)) return;
+  b0 = s_split[0];
+  b1 = s_split[1];
+  T = s_split[2];
+  ctas = s_split[3];
 
   // ---- join the warps' pieces of each unit, in key order: the runs of pieces of one unit, each piece's weight
   int *runs = reinterpret_cast<int*>(smem + SM::RUNS), *list = runs + 4 * NW, *rof = list + 2 * NW;

@@ -686,3 +686,29 @@ def test_prompt_attention_between_gemms(kv4):
         g.replay()
     no_error(kv4)
     assert torch.equal(o, first_o) and torch.equal(y, first_y)
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 8, 128), (14, 2, 64), (16, 1, 64), (10, 1, 128)])
+@pytest.mark.parametrize("kind", ["windows", "at the border", "long among short", "one row"])
+def test_attention_units_of_few_steps(kv4, nq, nkv, hd, kind):
+    """Units (a row's kv head) of a few steps of 32 keys are kept whole in a warp, longer ones are cut: both, mixed, and at
+    the border between them."""
+    rows = {"windows": 192, "at the border": 100, "long among short": 150, "one row": 1}[kind]
+    g = torch.Generator().manual_seed(rows + nq)
+    lens = torch.randint(1, 129, (rows,), generator=g)
+    if kind == "at the border":
+        lens = torch.tensor([255, 256, 257, 288, 289, 32, 33, 1, 0, 224])[torch.randint(0, 10, (rows,), generator=g)]
+    elif kind == "long among short":
+        lens[torch.randint(0, rows, (4,), generator=g)] = 1111
+        lens[-1] = 700
+    lens = lens.tolist()
+    top, CR = max(lens), 7
+    c, kv = filled(kv4, 31 + nq, {r: top for r in range(CR)}, CR, nkv, hd, top + 3)
+    kv = {r: x.cuda() for r, x in kv.items()}
+    q = rnd(9000 + rows, rows, nq * hd, scale=1.5).cuda()
+    rowmap = torch.randint(0, CR, (rows,), generator=g).tolist()
+    got = c.attention(q, i32(lens), i32(rowmap), max_len=top).double().view(rows, nq, hd)
+    no_error(kv4)
+    want, tol = gpu_reference(q, kv, list(zip(rowmap, lens)), nq, nkv, hd)
+    d = (got - want).abs()
+    assert bool((d <= tol).all()), float((d - tol).max())
