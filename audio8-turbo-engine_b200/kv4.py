@@ -150,16 +150,23 @@ class KV4Cache:
         dev = self.dev.index
         if dev is None:
             _need(False, "the cache is not on a GPU (there is no CPU fallback)")
+        capturing = _capturing()
         key = _current_stream(dev)
         have = self._ws.get(key)
-        if have is None or nq > have[0] or rows > have[1] or max_len > have[2] or _capturing():
-            if _capturing():
-                return self.workspace(nq, rows, max_len)
+        if have is None or nq > have[0] or rows > have[1] or max_len > have[2] or capturing:
+            if capturing:
+                return self._pointers(self.workspace(nq, rows, max_len))
             if have is not None:
                 nq, rows, max_len = max(nq, have[0]), max(rows, have[1]), max(max_len, have[2])
             with torch.cuda.device(self.dev):
-                have = self._ws[key] = (nq, rows, max_len, *self.workspace(nq, rows, max_len))
-        return have[3:]
+                have = self._ws[key] = (nq, rows, max_len, self._pointers(self.workspace(nq, rows, max_len)))
+        return have[3]
+
+    @staticmethod
+    def _pointers(ws):
+        """A workspace as the C call takes it, and the tensors themselves (to keep)."""
+        w, t = ws
+        return w.data_ptr(), w.numel(), t.data_ptr(), t.numel(), ws
 
     def attention(self, q, lens, rowmap=None, *, layer: int = 0, max_len: int = 0, scale: float = 0.0, out=None, ws=None):
         """Decode attention: q bf16 [rows, nq hd], row r over keys [0, min(lens[r], max_len)) of cache row rowmap[r]
@@ -171,9 +178,9 @@ class KV4Cache:
         plens = self._ints(lens, rows, "lens")           # (the tensors stay referenced until the launch)
         pmap = None if rowmap is None else self._ints(rowmap, rows, "rowmap")
         if rows:
-            w, t = ws if ws is not None else self._workspace(nq, rows, max_len)
+            pw, nw, pt, nt, held = self._workspace(nq, rows, max_len) if ws is None else self._pointers(ws)
             self._call(self._lib.a8_kv4_attention, layer, q.data_ptr(), ldq, nq, plens, pmap, rows, max_len, scale,
-                       out.data_ptr(), ldo, w.data_ptr(), w.numel(), t.data_ptr(), t.numel())
+                       out.data_ptr(), ldo, pw, nw, pt, nt)
         return out
 
     def _queries(self, q, out):
