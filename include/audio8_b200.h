@@ -156,10 +156,10 @@ long long a8_kv4_bytes(const A8KV4* c);
  * A8_EPI_BF16 and a bias gives), at position pos[r] of cache row slot[r] (NULL: r); with ring > 0 the cache position is
  * pos % ring. cos / sin bf16 [npos, hd] rotate_half tables (both halves alike) rotate q and k at pos in fp32, rounded once
  * to bf16; NULL: no rotation. q_out [rows, ldq] receives the query heads (it may be qkv itself with ldq = ld, else it does
- * not overlap it); nq = 0: k and v only, q_out unused. A row with pos < 0 is padding: nothing of it is written. A row whose cache row,
- * cache position or table row is out of range is not written and records ERR_BOUNDS (a8_get_error). Rows of one call that
- * share a cache row and position leave either row's codes or scales there (finite values; give a position once). Pointers
- * 16-byte aligned, ld and ldq multiples of 8. The counterpart of A8_EPI_ROPE for this cache. */
+ * not overlap it); nq = 0: k and v only, q_out unused. A row with pos < 0 is padding: nothing of it is written. A row whose
+ * cache row, cache position or table row is out of range is not written and records ERR_BOUNDS (a8_get_error). Rows of one
+ * call that share a cache row and position leave either row's codes or scales there (finite values; give a position once).
+ * Pointers 16-byte aligned, ld and ldq multiples of 8. The counterpart of A8_EPI_ROPE for this cache. */
 int a8_kv4_store(const A8KV4* c, int layer, const void* qkv, int ld, int nq, const void* cos, const void* sin, int npos,
                  const int* pos, const int* slot, int rows, int ring, void* q_out, int ldq, a8_stream_t stream);
 
@@ -176,9 +176,9 @@ int a8_kv4_attention_workspace(const A8KV4* c, int nq, int rows, int max_len, lo
  * cache row rowmap[r] (NULL: r), kv head h / (nq / nkv), L_r = min(lens[r], max_len). q / out bf16 [rows, stride] (16-byte
  * aligned, strides multiples of 8), nq / nkv from 1 to 16. L_r <= 0 gives zeros. A row whose cache row is out of range
  * gives zeros and records ERR_BOUNDS. scale <= 0: hd^-0.5. out may be q (of the same stride), else it does not overlap
- * it. counters: n_counters ints, zero before the first call (a call leaves them zero; after a recorded timeout, zero them again); ws (16-byte aligned) and counters
- * belong to one call at a time. The order of every sum depends only on the shape, lens, cache rows and max_len of a call, so
- * equal calls give equal bits. */
+ * it. counters: n_counters ints, zero before the first call (a call leaves them zero; after a recorded timeout, zero them
+ * again); ws (16-byte aligned) and counters belong to one call at a time. The order of every sum depends only on the shape,
+ * lens, cache rows and max_len of a call, so equal calls give equal bits. */
 int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* lens, const int* rowmap,
                      int rows, int max_len, float scale, void* out, int out_stride, float* ws, long long ws_floats,
                      int* counters, int n_counters, a8_stream_t stream);
