@@ -409,7 +409,7 @@ __device__ __forceinline__ void kv4_cursor_next(const Kv4AttnArgs& a, Kv4Cursor&
 // its operands would have to be written to shared memory as 16-bit values; here they never leave registers.
 // Bound: at long lengths by the instructions that unpack and scale and by their latency at four (three) warps a scheduler,
 // not by memory: hd 64 takes about 240 warp instructions a record (ALU 100, FMA 85), half of all issue slots of the
-// call below. 3 rows x 8 heads of 40,009 to 131,071 keys, hd 128: 407 MB in 101 us, 4.0 TB/s; 1,408 rows x 2 heads of 97 to
+// call below. 3 rows x 8 heads of 40,009 to 131,071 keys, hd 128: 407 MB in 100 us, 4.1 TB/s; 1,408 rows x 2 heads of 97 to
 // 911 keys, hd 64: 106 MB in 41 us, 2.6 TB/s. Short ones by latency: launch 2.5 us, lengths and the split 2.5, first
 // records and queries 1.5, joining 2.5, a cut unit's join 3 to 5: 192 rows of 1 to 2,047 keys 22 us, one row of 733 keys
 // 9.8, 192 rows x 8 heads of 1 to 128 keys (hd 128) 14.8.
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   int* pre = reinterpret_cast<int*>(smem + SM::PRE);
   int* meta = reinterpret_cast<int*>(smem + SM::META);
   __shared__ int s_sum[32], s_runs, s_pieces, s_last[2], s_split[4];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::BARS) + warp * NST;
   uint8_t* ring = smem + warp * SM::RING;
   pdl_launch();

@@ -13,14 +13,16 @@
 // multiplies back into its logit scale; V by 2^E, the largest scale met so far, which joins the running maximum's factor
 // on O when it grows; a query vector by its own largest element. P is fp16 with weights up to 2^14 (the running maximum
 // is moved only when a logit passes it by 2^8), rounded to 11 bits; sums and O in fp32.
-// Bound: 8,189 positions, 32 heads over 8, hd 128: 549 GFLOP in 656 us, 838 TFLOP/s, half of a library product's rate. A key
-// tile takes its CTA about 1.47 us, 2,800 cycles, and no one unit is full in them: the products take 1,280 (S, with both
+// Bound: 8,189 positions, 32 heads over 8, hd 128: 549 GFLOP in 606 to 629 us, 890 TFLOP/s, 0.53 of a library product's rate. A key
+// tile takes its CTA about 1.38 us, 2,700 cycles, and no one unit is full in them: the products take 1,280 (S, with both
 // operands in shared memory, 48 an instruction where its arithmetic takes 32; P V 64), the 256 x 64 exponentials 1,024, and
 // the issue slots of 8 softmax and 8 unpacking warps the most. An admission (2,048 ragged rows behind prefixes of 317, 14
 // heads over 2, hd 64) takes 21 to 29 us, as long as its longest prompt's last block and the filling of the pipeline.
 // Measured and not kept: exponentials as polynomials on the FMA pipe for 1/4, 1/2, 3/4 of the weights (707, 740, 998 us
 // against 693 then: issue slots are short, not the exponentials' unit). On the way: S and P V issued by one warp 905 us, by
-// two 693; every tile's maximum before its weights 693, only where their sum asks for it 673.
+// two 693; every tile's maximum before its weights 693, only where their sum asks for it 673; warp indexes that the compiler
+// cannot see are uniform 650, shuffled from one lane 620; the second half of S fetched behind the first half's weights 684
+// against 646; the two tiles' softmax started half a tile apart no gain.
 // Within a chunk of eight dims Q and K keep the order 0 4 1 5 2 6 3 7, in which the codes come out of their words.
 #include "common.cuh"
 
@@ -150,7 +152,8 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
            *p_free = p_full + 4;                         // the last three: [tile][stage]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_free + 4);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // (the warp's index from one lane: barrier addresses and branches are uniform to the compiler)
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   pdl_wait();
   // the last blocks first, all their heads together: they attend the most keys of a prompt
   const int hq = (a.group + 3) / 4, per = a.c.nkv * hq;
@@ -437,10 +440,11 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       for (int j = max(0, issued - KV4P_RAW); j < issued; ++j)
         mbar_wait(&raw_full[j % KV4P_RAW], (j / KV4P_RAW) & 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
     }
-    // a whole warp walks each issue loop (ring positions and descriptors stay warp-uniform), one elected lane issues
+    // a whole warp walks each issue loop (ring positions and descriptors stay warp-uniform), one lane, elected once, issues
     if (warp == 17) {
       constexpr uint32_t idS = umma_idesc(128, 64, 0);
       const uint64_t dQ = umma_desc_sw128(smem + SM::Q), dK = umma_desc_sw128(smem + SM::K);
+      const bool lead = elect_one();
       bool ok = mbar_wait_all(q_full, 0, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
       for (int j = 0; ok && j < nt; ++j) {
         const int st = j & 1, ph = (j >> 1) & 1;
@@ -450,7 +454,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
                      : kv4_wait2(&k_full[st], ph, &p_free[2 * x + st], ph ^ 1, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
           if (!ok) break;
           tc_fence_after();
-          if (elect_one()) {
+          if (lead) {
             const uint32_t d = tmem + x * 128 + st * 64;
             const uint64_t da = dQ + x * (SM::QT >> 4), db = dK + st * (SM::KT >> 4);
 #pragma unroll
@@ -466,6 +470,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
     } else if (warp == 18) {
       constexpr uint32_t idO = umma_idesc(128, HD, 0);
       const uint64_t dV = umma_desc_sw128(smem + SM::V);
+      const bool lead = elect_one();
       int vt = 0, vph = 0;
       for (int j = 0; j < nt; ++j) {
         const int st = j & 1;
@@ -474,7 +479,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
           ok = kv4_wait2(&p_full[2 * x + st], (j >> 1) & 1, &v_full[vt], vph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL);
           if (!ok) break;
           tc_fence_after();
-          if (elect_one()) {
+          if (lead) {
             const uint64_t db = dV + vt * (SM::VT >> 4);
             const uint32_t d = tmem + 256 + x * HD, ta = tmem + x * 128 + st * 64;
 #pragma unroll
