@@ -178,6 +178,10 @@ class KV4Cache:
         plens = self._ints(lens, rows, "lens")           # (the tensors stay referenced until the launch)
         pmap = None if rowmap is None else self._ints(rowmap, rows, "rowmap")
         if rows:
+            if ws is not None:
+                _need(ws[0].dtype is torch.float32 and ws[1].dtype is I32 and ws[0].device == ws[1].device == self.dev
+                      and ws[0].is_contiguous() and ws[1].is_contiguous(),
+                      f"ws: the (float32, int32) tensors of workspace() on {self.dev}")
             pw, nw, pt, nt, held = self._workspace(nq, rows, max_len) if ws is None else self._pointers(ws)
             self._call(self._lib.a8_kv4_attention, layer, q.data_ptr(), ldq, nq, plens, pmap, rows, max_len, scale,
                        out.data_ptr(), ldo, pw, nw, pt, nt)

@@ -712,3 +712,24 @@ def test_attention_units_of_few_steps(kv4, nq, nkv, hd, kind):
     want, tol = gpu_reference(q, kv, list(zip(rowmap, lens)), nq, nkv, hd)
     d = (got - want).abs()
     assert bool((d <= tol).all()), float((d - tol).max())
+
+
+def test_attention_with_a_workspace_of_the_callers(kv4):
+    """The caller's workspace serves smaller calls too, comes back ready for the next, and is refused when it is too small
+    or not what workspace() gives."""
+    nq, nkv, hd, lens = 14, 2, 64, [1900, 0, 700, 1]
+    c, kv = filled(kv4, 12, dict(enumerate(lens)), 4, nkv, hd, 2000)
+    q = rnd(150, 4, nq * hd, scale=1.5)
+    ws = c.workspace(nq, 4, 2000)
+    want = c.attention(q.cuda(), i32(lens))
+    for n in (4, 2, 4):
+        got = c.attention(q[:n].cuda(), i32(lens[:n]), ws=ws, max_len=2000)
+        no_error(kv4)
+        assert torch.equal(got, c.attention(q[:n].cuda(), i32(lens[:n]))) and not bool(ws[1].any())
+    assert torch.equal(got, want)
+    check_rows(got, q, kv, [(r, 1, r, n - 1) for r, n in enumerate(lens)], nq, nkv, hd)
+    for bad in ((ws[0][:8], ws[1]), (ws[0], ws[1][:7]), (ws[0].double(), ws[1]), (ws[0], ws[1].long()),
+                (ws[0].cpu(), ws[1]), (ws[0][::2], ws[1])):
+        with pytest.raises(kv4.A8Error):
+            c.attention(q.cuda(), i32(lens), ws=bad)
+    assert torch.equal(want, c.attention(q.cuda(), i32(lens)))
