@@ -291,10 +291,11 @@ constexpr float KV4_LAZY = 8.f;       // a running maximum moves when a logit pa
 
 template <int HD, int NT>
 struct Kv4DecSmem {
-  // Warps: as many as their registers (O [hd][8 NT], the queries, a record's scores) leave without spilling in the loop.
+  // Warps: as many as their registers (O [hd][8 NT], the queries, a record's scores) leave with little or no spilling.
   // hd 64, 192 rows of 1 to 2,047 keys: 16 warps (128 registers) 22 us, 20, 24 and 28 no better. hd 128, 3 rows x 8 heads of
   // 40,009 to 131,071 keys: 8 warps 106 us, 10 123 (the SM's quarters are uneven), 12 101, 14 121 and 16 114 (spills).
-  static constexpr int NW = HD == 64 ? 16 : NT == 1 ? 12 : 8;
+  // More than 8 query heads a kv head (NT 2), hd 64, 1,000 rows x 2 heads of 1 to 2,047 keys: 12 warps 67.4 us, 16 69.6 (spills).
+  static constexpr int NW = HD == 64 ? (NT == 1 ? 16 : 12) : NT == 1 ? 12 : 8;
   // Steps in flight a warp: 148 SMs x 16 x 4 x 2.3 KB or 12 x 3 x 4.6 KB are 22 to 24 MB, well above what 6.5 TB/s times
   // the latency of a load (about 1 us) asks for; what shared memory holds beside the partials.
   static constexpr int NST = HD == 64 ? 4 : 3;
