@@ -247,7 +247,8 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       tc_fence_after();
       float sv[64];
       tmem_ld64(tS + (j & 1) * 64, sv);
-      const float f = qs * pow2_biased(ek[j & 15]);
+      // (never 0, which would make a masked -infinity NaN; at this least value every logit is below 2^-110)
+      const float f = fmaxf(qs * pow2_biased(ek[j & 15]), 0x1p-126f);
       const int Ej = ev[j & 15];
       const int kmax = pos - 64 * j;                     // keys c <= kmax of this tile are causal for this row
       if (__any_sync(0xffffffffu, kmax < 63)) {

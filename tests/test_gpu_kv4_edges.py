@@ -1,0 +1,95 @@
+"""Calls of the 4-bit cache's operators that its other tests do not make, on the GPU: degenerate and tiny queries and keys,
+against the 64-bit definition (oracle/kv4_ref.py) under its derived bounds."""
+import pytest
+import torch
+
+from oracle import kv4_ref as R
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+I32 = torch.int32
+
+
+@pytest.fixture(scope="module")
+def kv4(a8):
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    a8.load()
+    a8._lib.call("a8_clear_error")
+    return a8
+
+
+def no_error(a8):
+    torch.cuda.synchronize()
+    assert a8.device_error()[0] == 0, a8.device_error()
+
+
+def rnd(seed, *shape, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(BF)
+
+
+def one_row(a8, x, hd):
+    """A cache of one row that holds x [n, 2, nkv, hd] at positions 0 .. n - 1."""
+    n, _, nkv, _ = x.shape
+    c = a8.KV4Cache(1, nkv, hd, n)
+    c.store(x.reshape(n, -1).cuda(), torch.arange(n, dtype=I32).cuda(), torch.zeros(n, dtype=I32).cuda())
+    return c
+
+
+def prompt(a8, c, q, n, **kw):
+    blocks = torch.from_numpy(a8.FastEngine.query_blocks(list(range(n)), [0] * n)).cuda()
+    out = c.prefill_attention(q.cuda(), blocks, **kw)
+    no_error(a8)
+    return out.cpu().double()
+
+
+def check_prompt(a8, x, q, hd, scale=None):
+    """All n causal rows of q [n, nq hd] over x against the definition."""
+    n, nkv, nq = x.shape[0], x.shape[2], q.shape[1] // hd
+    got = prompt(a8, one_row(a8, x, hd), q, n, scale=scale or 0.0).view(n, nq, hd)
+    kv, qd, scale = R.values(x), q.double().view(n, nq, hd), scale or hd ** -0.5
+    for h in range(nq):
+        k, v = kv[:, 0, h * nkv // nq], kv[:, 1, h * nkv // nq]
+        o, tol = R.attention(qd[:, h], k, v, 0, scale)
+        tol = tol + R.prompt_slack(qd[:, h], k, v, 0, scale)
+        d = (got[:, h] - o).abs()
+        assert bool((d <= tol).all()), (h, float((d - tol).max()), int(got.isnan().sum()))
+
+
+# ------------------------------------------------------------------------------------------------- logits that vanish
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("qs,ks", [(0.0, 0.0), (0.0, 1.0), (0.0, 2.0 ** -30), (2.0 ** -30, 0.0), (2.0 ** -75, 2.0 ** -75),
+                                   (1.0, 0.0), (2.0 ** -120, 2.0 ** -120)])
+def test_prompt_of_vanishing_logits_is_the_mean(kv4, hd, qs, ks):
+    """Queries and keys of nothing, or so small that their product underflows: every weight is the same, a row is the mean of
+    its values (over an empty cache, zero)."""
+    n, nq, nkv = 150, 4, 2
+    x = rnd(1, n, 2, nkv, hd)
+    x[:, 0] = (x[:, 0].float() * ks).to(BF)
+    check_prompt(kv4, x, (rnd(2, n, nq * hd).float() * qs).to(BF), hd)
+
+
+def test_prompt_of_an_empty_cache_is_zero(kv4):
+    nq, nkv, hd, n = 14, 2, 64, 100
+    c = kv4.KV4Cache(1, nkv, hd, n)
+    assert bool((prompt(kv4, c, torch.zeros(n, nq * hd, dtype=BF), n) == 0).all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_with_some_vanishing_rows_and_tiles(kv4, hd):
+    """Zero queries between others, a whole tile of zero keys between others."""
+    n, nq, nkv = 200, 4, 2
+    x, q = rnd(3, n, 2, nkv, hd), rnd(4, n, nq * hd)
+    x[64:128, 0] = 0
+    q[::3] = 0
+    q[100:140, :hd] = 0
+    check_prompt(kv4, x, q, hd)
+
+
+@pytest.mark.parametrize("scale", [1e-9, 1e-37])
+def test_prompt_of_a_tiny_scale(kv4, scale):
+    n, hd = 150, 64
+    x, q = rnd(5, n, 2, 2, hd), rnd(6, n, 4 * hd)
+    x[:64, 0] = (x[:64, 0].float() * 2.0 ** -60).to(BF)
+    q[::2] = 0
+    check_prompt(kv4, x, q, hd, scale)
