@@ -724,7 +724,8 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const uint32_t ex = max(top >> 7, 8u);
         const float up = __uint_as_float((261u - ex) << 23);
-        qs[u] = a.scale_log2 * __uint_as_float((ex - 7u) << 23) * 0x1p24f;
+        // (never 0, which would make a masked -infinity NaN)
+        qs[u] = fmaxf(a.scale_log2 * 0x1p24f * __uint_as_float((ex - 7u) << 23), 0x1p-126f);
 #pragma unroll
         for (int s = 0; s < G; ++s) {
           const float2 d01 = unpack_bf16(x[s].x), d23 = unpack_bf16(x[s].y), d45 = unpack_bf16(x[s].z),

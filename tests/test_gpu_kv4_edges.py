@@ -93,3 +93,25 @@ def test_prompt_of_a_tiny_scale(kv4, scale):
     x[:64, 0] = (x[:64, 0].float() * 2.0 ** -60).to(BF)
     q[::2] = 0
     check_prompt(kv4, x, q, hd, scale)
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(4, 2, 64), (4, 2, 128), (10, 1, 64)])
+@pytest.mark.parametrize("scale", [1e-8, 1e-9, 1e-30, 1e-37])
+def test_decode_of_a_tiny_scale(kv4, nq, nkv, hd, scale):
+    """Rows of zero, tiny and ordinary queries under a scale that leaves nothing of a logit: the mean of the values."""
+    n, rows = 77, 6
+    x, q = rnd(7, n, 2, nkv, hd), rnd(8, rows, nq * hd)
+    q[::2] = 0
+    q[1] = (q[1].float() * 2.0 ** -100).to(BF)
+    lens = [n, n, 33, 70, 1, 40]
+    c = one_row(kv4, x, hd)
+    got = c.attention(q.cuda(), torch.tensor(lens, dtype=I32, device="cuda"), torch.zeros(rows, dtype=I32, device="cuda"),
+                      scale=scale)
+    no_error(kv4)
+    got, kv, qd = got.cpu().double().view(rows, nq, hd), R.values(x), q.double().view(rows, nq, hd)
+    for r, m in enumerate(lens):
+        for h in range(nq):
+            k, v = kv[:m, 0, h * nkv // nq], kv[:m, 1, h * nkv // nq]
+            o, tol = R.attention(qd[r:r + 1, h], k, v, m - 1, scale)
+            d = (got[r:r + 1, h] - o).abs()
+            assert bool((d <= tol).all()), (r, h, float((d - tol).max()))
