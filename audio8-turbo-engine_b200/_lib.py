@@ -38,7 +38,7 @@ class A8StackDesc(C.Structure):
                 ("eps", c_float), ("wqkv", c_void_p), ("bqkv", c_void_p), ("wo", c_void_p), ("w13", c_void_p),
                 ("w2", c_void_p), ("ln1", c_void_p), ("ln2", c_void_p), ("norm", c_void_p), ("cos", c_void_p),
                 ("sin", c_void_p), ("kc", c_void_p), ("vc", c_void_p), ("cache_rows", c_int), ("cache_len", c_int),
-                ("ring", c_int), ("kv4", c_void_p)]
+                ("ring", c_int)]
 
 
 class A8StackRun(C.Structure):

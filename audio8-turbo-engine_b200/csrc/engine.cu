@@ -61,13 +61,14 @@ int stack_forward(const A8StackDesc& d, const A8StackRun& r, cudaStream_t s) {
   void* res = r.x;
   const bool fuse = sc.ssq != nullptr && sc.ssq_ld >= R && D <= 1024 && D % 64 == 0;
   a8_stream_t st = reinterpret_cast<a8_stream_t>(s);
+  const bool four = d.vc == nullptr;            // the caches in 4 bits, at kc
+  const A8KV4 kv4 = {d.kc, d.layers, d.cache_rows, d.nkv, d.hd, d.cache_len};
+  if (d.kc == nullptr) return A8_ERR_ARG;
+  if (four && NQKV > d.inter) return A8_ERR_SIZE;
+  if (four && d.ring > 0 && r.nblocks > 0) return A8_ERR_ARG;   // (the prompt form reads position p at p)
   A8_TRY(a8_rmsnorm(r.x, r.ldx, nullptr, 0, d.ln1, h, D, R, D, d.eps, st));
   CUtensorMap mk, mv;
   const long long total = (long long)d.layers * d.cache_rows * d.nkv * d.cache_len;
-  const bool four = d.kv4 != nullptr;           // the caches in 4 bits
-  const A8KV4 kv4 = {d.kv4, d.layers, d.cache_rows, d.nkv, d.hd, d.cache_len};
-  if (four && NQKV > d.inter) return A8_ERR_SIZE;
-  if (four && d.ring > 0 && r.nblocks > 0) return A8_ERR_ARG;   // (the prompt form reads position p at p)
   if (!four) A8_TRY(attn_maps(&mk, &mv, d.kc, d.vc, total, d.hd));
   const int max_len = r.max_len > 0 ? r.max_len : d.cache_len;
   // packed prefill rows with a query-block table go to the tensor-core prefill attention

@@ -108,9 +108,9 @@ class PackedStack:
         self.desc = L.A8StackDesc(
             layers=nl, dim=self.dim, nq=nq, nkv=nkv, hd=hd, inter=self.inter, eps=self.eps, wqkv=L.ptr(self.wqkv),
             bqkv=L.ptr(self.bqkv), wo=L.ptr(self.wo), w13=L.ptr(self.w13), w2=L.ptr(self.w2), ln1=L.ptr(self.ln1),
-            ln2=L.ptr(self.ln2), norm=L.ptr(self.norm), cos=L.ptr(self.cos), sin=L.ptr(self.sin), kc=L.ptr(self.kc),
-            vc=L.ptr(self.vc), cache_rows=cache_rows, cache_len=cache_len, ring=self.ring,
-            kv4=None if self.kv4 is None else L.ptr(self.kv4.buf))
+            ln2=L.ptr(self.ln2), norm=L.ptr(self.norm), cos=L.ptr(self.cos), sin=L.ptr(self.sin),
+            kc=L.ptr(self.kc if self.kv4 is None else self.kv4.buf), vc=L.ptr(self.vc), cache_rows=cache_rows,
+            cache_len=cache_len, ring=self.ring)
 
 
 class Scratch:

@@ -307,13 +307,12 @@ typedef struct A8StackDesc {
   const void* norm;     /* bf16 [dim] */
   const void* cos;      /* bf16 [npos, hd] */
   const void* sin;      /* bf16 [npos, hd] */
-  void* kc;             /* bf16 [layers, cache_rows, nkv, cache_len, hd] */
-  void* vc;
+  void* kc;             /* bf16 [layers, cache_rows, nkv, cache_len, hd], or (vc NULL) the caches in 4 bits: the buffer of
+                           an A8KV4 with these layers, cache_rows, nkv, hd and cache_len. The q, k and v rows pass through
+                           scratch.mlp then, so (nq + 2 nkv) hd <= inter; scratch.attn_ws and attn_counters hold
+                           a8_kv4_attention's workspace. No query blocks with a ring */
+  void* vc;             /* bf16, as kc; NULL: kc is a 4-bit cache */
   int cache_rows, cache_len, ring;   /* ring 0: positions stored at pos, else at pos % ring */
-  void* kv4;            /* the caches in 4 bits instead (A8KV4 with these layers, cache_rows, nkv, hd, cache_len; kc and vc
-                           are unused then), or NULL. The q, k and v rows pass through scratch.mlp, so
-                           (nq + 2 nkv) hd <= inter; scratch.attn_ws and attn_counters hold a8_kv4_attention's workspace.
-                           No query blocks with a ring */
 } A8StackDesc;
 
 typedef struct A8StackRun {
@@ -327,7 +326,7 @@ typedef struct A8StackRun {
   const int* rowmap;    /* int32 [rows] cache row attended (NULL: the row index) */
   int max_len;          /* bound of any row's keys (0: cache_len); sets the split count */
   A8Scratch scratch;    /* output in scratch.h */
-  const int* blocks;    /* packed causal prefill (hd 64): int32 [nblocks][4] query blocks as a8_prefill_attention
+  const int* blocks;    /* packed causal prefill (hd 64; 64 or 128 on a 4-bit cache): int32 [nblocks][4] query blocks as a8_prefill_attention
                            (pos / slot must agree); NULL: every row by the decode attention */
   int nblocks;
 } A8StackRun;

@@ -1,0 +1,55 @@
+"""The 4-bit cache's entry points on the CPU: calls at the edges of what their arguments allow. Nothing is launched."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+import torch
+
+from conftest import REPO
+
+ARG, CUDA, ALIGN, SIZE, OK = 1, 2, 3, 4, 0
+
+
+@pytest.fixture(scope="module")
+def L(a8):
+    a8.load()
+    return a8._lib
+
+
+# A8StackDesc as callers of a bf16 cache have it compiled in
+STACK = """typedef struct { int layers, dim, nq, nkv, hd, inter; float eps; const void *wqkv, *bqkv, *wo, *w13, *w2, *ln1, *ln2,
+*norm, *cos, *sin; void *kc, *vc; int cache_rows, cache_len, ring; } Stack;"""
+
+
+def test_stack_struct_is_the_bf16_cache_s(L, tmp_path):
+    """A 4-bit cache is told by vc NULL, not by a field behind the struct that a caller compiled before it does not have."""
+    import shutil
+    assert [f[0] for f in L.A8StackDesc._fields_][-3:] == ["cache_rows", "cache_len", "ring"]
+    if shutil.which("gcc") is None:
+        pytest.skip("no C compiler")
+    src = tmp_path / "s.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "audio8_b200.h"\n' + STACK + "\nint main(void)"
+                   '{printf("%d %d %zu", sizeof(Stack) == sizeof(A8StackDesc), offsetof(Stack, ring) == '
+                   'offsetof(A8StackDesc, ring), sizeof(A8StackDesc));return 0;}')
+    subprocess.run(["gcc", "-I", os.path.join(REPO, "include"), str(src), "-o", str(tmp_path / "s")], check=True)
+    out = subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split()
+    assert out == ["1", "1", str(C.sizeof(L.A8StackDesc))]
+
+
+def test_stack_refuses_before_it_launches(L):
+    """No cache at all; with a 4-bit one, an MLP too narrow for the q, k and v rows, and query blocks with a ring."""
+    p = C.c_void_p(256)
+
+    def run(nblocks=0, **kw):
+        d = dict(layers=1, dim=896, nq=14, nkv=2, hd=64, inter=4864, eps=1e-6, kc=p, vc=None, cache_rows=1, cache_len=64,
+                 ring=0)
+        d.update(kw)
+        r = L.A8StackRun(x=p, ldx=896, rows=1, pos=p, blocks=p if nblocks else None, nblocks=nblocks)
+        before = L.load().a8_launch_count()
+        rc = L.load().a8_stack_forward(C.byref(L.A8StackDesc(**d)), C.byref(r), None)
+        assert L.load().a8_launch_count() == before
+        return rc
+    assert run(kc=None) == ARG and run(kc=None, vc=p) == ARG
+    assert run(inter=1088) == SIZE
+    assert run(ring=32, nblocks=1) == ARG
