@@ -1028,11 +1028,16 @@ static cudaError_t kv4_launch(const void* fn, dim3 grid, int threads, size_t sme
   return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
-// Dynamic shared memory above 48 KB is a kernel's attribute on each device: set once a device (bit of `ready`).
-static bool kv4_smem_ready(std::atomic<uint64_t>& ready, const void* fn, int bytes) {
+// Dynamic shared memory above 48 KB is a kernel's attribute on each device: set once a device (bit of `ready`), and the
+// registers that the kernel was compiled to looked at, where it depends on them.
+static bool kv4_ready(std::atomic<uint64_t>& ready, const void* fn, int bytes, bool (*registers)(int) = nullptr) {
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
   if (ready.load(std::memory_order_relaxed) >> dev & 1) return true;
+  if (registers != nullptr) {
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess || !registers(fa.numRegs)) return false;
+  }
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
   ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   return true;
@@ -1176,7 +1181,7 @@ static int kv4_attn_launch(Kv4AttnArgs& a, int ctas, cudaStream_t s) {
   using SM = Kv4DecSmem<HD, NT>;
   const void* fn = (const void*)k_kv4_attn<HD, NT>;
   static std::atomic<uint64_t> ready{0};
-  if (!kv4_smem_ready(ready, fn, SM::TOTAL)) return A8_ERR_CUDA;
+  if (!kv4_ready(ready, fn, SM::TOTAL)) return A8_ERR_CUDA;
   void* args[] = {&a};
   return kv4_launch(fn, dim3(ctas), SM::NW * 32, SM::TOTAL, args, s) == cudaSuccess ? A8_OK : A8_ERR_CUDA;
 }

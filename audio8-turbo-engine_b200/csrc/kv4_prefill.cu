@@ -30,9 +30,15 @@ namespace a8 {
 
 constexpr int KERNEL_ID_KV4_PREFILL = 12;
 constexpr int KV4P_SOFT = 8, KV4P_DEQ = 4;               // softmax warps; warps of each of K and V
-constexpr int KV4P_THREADS = (KV4P_SOFT + 2 * KV4P_DEQ + 4) * 32;   // five warpgroups (the last: warps 16, 17 and two idle)
+constexpr int KV4P_THREADS = (KV4P_SOFT + 2 * KV4P_DEQ + 4) * 32;   // five warpgroups (the last: warps 16 to 19)
 // Registers a thread after the warpgroups' redistribution: 256 x 144 + 256 x 64 + 128 x 64, all of the 640 x 96 = 61,440
-// that the block is launched with.
+// that the block is launched with. A compiler that gave the kernel fewer would leave the softmax warps waiting for registers
+// that never come free, so the host looks at what it gave before the first launch.
+constexpr int KV4P_REG_SOFT = 144, KV4P_REG_REST = 64;
+constexpr bool kv4p_registers_cover(int per_thread) {
+  return per_thread * KV4P_THREADS >= KV4P_SOFT * 32 * KV4P_REG_SOFT + (2 * KV4P_DEQ + 4) * 32 * KV4P_REG_REST;
+}
+static_assert(kv4p_registers_cover(96), "");
 #define A8_SETMAXNREG(op, n) asm volatile("setmaxnreg." op ".sync.aligned.u32 %0;" ::"n"(n))
 constexpr int KV4P_RAW = 6;                              // raw key tiles in flight
 constexpr int KV4P_VST = 3;                              // V tiles at hand
@@ -203,7 +209,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
   pdl_launch();
 
   if (warp < KV4P_SOFT) {
-    A8_SETMAXNREG("inc", 144);
+    A8_SETMAXNREG("inc", KV4P_REG_SOFT);
     // ---- softmax: thread = query vector (head 2 x + half, position pos0 + r)
     const int x = warp >> 2, row = (warp & 3) * 32 + lane, r = row & 63, hi = row >> 6;
     const int head = 2 * x + hi;
@@ -337,7 +343,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       }
     }
   } else if (warp < KV4P_SOFT + 2 * KV4P_DEQ) {
-    A8_SETMAXNREG("dec", 64);
+    A8_SETMAXNREG("dec", KV4P_REG_REST);
     // ---- codes to fp16: 128 threads for K, 128 for V
     const bool isv = warp >= KV4P_SOFT + KV4P_DEQ;
     const int dw = (warp - KV4P_SOFT) & 3, dt = dw * 32 + lane;
@@ -424,7 +430,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       }
     }
   } else {
-    A8_SETMAXNREG("dec", 64);
+    A8_SETMAXNREG("dec", KV4P_REG_REST);
     if (warp == 16 && lane == 0) {
       const uint8_t* src = kv4_rec(a.c, F::REC, crow, kvh, 0);
       int issued = 0;
@@ -596,7 +602,7 @@ template <int HD>
 static int kv4_prefill_launch(Kv4AttnArgs& a, int nblocks, cudaStream_t s) {
   const void* fn = (const void*)k_kv4_prefill<HD>;
   static std::atomic<uint64_t> ready{0};
-  if (!kv4_smem_ready(ready, fn, Kv4PreSmem<HD>::TOTAL)) return A8_ERR_CUDA;
+  if (!kv4_ready(ready, fn, Kv4PreSmem<HD>::TOTAL, kv4p_registers_cover)) return A8_ERR_CUDA;
   const long long per = (long long)a.c.nkv * ((a.group + 3) / 4);
   if (nblocks * per >= (1ll << 31)) return A8_ERR_SIZE;
   void* args[] = {&a};

@@ -53,3 +53,31 @@ def test_stack_refuses_before_it_launches(L):
     assert run(kc=None) == ARG and run(kc=None, vc=p) == ARG
     assert run(inter=1088) == SIZE
     assert run(ring=32, nblocks=1) == ARG
+
+
+def test_prompt_kernel_s_registers(tmp_path):
+    """The registers that the prompt kernel is compiled to cover what its warpgroups take (one that asks for more than the
+    block has waits for good), and the rule by which the host refuses to launch it otherwise."""
+    import re
+    import shutil
+    if shutil.which("nvcc") is None:
+        pytest.skip("no CUDA compiler")
+    src = tmp_path / "t.cu"
+    src.write_text("""#include <stdio.h>
+#include "common.cuh"
+namespace a8 {
+static long long g_launches;
+__device__ __forceinline__ uint32_t sw128(int row, int c) { return row * 128 + ((c ^ (row & 7)) << 4); }
+}
+#include "kv4.cu"
+#include "kv4_prefill.cu"
+int main() { for (int r : {64, 80, 88, 96, 102}) printf("%d ", a8::kv4p_registers_cover(r)); }
+""")
+    r = subprocess.run(["nvcc", "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-diag-suppress", "177",
+                        "-Xptxas", "-v", "-I", os.path.join(REPO, "include"), "-I",
+                        os.path.join(REPO, "audio8-turbo-engine_b200", "csrc"), str(src), "-o", str(tmp_path / "t")],
+                       capture_output=True, text=True, check=True)
+    used = re.findall(r"Compiling entry function '(\w*k_kv4_prefill\w*)'.*?Used (\d+) registers", r.stderr, flags=re.S)
+    assert len(used) == 2 and all(int(n) == 96 for _, n in used), used
+    out = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout.split()
+    assert out == ["0", "0", "0", "1", "1"]
