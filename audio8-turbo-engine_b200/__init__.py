@@ -5,7 +5,7 @@ libaudio8_b200.so (include/audio8_b200.h). The directory name is not a Python id
 by path (``__graft_entry__.load_package()``) under the module name ``audio8_b200``.
 """
 from . import _lib  # noqa: F401
-from ._lib import A8Error, device_error, load  # noqa: F401
+from ._lib import A8Error, clear_error, device_error, load  # noqa: F401
 
 
 def __getattr__(name):

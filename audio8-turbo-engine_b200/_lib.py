@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import weakref
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libaudio8_b200.so")
@@ -211,6 +212,18 @@ def device_error():
     out = (c_int * 4)()
     check(load().a8_get_error(out), "a8_get_error")
     return tuple(out)
+
+
+# What keeps attention counters on the device between calls: objects with a reset()
+counters = weakref.WeakSet()
+
+
+def clear_error():
+    """Clear the device-side error record, and the counters that a kernel which gave up a wait may have left partly
+    advanced: those of every live KV4Cache and engine scratch (a workspace of the caller's own is the caller's to zero)."""
+    call("a8_clear_error")
+    for o in list(counters):
+        o.reset()
 
 
 def ptr(t):

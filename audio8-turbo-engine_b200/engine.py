@@ -132,6 +132,12 @@ class Scratch:
             attn_ws=L.ptr(self.attn_ws), attn_ws_floats=self.attn_ws.numel(), attn_counters=L.ptr(self.attn_counters),
             n_attn_counters=self.attn_counters.numel(), ssq=L.ptr(self.ssq), ssq_ld=rows)
         self.rows = rows
+        L.counters.add(self)
+
+    def reset(self):
+        """The counters as they were at first (`clear_error` calls it; nothing may be in flight)."""
+        self.attn_counters.zero_()
+        torch.cuda.synchronize(self.attn_counters.device)
 
 
 class FastEngine:

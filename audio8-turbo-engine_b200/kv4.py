@@ -42,6 +42,12 @@ class KV4Cache:
         self._ref = C.byref(self.desc)
         self._lib = L.load()
         self._ws = {}
+        L.counters.add(self)
+
+    def reset(self):
+        """Drop the workspaces of `attention`: after a wait that ran out (`device_error`) their tickets may be partly taken,
+        and later calls would join too early. `clear_error` of the package calls it for every cache."""
+        self._ws.clear()
 
     @property
     def nbytes(self) -> int:

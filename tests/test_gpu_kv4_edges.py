@@ -115,3 +115,28 @@ def test_decode_of_a_tiny_scale(kv4, nq, nkv, hd, scale):
             o, tol = R.attention(qd[r:r + 1, h], k, v, m - 1, scale)
             d = (got[r:r + 1, h] - o).abs()
             assert bool((d <= tol).all()), (r, h, float((d - tol).max()))
+
+
+# ------------------------------------------------------------------------------------------------- after a timeout
+def test_clear_error_restores_the_tickets(kv4):
+    """Tickets left partly taken, as by a kernel that gave up a wait: clear_error() brings a cache's and an engine's back."""
+    nq, nkv, hd, n = 14, 2, 64, 3000
+    x = rnd(9, n, 2, nkv, hd)
+    c = one_row(kv4, x, hd)
+    q = rnd(10, 3, nq * hd).cuda()
+    lens, row = torch.tensor([n, 17, 2900], dtype=I32, device="cuda"), torch.zeros(3, dtype=I32, device="cuda")
+    want = c.attention(q, lens, row)
+    no_error(kv4)
+    assert c._ws
+    for *_, tensors in (have[3] for have in c._ws.values()):
+        assert not bool(tensors[1].any())                    # a call leaves them zero
+        tensors[1].fill_(1)
+        tensors[0].fill_(float("nan"))
+    from audio8_b200.engine import Scratch
+    sc = Scratch(8, 64, 128, 64, 2, 64, 200, torch.device("cuda", 0), c)
+    sc.attn_counters.fill_(1)
+    kv4.clear_error()
+    assert not bool(sc.attn_counters.any())
+    for _ in range(2):
+        assert torch.equal(c.attention(q, lens, row), want)
+    no_error(kv4)

@@ -81,3 +81,15 @@ int main() { for (int r : {64, 80, 88, 96, 102}) printf("%d ", a8::kv4p_register
     assert len(used) == 2 and all(int(n) == 96 for _, n in used), used
     out = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout.split()
     assert out == ["0", "0", "0", "1", "1"]
+
+
+def test_clear_error_reaches_every_cache(a8, L, monkeypatch):
+    """The package's clear_error clears the record, and the counters of what is alive (here without a device)."""
+    c, gone = (a8.KV4Cache(1, 1, 64, 16, dev="cpu") for _ in range(2))
+    c._ws["stream"] = gone._ws["stream"] = "tickets"
+    del gone
+    calls = []
+    monkeypatch.setattr(L, "call", lambda name, *a: calls.append(name))
+    monkeypatch.setattr(L, "counters", [o for o in L.counters if o is c])       # (others may need a device)
+    a8.clear_error()
+    assert calls == ["a8_clear_error"] and c._ws == {}
