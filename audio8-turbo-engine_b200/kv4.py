@@ -14,8 +14,6 @@ import torch
 from . import _lib as L
 
 BF16, I32 = torch.bfloat16, torch.int32
-_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def _need(ok, what):
@@ -37,8 +35,12 @@ class KV4Cache:
         self.buf = torch.zeros(n, dtype=torch.uint8, device=torch.device("cuda" if dev is None else dev))
         self.dev = self.buf.device
         self.desc.buf = self.buf.data_ptr()
-        if self.dev.type == "cuda" and self.dev.index is None:
-            self.dev = torch.device("cuda", torch.cuda.current_device())
+        if self.dev.type == "cuda":
+            if self.dev.index is None:
+                self.dev = torch.device("cuda", torch.cuda.current_device())
+            # (a torch without CUDA has none of these)
+            self._current_device, self._current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+            self._capturing = torch._C._cuda_isCurrentStreamCapturing
         self._ref = C.byref(self.desc)
         self._lib = L.load()
         self._ws = {}
@@ -81,11 +83,11 @@ class KV4Cache:
         dev = self.dev.index
         if dev is None:
             _need(False, "the cache is not on a GPU (there is no CPU fallback)")
-        if dev == _current_device():
-            rc = fn(self._ref, *args, _current_stream(dev))
+        if dev == self._current_device():
+            rc = fn(self._ref, *args, self._current_stream(dev))
         else:
             with torch.cuda.device(dev):
-                rc = fn(self._ref, *args, _current_stream(dev))
+                rc = fn(self._ref, *args, self._current_stream(dev))
         if rc:
             L.check(rc, fn.__name__)
 
@@ -156,8 +158,8 @@ class KV4Cache:
         dev = self.dev.index
         if dev is None:
             _need(False, "the cache is not on a GPU (there is no CPU fallback)")
-        capturing = _capturing()
-        key = _current_stream(dev)
+        capturing = self._capturing()
+        key = self._current_stream(dev)
         have = self._ws.get(key)
         if have is None or nq > have[0] or rows > have[1] or max_len > have[2] or capturing:
             if capturing:

@@ -93,3 +93,15 @@ def test_clear_error_reaches_every_cache(a8, L, monkeypatch):
     monkeypatch.setattr(L, "counters", [o for o in L.counters if o is c])       # (others may need a device)
     a8.clear_error()
     assert calls == ["a8_clear_error"] and c._ws == {}
+
+
+def test_imports_on_a_torch_without_cuda():
+    """The engine and the cache import, and a cache on the CPU can be made, where torch has no CUDA bindings."""
+    code = ("import torch\n"
+            "for n in ('_cuda_getDevice', '_cuda_getCurrentRawStream', '_cuda_isCurrentStreamCapturing'):\n"
+            "    delattr(torch._C, n)\n"
+            "import __graft_entry__ as g\n"
+            "a8 = g.load_package()\n"
+            "a8.FastEngine, a8.KV4Cache(1, 1, 64, 16, dev='cpu')\n")
+    r = subprocess.run([os.sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-800:]
