@@ -158,6 +158,9 @@ class KV4Cache:
         dev = self.dev.index
         if dev is None:
             _need(False, "the cache is not on a GPU (there is no CPU fallback)")
+        if dev != self._current_device():                # (whether a stream captures is asked of the current device)
+            with torch.cuda.device(dev):
+                return self._workspace(nq, rows, max_len)
         capturing = self._capturing()
         key = self._current_stream(dev)
         have = self._ws.get(key)
@@ -166,8 +169,7 @@ class KV4Cache:
                 return self._pointers(self.workspace(nq, rows, max_len))
             if have is not None:
                 nq, rows, max_len = max(nq, have[0]), max(rows, have[1]), max(max_len, have[2])
-            with torch.cuda.device(self.dev):
-                have = self._ws[key] = (nq, rows, max_len, self._pointers(self.workspace(nq, rows, max_len)))
+            have = self._ws[key] = (nq, rows, max_len, self._pointers(self.workspace(nq, rows, max_len)))
         return have[3]
 
     @staticmethod

@@ -105,3 +105,35 @@ def test_imports_on_a_torch_without_cuda():
             "a8.FastEngine, a8.KV4Cache(1, 1, 64, 16, dev='cpu')\n")
     r = subprocess.run([os.sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr[-800:]
+
+
+def test_a_capture_on_the_cache_s_device_is_noticed(a8, monkeypatch):
+    """With another device current, whether the call is captured is the cache's device's matter: a captured call gets a
+    workspace of its own, an eager one the stream's."""
+    c = a8.KV4Cache(2, 2, 64, 64, dev="cpu")
+    c.dev = torch.device("cuda", 1)
+    current, capturing, made = [0], {0: False, 1: True}, []
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = torch.device(dev).index if not isinstance(dev, int) else dev
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.dev
+
+        def __exit__(self, *a):
+            current[0] = self.was
+
+    def workspace(nq, rows, max_len):
+        made.append(current[0])
+        return torch.zeros(4), torch.zeros(4, dtype=torch.int32)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    c.workspace = workspace
+    c._current_device = lambda: current[0]
+    c._current_stream = lambda dev: 7
+    c._capturing = lambda: capturing[current[0]]
+    a, b = c._workspace(14, 2, 64), c._workspace(14, 2, 64)
+    assert a[0] != b[0] and not c._ws                    # captured: each its own, nothing kept
+    capturing.update({0: True, 1: False})                # another device's capture is not this call's
+    assert c._workspace(14, 2, 64)[0] == c._workspace(14, 2, 64)[0] and set(c._ws) == {7}
+    assert made == [1, 1, 1]                             # where the call will run
