@@ -16,6 +16,9 @@ from . import _lib as L
 BF16, I32 = torch.bfloat16, torch.int32
 
 
+INT = (1 << 31) - 1      # what a number or a row stride may be: ctypes would cut more to 32 bits, without a word
+
+
 def _need(ok, what):
     if not ok:
         raise L.A8Error(f"kv4: {what}")
@@ -31,7 +34,8 @@ class KV4Cache:
         self.cache_len = int(cache_len)
         self.desc = L.A8KV4(None, self.layers, self.cache_rows, self.nkv, self.hd, self.cache_len)
         n = L.load().a8_kv4_bytes(C.byref(self.desc))
-        _need(n > 0, f"unsupported shape {(layers, cache_rows, nkv, hd, cache_len)} (hd 64 or 128)")
+        _need(n > 0 and max(self.layers, self.cache_rows, self.nkv, self.hd, self.cache_len) <= INT
+              and min(self.layers, self.cache_rows, self.nkv, self.hd, self.cache_len) > 0, f"unsupported shape {(layers, cache_rows, nkv, hd, cache_len)} (hd 64 or 128)")
         self.buf = torch.zeros(n, dtype=torch.uint8, device=torch.device("cuda" if dev is None else dev))
         self.dev = self.buf.device
         self.desc.buf = self.buf.data_ptr()
@@ -63,7 +67,12 @@ class KV4Cache:
         if one != 1 or t.dtype is not BF16 or t.device != self.dev or shape[0] < rows or shape[1] < width:
             _need(False, f"{what}: bf16 [at least {rows}, at least {width}] on {self.dev}, rows contiguous")
         # (the row stride of a single row means nothing: torch may give it any value)
-        return ld if shape[0] > 1 else max(ld, shape[1])
+        return self._stride(ld if shape[0] > 1 else max(ld, shape[1]), what)
+
+    def _stride(self, ld, what):
+        if ld > INT:
+            _need(False, f"{what}: a row stride of {ld}")
+        return ld
 
     def _heads(self, t, rows, what):
         """Row stride of bf16 [>= rows, nkv, hd] with contiguous heads."""
@@ -71,23 +80,31 @@ class KV4Cache:
               and t.shape[1:] == (self.nkv, self.hd) and t.stride(2) == 1
               and (self.nkv == 1 or t.stride(1) == self.hd),
               f"{what}: bf16 [at least {rows}, {self.nkv}, {self.hd}] on {self.dev}, heads contiguous")
-        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), self.nkv * self.hd)
+        return self._stride(t.stride(0) if t.shape[0] > 1 else max(t.stride(0), self.nkv * self.hd), what)
 
     def _ints(self, t, n, what):
-        if t.dtype is not I32 or t.device != self.dev or not t.is_contiguous() or t.numel() < n:
+        if t.dtype is not I32 or t.device != self.dev or not t.is_contiguous() or t.numel() < n or n > INT:
             _need(False, f"{what}: {n} contiguous int32 on {self.dev}")
         return t.data_ptr()
 
-    def _call(self, fn, *args):
-        """fn(cache, *args, the current stream of the cache's device)."""
+    @staticmethod
+    def _scale(scale):
+        if 0.0 < scale < 1.2e-38:
+            _need(False, f"scale {scale}: below the least normal fp32 number")
+        return scale
+
+    def _call(self, fn, layer, *args):
+        """fn(cache, layer, *args, the current stream of the cache's device)."""
         dev = self.dev.index
+        if not 0 <= layer < self.layers:
+            _need(False, f"layer {layer} of {self.layers}")
         if dev is None:
             _need(False, "the cache is not on a GPU (there is no CPU fallback)")
         if dev == self._current_device():
-            rc = fn(self._ref, *args, self._current_stream(dev))
+            rc = fn(self._ref, layer, *args, self._current_stream(dev))
         else:
             with torch.cuda.device(dev):
-                rc = fn(self._ref, *args, self._current_stream(dev))
+                rc = fn(self._ref, layer, *args, self._current_stream(dev))
         if rc:
             L.check(rc, fn.__name__)
 
@@ -111,6 +128,8 @@ class KV4Cache:
             pcos, psin = cos.data_ptr(), sin.data_ptr()
         else:
             _need(cos is None and sin is None, "cos and sin come together")
+        if not 0 <= ring <= self.cache_len:
+            _need(False, f"ring {ring} of a cache of {self.cache_len}")
         ldq = pq = None
         if nq > 0:
             if q is None:
@@ -146,6 +165,7 @@ class KV4Cache:
 
     def workspace(self, nq: int, rows: int, max_len: int):
         """A workspace (partials, tickets) for `attention` calls up to these sizes; one call at a time uses it."""
+        _need(0 < nq <= INT and 0 < rows <= INT and 0 < max_len <= self.cache_len, f"workspace of {nq, rows, max_len}")
         n, t = C.c_longlong(), C.c_int()
         L.check(L.load().a8_kv4_attention_workspace(self._ref, nq, rows, max_len, C.byref(n), C.byref(t)),
                 "a8_kv4_attention_workspace")
@@ -185,6 +205,8 @@ class KV4Cache:
         nq, ldq, ldo, out = self._queries(q, out)
         rows = q.shape[0]
         max_len = max_len or self.cache_len
+        if not 0 < max_len <= self.cache_len:
+            _need(False, f"max_len {max_len} of a cache of {self.cache_len}")
         plens = self._ints(lens, rows, "lens")           # (the tensors stay referenced until the launch)
         pmap = None if rowmap is None else self._ints(rowmap, rows, "rowmap")
         if rows:
@@ -193,8 +215,8 @@ class KV4Cache:
                       and ws[0].is_contiguous() and ws[1].is_contiguous(),
                       f"ws: the (float32, int32) tensors of workspace() on {self.dev}")
             pw, nw, pt, nt, held = self._workspace(nq, rows, max_len) if ws is None else self._pointers(ws)
-            self._call(self._lib.a8_kv4_attention, layer, q.data_ptr(), ldq, nq, plens, pmap, rows, max_len, scale,
-                       out.data_ptr(), ldo, pw, nw, pt, nt)
+            self._call(self._lib.a8_kv4_attention, layer, q.data_ptr(), ldq, nq, plens, pmap, rows, max_len,
+                       self._scale(scale), out.data_ptr(), ldo, pw, nw, pt, nt)
         return out
 
     def _queries(self, q, out):
@@ -216,6 +238,6 @@ class KV4Cache:
         n = blocks.shape[0]
         pblocks = self._ints(blocks, 4 * n, "blocks")
         if rows and n:
-            self._call(self._lib.a8_kv4_prefill_attention, layer, q.data_ptr(), ldq, nq, pblocks, n, rows, scale,
-                       out.data_ptr(), ldo)
+            self._call(self._lib.a8_kv4_prefill_attention, layer, q.data_ptr(), ldq, nq, pblocks, n, rows,
+                       self._scale(scale), out.data_ptr(), ldo)
         return out

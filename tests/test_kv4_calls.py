@@ -137,3 +137,53 @@ def test_a_capture_on_the_cache_s_device_is_noticed(a8, monkeypatch):
     capturing.update({0: True, 1: False})                # another device's capture is not this call's
     assert c._workspace(14, 2, 64)[0] == c._workspace(14, 2, 64)[0] and set(c._ws) == {7}
     assert made == [1, 1, 1]                             # where the call will run
+
+
+def test_numbers_that_a_c_int_would_wrap_are_refused(a8):
+    """2^32 + n is not n: layers, rings, bounds, shapes and row strides are refused, not cut to 32 bits."""
+    W = 1 << 32
+    for shape in ((W + 2, 2, 64, 40), (2, W + 2, 64, 40), (2, 2, W + 64, 40), (2, 2, 64, W + 40), (2, 2, 64, -W + 40)):
+        with pytest.raises(a8.A8Error, match="unsupported shape"):
+            a8.KV4Cache(*shape, dev="cpu")
+    with pytest.raises(a8.A8Error, match="unsupported shape"):
+        a8.KV4Cache(2, 2, 64, 40, dev="cpu", layers=W + 1)
+    c = a8.KV4Cache(2, 2, 64, 40, dev="cpu", layers=3)
+    c._workspace = lambda *a: (0, 0, 0, 0, None)
+    bf, i32 = torch.bfloat16, torch.int32
+    x, i, q = torch.zeros(3, 18 * 64, dtype=bf), torch.zeros(3, dtype=i32), torch.zeros(3, 896, dtype=bf)
+    b = torch.zeros(1, 4, dtype=i32)
+    for layer in (-1, 3, W, W + 1, -W):
+        for f in (lambda: c.store(x, i, nq=14, layer=layer), lambda: c.load(i, layer=layer),
+                  lambda: c.attention(q, i, layer=layer), lambda: c.prefill_attention(q, b, layer=layer)):
+            with pytest.raises(a8.A8Error, match="layer"):
+                f()
+    for ring in (-1, 41, W, W + 8):
+        with pytest.raises(a8.A8Error, match="ring"):
+            c.store(x, i, nq=14, ring=ring)
+    for n in (-1, 41, W + 40):
+        with pytest.raises(a8.A8Error, match="max_len"):
+            c.attention(q, i, max_len=n)
+        with pytest.raises(a8.A8Error):
+            c.workspace(14, 3, n)
+    for nq, rows in ((W + 14, 3), (14, W + 3), (14, 0)):
+        with pytest.raises(a8.A8Error):
+            c.workspace(nq, rows, 40)
+    for scale in (1e-39, 1e-60):                         # (0 in a C float: the default)
+        for f in (lambda: c.attention(q, i, scale=scale), lambda: c.prefill_attention(q, b, scale=scale)):
+            with pytest.raises(a8.A8Error, match="scale"):
+                f()
+
+
+def test_strides_past_32_bits_are_refused(a8):
+    c = a8.KV4Cache(2, 2, 64, 40, dev="cpu")
+    i = torch.zeros(2, dtype=torch.int32)
+    # (two rows 2^32 + 1,152 elements apart, on a meta tensor: only its shape and strides are looked at)
+    far = torch.empty_strided((2, 18 * 64), ((1 << 32) + 18 * 64, 1), dtype=torch.bfloat16, device="meta")
+    kv = torch.empty_strided((2, 2, 64), ((1 << 32) + 128, 64, 1), dtype=torch.bfloat16, device="meta")
+    c.dev = far.device
+    i = i.to("meta")
+    for f in (lambda: c.store(far, i, nq=14), lambda: c.attention(far[:, :896], i),
+              lambda: c.prefill_attention(far[:, :896], torch.zeros(1, 4, dtype=torch.int32, device="meta")),
+              lambda: c.load(i, k=kv), lambda: c.load(i, v=kv)):
+        with pytest.raises(a8.A8Error, match="stride"):
+            f()
