@@ -123,8 +123,8 @@ class KV4Cache:
             npos = cos.shape[0]
             if (cos.dtype is not BF16 or sin.dtype is not BF16 or cos.shape != (npos, hd) or sin.shape != (npos, hd)
                     or not cos.is_contiguous() or not sin.is_contiguous() or cos.device != self.dev
-                    or sin.device != self.dev):
-                _need(False, f"cos, sin: two contiguous bf16 [npos, {hd}] tables on {self.dev}")
+                    or sin.device != self.dev or npos == 0):
+                _need(False, f"cos, sin: two contiguous bf16 [npos, {hd}] tables on {self.dev}, npos at least 1")
             pcos, psin = cos.data_ptr(), sin.data_ptr()
         else:
             _need(cos is None and sin is None, "cos and sin come together")

@@ -187,3 +187,11 @@ def test_strides_past_32_bits_are_refused(a8):
               lambda: c.load(i, k=kv), lambda: c.load(i, v=kv)):
         with pytest.raises(a8.A8Error, match="stride"):
             f()
+
+
+def test_rotation_tables_without_rows_are_refused(a8):
+    """cos and sin of no rows have no address, which the C call takes for no rotation at all."""
+    c = a8.KV4Cache(2, 2, 64, 40, dev="cpu")
+    x, t = torch.zeros(3, 18 * 64, dtype=torch.bfloat16), torch.zeros(0, 64, dtype=torch.bfloat16)
+    with pytest.raises(a8.A8Error, match="cos, sin"):
+        c.store(x, torch.zeros(3, dtype=torch.int32), nq=14, cos=t, sin=t)
