@@ -1195,8 +1195,9 @@ static int kv4_attention(const A8KV4* c, int layer, const void* q, int q_stride,
   if (rc) return rc;
   // (in place: a unit's result is written after its last read of the queries it stands in)
   if (lens == nullptr || max_len <= 0 || max_len > c->cache_len || (out == q && out_stride != q_stride)) return A8_ERR_ARG;
-  // the steps of all rows are counted in 32 bits
-  if (rows > (1 << 24) || (long long)rows * c->nkv * ((max_len + KV4_STEP - 1) / KV4_STEP) >= (1ll << 31)) return A8_ERR_SIZE;
+  // the steps of all rows are counted in 32 bits, and rounded up to CTAs' shares there
+  const long long steps = (long long)rows * c->nkv * ((max_len + KV4_STEP - 1) / KV4_STEP);
+  if (rows > (1 << 24) || steps >= (1ll << 31) - KV4_CTA_STEPS) return A8_ERR_SIZE;
   const int ctas = kv4_ctas(c, rows, max_len);
   a.part = kv4_part(c, nq);
   if (ws == nullptr || ws_floats < 2ll * ctas * a.part || counters == nullptr || n_counters < (long long)rows * c->nkv)

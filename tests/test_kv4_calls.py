@@ -195,3 +195,18 @@ def test_rotation_tables_without_rows_are_refused(a8):
     x, t = torch.zeros(3, 18 * 64, dtype=torch.bfloat16), torch.zeros(0, 64, dtype=torch.bfloat16)
     with pytest.raises(a8.A8Error, match="cos, sin"):
         c.store(x, torch.zeros(3, dtype=torch.int32), nq=14, cos=t, sin=t)
+
+
+def test_attention_steps_stay_within_32_bits(L):
+    """The steps of 32 keys of all rows are counted in 32 bits, a CTA's share rounded up among them: calls that could pass
+    them are refused, the next smaller ones are not."""
+    lib, N, p = L.load(), None, C.c_void_p(256)
+
+    def attn(rows, steps):
+        d = L.A8KV4(256, 1, 1, 1, 64, steps * 32)
+        return lib.a8_kv4_attention(C.byref(d), 0, p, 64, 1, p, N, rows, steps * 32, 0.0, p, 64, p, 1 << 40, p, 1 << 30, N)
+    top = (1 << 31) - 1
+    for rows, steps in ((104643, 20522), (1 << 11, 1 << 20)):        # 2^31 - 2 and 2^31
+        assert top - 24 < rows * steps and attn(rows, steps) == SIZE, (rows, steps)
+    if not torch.cuda.is_available():
+        assert attn((1 << 11) - 1, 1 << 20) == CUDA                   # (no device here: the launch itself fails)
