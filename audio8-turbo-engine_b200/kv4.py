@@ -67,7 +67,7 @@ class KV4Cache:
         if one != 1 or t.dtype is not BF16 or t.device != self.dev or shape[0] < rows or shape[1] < width:
             _need(False, f"{what}: bf16 [at least {rows}, at least {width}] on {self.dev}, rows contiguous")
         # (the row stride of a single row means nothing: torch may give it any value)
-        return self._stride(ld if shape[0] > 1 else max(ld, shape[1]), what)
+        return self._stride(ld, what) if rows > 1 else width
 
     def _stride(self, ld, what):
         if ld > INT:
@@ -80,7 +80,7 @@ class KV4Cache:
               and t.shape[1:] == (self.nkv, self.hd) and t.stride(2) == 1
               and (self.nkv == 1 or t.stride(1) == self.hd),
               f"{what}: bf16 [at least {rows}, {self.nkv}, {self.hd}] on {self.dev}, heads contiguous")
-        return self._stride(t.stride(0) if t.shape[0] > 1 else max(t.stride(0), self.nkv * self.hd), what)
+        return self._stride(t.stride(0), what) if rows > 1 else self.nkv * self.hd
 
     def _ints(self, t, n, what):
         if t.dtype is not I32 or t.device != self.dev or not t.is_contiguous() or t.numel() < n or n > INT:
@@ -137,6 +137,8 @@ class KV4Cache:
                 q = torch.empty(rows, ldq, dtype=BF16, device=self.dev)
             else:
                 ldq = self._rows(q, rows, nq * hd, "q")
+                if rows == 1:                            # (in place asks for one stride)
+                    ldq = ld
             pq = q.data_ptr()
         if rows:
             self._call(self._lib.a8_kv4_store, layer, qkv.data_ptr(), ld, nq, pcos, psin, npos or 0, ppos, pslot, rows,

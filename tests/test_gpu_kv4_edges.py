@@ -140,3 +140,43 @@ def test_clear_error_restores_the_tickets(kv4):
     for _ in range(2):
         assert torch.equal(c.attention(q, lens, row), want)
     no_error(kv4)
+
+
+# ------------------------------------------------------------------------------------------------- one row
+def test_a_single_row_of_any_row_stride(kv4):
+    """The row stride of a single row is never used: rows cut from wider or oddly strided tensors are taken as they are, in
+    place too, and nothing beside them is touched."""
+    nq, nkv, hd = 6, 2, 64
+    W, Q = (nq + 2 * nkv) * hd, nq * hd
+    x = rnd(20, 1, W)
+    i0, i1 = torch.zeros(1, dtype=I32, device="cuda"), torch.ones(1, dtype=I32, device="cuda")
+    c = kv4.KV4Cache(1, nkv, hd, 20)
+    want = c.store(x.cuda(), i0, i0, nq=nq)
+    wk, wv = c.load(i0, i0)
+    wo = c.attention(want, i1)
+    blocks = torch.tensor([[0, 1, 0, 0]], dtype=I32, device="cuda")
+    wp = c.prefill_attention(want, blocks)
+    no_error(kv4)
+    for width, stride in ((W + 4, W + 4), (W, W + 3), (W, 1), (W, W)):
+        c = kv4.KV4Cache(1, nkv, hd, 20)
+        base = torch.full((2 * W + 64,), 5.0, dtype=BF, device="cuda")
+        qkv = torch.as_strided(base, (1, width), (stride, 1))
+        qkv[:, :W] = x.cuda()
+        q = c.store(qkv, i0, i0, nq=nq)
+        kv = torch.full((2 * W + 64,), 5.0, dtype=BF, device="cuda")
+        k = torch.as_strided(kv, (1, nkv, hd), (stride, hd, 1))
+        gk, gv = c.load(i0, i0, k=k)
+        big = torch.full((2 * W + 64,), 5.0, dtype=BF, device="cuda")
+        out = torch.as_strided(big, (1, Q), (stride, 1))
+        qrow = torch.as_strided(base.clone(), (1, Q), (stride, 1))
+        qrow.copy_(q)
+        o = c.attention(qrow, i1, out=out).clone()
+        p = c.prefill_attention(qrow, blocks, out=out)
+        no_error(kv4)
+        assert torch.equal(q, want) and torch.equal(gk, wk) and torch.equal(gv, wv)
+        assert torch.equal(o, wo) and torch.equal(p, wp)
+        assert bool((big[Q:] == 5).all()) and bool((kv[nkv * hd:] == 5).all()) and bool((base[W:] == 5).all())
+        # in place
+        assert c.store(qkv, i0, i0, nq=nq, q=qkv[:, :Q]).data_ptr() == base.data_ptr()
+        no_error(kv4)
+        assert torch.equal(base[:Q], want[0]) and torch.equal(base[Q:W], x[0, Q:].cuda()) and bool((base[W:] == 5).all())
