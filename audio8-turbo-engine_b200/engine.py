@@ -142,10 +142,11 @@ class Scratch:
 
 class FastEngine:
     """serve/fast_engine.py:570 on sm_100a kernels. Sampling noise: Philox keyed by `seed` (default from
-    TTS_SEED, else 1234), counted by the engine's tick number."""
+    TTS_SEED, else 1234), counted by the engine's tick number. kv_bits: the slow stack's keys and values in 16 or 4 bits
+    (default from TTS_KV_BITS, else 16)."""
 
     def __init__(self, model, tokenizer, gen_params: dict, max_slots: int = 32, max_seq: int = 2048, buckets=None,
-                 seq_from_env=True, seed=None):
+                 seq_from_env=True, seed=None, kv_bits=None):
         if not torch.cuda.is_available():
             raise L.A8Error("FastEngine needs a CUDA device (B200); there is no CPU fallback")
         L.load()
@@ -181,7 +182,7 @@ class FastEngine:
         self.SCR = B
         self.slow = PackedStack(model.layers, model.norm, c.n_head, c.n_local_heads, c.head_dim, c.norm_eps,
                                 c.rope_base, cache_rows=B + 1, cache_len=self.S, max_pos=self.S, dev=dev,
-                                kv_bits=int(os.environ.get("TTS_KV_BITS", "16")))
+                                kv_bits=int(os.environ.get("TTS_KV_BITS", "16") if kv_bits is None else kv_bits))
         self.fast = PackedStack(model.fast_layers, model.fast_norm, c.fast_n_head, c.fast_n_local_heads,
                                 c.fast_head_dim, c.norm_eps, c.rope_base, cache_rows=B, cache_len=self.ncg,
                                 max_pos=self.ncg, dev=dev)

@@ -19,6 +19,8 @@ length drawn uniform in [200, 1500] from seed 1, one new token a slot, the stand
 + state update, replayed from one CUDA graph; every slot's position is restored before each step so the workload is
 the same at every step. Data: synthetic (seeded random weights and KV; no checkpoint or dataset is involved).
 
+TTS_KV_BITS=4 runs any workload of ours on a slow cache in 4 bits (the line's config says so); default 16, bf16.
+
 --impl reference times the reference's own CPU implementation of the path: the reference has none (Triton only),
 so it is the CPU restatement oracle/ref_cpu.py on all host threads, on a bounded sample of the same workload.
 Multi-GPU (torchrun, N > 1): one independent replica per GPU (streams shard across replicas; nothing is exchanged),
@@ -39,6 +41,7 @@ sys.path.insert(0, REPO)
 
 B_CFG1 = 64
 L_LO, L_HI = 200, 1500
+KV4_BYTES = 0.5 + 2 / 32                                    # an element of a 4-bit cache: its code, its share of a scale
 METRIC = "tick frames/s"
 UNIT = "frames/s"
 
@@ -105,14 +108,34 @@ def cfg1_lengths():
     return torch.randint(L_LO, L_HI + 1, (B_CFG1,), generator=g)
 
 
-def cfg1_bytes_flops(lens, layers=24):
-    """Algorithmic HBM bytes and FLOPs of one cfg1 step (no padding rows or columns counted)."""
+def fill_slow(st, g, rows):
+    """Random keys and values in the first `rows` rows of a stack's cache, in bf16 or (TTS_KV_BITS=4) in 4 bits."""
+    import torch
+    if st.kv4 is None:
+        for t in (st.kc, st.vc):
+            t[:, :rows].normal_(generator=g)
+        return
+    pos = torch.arange(st.kv4.cache_len, dtype=torch.int32, device=st.kv4.dev).repeat(rows)
+    slot = torch.arange(rows, dtype=torch.int32, device=st.kv4.dev).repeat_interleave(st.kv4.cache_len)
+    kv = torch.empty(len(pos), 2 * st.nkv * st.hd, dtype=torch.bfloat16, device=st.kv4.dev)
+    for l in range(st.layers):
+        st.kv4.store(kv.normal_(generator=g), pos, slot, layer=l)
+
+
+def with_cache(config, st):
+    """A workload's config, naming a slow cache that is not the bf16 one."""
+    return config if st.kv4 is None else dict(config, kv_cache="slow AR in 4 bits (4.5 with scales, 9 / 32 of a bf16 cache)")
+
+
+def cfg1_bytes_flops(lens, layers=24, kv_bytes=2):
+    """Algorithmic HBM bytes and FLOPs of one cfg1 step (no padding rows or columns counted); kv_bytes a cached
+    element."""
     b = len(lens)
     sl = int(lens.sum())
     w_layer = (1152 * 896 + 1152) * 2 + 896 * 896 * 2 + 9728 * 896 * 2 + 896 * 4864 * 2 + 2 * 896 * 2
     weights = layers * w_layer + 4097 * 896 * 2
-    kv = layers * 2 * 2 * 64 * 2 * sl                       # K and V, 2 kv heads, hd 64, bf16
-    kv_write = layers * 2 * 2 * 64 * 2 * b
+    kv = int(layers * 2 * 2 * 64 * kv_bytes * sl)           # K and V, 2 kv heads, hd 64
+    kv_write = int(layers * 2 * 2 * 64 * kv_bytes * b)
     flops = 2 * b * (layers * 14_909_440 + 4097 * 896) + layers * 4 * 14 * 64 * sl
     return weights + kv + kv_write, flops, kv // layers
 
@@ -219,8 +242,7 @@ def run_ours(args, rank, world, local):
     b = B_CFG1
     lens = cfg1_lengths()
     g = torch.Generator(device=dev).manual_seed(3 + rank)
-    for t in (eng.slow.kc, eng.slow.vc):
-        t[:, :b].normal_(generator=g)
+    fill_slow(eng.slow, g, b)
     cpos0 = (lens - 1).to(torch.int32).to(dev)
     eng.cpos[:b].copy_(cpos0)
     tok0 = (eng.sb + torch.randint(0, 4096, (b,), generator=g, device=dev)).long()
@@ -297,11 +319,11 @@ def run_ours(args, rank, world, local):
     roof = roofline(eng, L, lens, dev, args)
     line = None
     if rank == 0:
-        nbytes, flops, _ = cfg1_bytes_flops(lens)
+        nbytes, flops, _ = cfg1_bytes_flops(lens, kv_bytes=KV4_BYTES if eng.slow.kv4 is not None else 2)
         line = {"metric": METRIC, "value": round(value, 3), "unit": UNIT, "n_gpus": world, "steps": args.steps,
                 "warmup": args.warmup, "ms_per_step": round(ms / args.steps, 4), "higher_is_better": True,
                 "scaling": "weak", "vs_baseline": None, "dtype": "bf16", "data": "synthetic",
-                "config": cfg_dict(world), "roofline": roof, "e2e": e2e, "gpu_launches": int(launches) * args.steps,
+                "config": with_cache(cfg_dict(world), eng.slow), "roofline": roof, "e2e": e2e, "gpu_launches": int(launches) * args.steps,
                 "clocks": clk.summary(),
                 "step_roofline": {"bound": "hbm", "algorithmic_bytes": nbytes, "flops": flops,
                                   "achieved_gbs": round(nbytes / (ms / args.steps / 1000.0) / 1e9, 1)}}
@@ -353,6 +375,11 @@ def roofline(eng, L, lens, dev, args):
 
     def attn_all():
         for l in range(st.layers):
+            if st.kv4 is not None:
+                L.call("a8_kv4_attention", C.byref(st.kv4.desc), l, L.ptr(sc.q), 896, 14, L.ptr(lens_d), None, b,
+                       st.cache_len, 0.0, L.ptr(sc.o), 896, L.ptr(sc.attn_ws), sc.attn_ws.numel(), L.ptr(sc.attn_counters),
+                       sc.attn_counters.numel(), L.stream_handle())
+                continue
             L.call("a8_attention", L.ptr(sc.q), 896, L.ptr(st.kc), L.ptr(st.vc), st.layers, st.cache_rows, 14, 2, 64,
                    st.cache_len, l, L.ptr(lens_d), None, b, st.cache_len, 0.0, L.ptr(sc.o), 896, L.ptr(sc.attn_ws),
                    sc.attn_ws.numel(), L.ptr(sc.attn_counters), sc.attn_counters.numel(), L.stream_handle())
@@ -364,7 +391,7 @@ def roofline(eng, L, lens, dev, args):
                    st.inter, C.byref(e), 0, L.stream_handle())
 
     t_attn = timed(attn_all, st.layers)
-    kv_bytes = 2 * 2 * 64 * 2 * int(lens.sum()) + b * 14 * 64 * 2 * 2
+    kv_bytes = int(2 * 2 * 64 * (2 if st.kv4 is None else KV4_BYTES) * int(lens.sum())) + b * 14 * 64 * 2 * 2
     t_w13 = timed(w13_all, st.layers)
     w13_bytes = 2 * st.inter * 896 * 2 + b * (896 + st.inter) * 2
     cand = {"attention": (t_attn, kv_bytes), "w13_gemm": (t_w13, w13_bytes)}
@@ -375,7 +402,7 @@ def roofline(eng, L, lens, dev, args):
     tp = os.path.join(REPO, "profiles", "traffic.json")
     if os.path.exists(tp):
         tr = json.load(open(tp)).get(name)
-        if tr:
+        if tr and (name != "attention" or st.kv4 is None):
             traffic = int(tr["bytes_per_unit"] * (int(lens.sum()) if name == "attention" else 1))
     return {"kernel": name, "bound": "hbm", "achieved": round(achieved, 1), "peak": hbm, "unit": "GB/s",
             "frac": round(achieved / hbm, 4), "peak_kind": kind, "traffic": traffic,
@@ -458,7 +485,8 @@ def run_ours_cfg2(args, rank, world, local):
     del model
     lens = cfg2_lengths()
     g = torch.Generator(device=dev).manual_seed(3 + rank)
-    for t in (eng.slow.kc, eng.slow.vc, eng.voc.post.kc, eng.voc.post.vc):
+    fill_slow(eng.slow, g, eng.slow.cache_rows)
+    for t in (eng.voc.post.kc, eng.voc.post.vc):
         t.normal_(generator=g)
     eng.voc.pos.fill_(1000)                               # steady state: every row attends a full 128-frame window
     cpos0 = (lens - 1).to(torch.int32).to(dev)
@@ -546,7 +574,7 @@ def run_ours_cfg2(args, rank, world, local):
         line = {"metric": METRIC, "value": round(value, 3), "unit": UNIT, "n_gpus": world, "steps": args.steps,
                 "warmup": args.warmup, "ms_per_step": round(tick_ms, 4), "higher_is_better": True,
                 "scaling": "weak", "vs_baseline": None, "dtype": "bf16 (codec convs fp16)", "data": "synthetic",
-                "config": cfg2_dict(world), "roofline": roof, "e2e": e2e, "gpu_launches": int(launches) * args.steps,
+                "config": with_cache(cfg2_dict(world), eng.slow), "roofline": roof, "e2e": e2e, "gpu_launches": int(launches) * args.steps,
                 "clocks": clk.summary(),
                 "realtime": {"frame_ms": round(1000 * eng.up / eng.sr, 3), "rtf_at_192": round(
                     tick_ms / (1000 * eng.up / eng.sr), 4)},
@@ -707,7 +735,7 @@ def run_serving(args, rank, world, local):
             "steps": sum(a["ticks"] for a in allr), "warmup": len(warm), "ms_per_step": round(
                 1000 * wall / max(1, max(a["ticks"] for a in allr)), 3),
             "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": "bf16 (codec convs fp16)",
-            "data": "synthetic", "config": serve_dict(args, world),
+            "data": "synthetic", "config": with_cache(serve_dict(args, world), eng.slow),
             "meets_target": ok, "mean_streams": round(streams, 1), "rtf_p95": round(p95_rtf, 4), "rtf_p50": round(float(np.percentile(rtf, 50)), 4),
             "ttfa_ms_p95": round(p95_ttfa, 1), "ttfa_ms_p50": round(float(np.percentile(ttfa, 50)), 1),
             "frames_per_s": round(frames / wall, 1), "finished": int(len(rtf)),
@@ -738,7 +766,8 @@ def cfg2_engine(rank=0):
     del model
     lens = cfg2_lengths()
     g = torch.Generator(device=dev).manual_seed(3 + rank)
-    for t in (eng.slow.kc, eng.slow.vc, eng.voc.post.kc, eng.voc.post.vc):
+    fill_slow(eng.slow, g, eng.slow.cache_rows)
+    for t in (eng.voc.post.kc, eng.voc.post.vc):
         t.normal_(generator=g)
     eng.voc.pos.fill_(1000)
     cpos0 = (lens - 1).to(torch.int32).to(dev)
