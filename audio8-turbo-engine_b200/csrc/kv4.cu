@@ -11,7 +11,7 @@
 // so any run of positions is one contiguous, 16-byte aligned piece (one bulk copy) with its scales beside its codes. The
 // order inside a record is the one in which tensor-core fragments (m16n8k16) are read from shared memory without bank
 // conflicts (position j = 4 i + (t ^ (3 if i odd)) is the i-th of the four positions that lane-in-quad t owns):
-//   K word (t', slot): dims 32 g + 8 t' .. + 7 at byte  j hd / 2 + (t' G + slot) 4
+//   K word (t', slot): dims 32 g + 8 t' .. + 7 at byte  j hd / 2 + (t' G + slot) 4, the first in the lowest nibble
 //   V half (q, slot):  dims 32 g + 4 q .. + 3 at byte   j hd / 2 + ((q ^ sw) G + slot) 2,  sw = 4 (j >> 1 & 1) at hd 128
 //   scale (j, slot):   element (4 t + i) G + slot
 // slot orders the groups so that group g and g + G / 2 (the two dims of a RoPE pair) are neighbours: 0, 2, 1, 3 at hd 128.
@@ -303,7 +303,7 @@ struct Kv4DecSmem {
   static constexpr int PART = (8 * NT * HD + 16 * NT) * 4;        // bytes: O [8 NT][hd], (max, sum) [8 NT]
   static constexpr int HEADP = NW * RING;                         // first partials; the last ones go into the rings
   static constexpr int PRE = HEADP + NW * PART;                   // prefix of the rows' steps by thread
-  static constexpr int META = PRE + (NW * 32 + 4) * 4;            // int [2 NW][3]: a piece's unit, its first and end step
+  static constexpr int META = PRE + (NW * 32 + 4) * 4;            // int [2 NW][4]: a piece's unit, its first and end step
   static constexpr int RUNS = META + 2 * NW * 4 * 4;              // int [2 NW] x 4: a unit's pieces [from, to); the pieces in
                                                                   // order; their runs
   static constexpr int WGT = RUNS + 2 * NW * 4 * 4;               // float [2 NW][8 NT]: a piece's weight in its unit
@@ -404,7 +404,8 @@ __device__ __forceinline__ void kv4_cursor_next(const Kv4AttnArgs& a, Kv4Cursor&
 //   layout of S is the B operand of the second product, no exchange between lanes. Codes are operands as they stand: K's
 //   nibbles are masked to fp16 subnormals u 2^-24 (code + 8 = u: 8 times the query's sum is taken off each group's product
 //   in fp32, then it is scaled by s_k); V's become bf16 by a mask and a fused multiply-add; P is multiplied by s_v in fp32
-//   before its rounding to bf16. The query is fp16, scaled by a power of two (8 bits in 11).
+//   before its rounding to bf16, whose range holds the product whatever the scale (fp16 would take a running power of two of
+//   the scales); it is the rounding that the bf16 cache's decode attention gives its weights. The query is fp16, scaled by a power of two (8 bits in 11).
 //   Running maximum per head, moved only when a logit passes it by 2^8 (then O and the sum are rescaled); sums and O fp32.
 // Why mma.sync and not tcgen05: up to 16 query heads share a kv head, a 128-row tile would be an eighth full at best, and
 // its operands would have to be written to shared memory as 16-bit values; here they never leave registers.

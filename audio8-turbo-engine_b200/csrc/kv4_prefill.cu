@@ -11,8 +11,10 @@
 // fp16, not bf16: code * s has 8 + 3 significant bits, so K and V are exact in fp16's 11 where bf16 would round each to 8.
 // Its narrow range is met by powers of two: a tile's K is divided by 2^ek (its largest scale in [1, 2)), which the softmax
 // multiplies back into its logit scale; V by 2^E, the largest scale met so far, which joins the running maximum's factor
-// on O when it grows; a query vector by its own largest element. P is fp16 with weights up to 2^14 (the running maximum
-// is moved only when a logit passes it by 2^8), rounded to 11 bits; sums and O in fp32.
+// on O when it grows; a query vector by its own largest element. The exponents are those of the tile's keys up to the
+// block's last position, keys behind a row among them. P is fp16 with weights up to 2^15 (the running maximum is moved where a
+// logit passes it by 2^8, and only looked at where a tile's weights of a row sum to more than 2^15), rounded to 11 bits; sums
+// and O in fp32.
 // Bound: 8,189 positions, 32 heads over 8, hd 128: 549 GFLOP in 606 to 629 us, 890 TFLOP/s, 0.53 of a library product's rate. A key
 // tile takes its CTA about 1.38 us, 2,700 cycles, and no one unit is full in them: the products take 1,280 (S, with both
 // operands in shared memory, 48 an instruction where its arithmetic takes 32; P V 64), the 256 x 64 exponentials 1,024, and

@@ -178,7 +178,9 @@ int a8_kv4_attention_workspace(const A8KV4* c, int nq, int rows, int max_len, lo
  * gives zeros and records ERR_BOUNDS. scale <= 0: hd^-0.5. out may be q (of the same stride), else it does not overlap
  * it. counters: n_counters ints, zero before the first call (a call leaves them zero; after a recorded timeout, zero them
  * again); ws (16-byte aligned) and counters belong to one call at a time. The order of every sum depends only on the shape,
- * lens, cache rows and max_len of a call, so equal calls give equal bits. */
+ * lens, cache rows and max_len of a call, so equal calls give equal bits. Logits, sums and results are fp32; a softmax weight
+ * times its value's scale is rounded to bf16 (as a8_attention rounds its weights). Meant for |q| below 2^110 and
+ * |scale q.K| below 2^24; a larger one may give a NaN. */
 int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* lens, const int* rowmap,
                      int rows, int max_len, float scale, void* out, int out_stride, float* ws, long long ws_floats,
                      int* counters, int n_counters, a8_stream_t stream);
@@ -188,7 +190,9 @@ int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_stride, int
  * block with n <= 0 is skipped and rows of out that no block covers are left as they are; a row is in one block at most. A
  * block whose rows, cache row or positions are out of range writes nothing and records ERR_BOUNDS. hd 64 or 128, nq / nkv
  * from 1 to 16; out may be q (of the same stride). Codes times scales are exact in the fp16 that the products take, except
- * for values below 2^-14 of the largest in their 64-key tile (or, of V, in an earlier one): those are held to 2^-24 of it. */
+ * for values below 2^-14 of the largest in their 64-key tile (or, of V, in an earlier one): those are held to 2^-24 of it. The
+ * tile's keys behind a row count among them, up to the block's last position: one more than 2^14 times larger costs earlier
+ * rows of its tile bits. Softmax weights are rounded to fp16; logits and sums are fp32, |scale q.K| below 2^24 as above. */
 int a8_kv4_prefill_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* blocks,
                              int nblocks, int rows, float scale, void* out, int out_stride, a8_stream_t stream);
 

@@ -180,3 +180,114 @@ def test_a_single_row_of_any_row_stride(kv4):
         assert c.store(qkv, i0, i0, nq=nq, q=qkv[:, :Q]).data_ptr() == base.data_ptr()
         no_error(kv4)
         assert torch.equal(base[:Q], want[0]) and torch.equal(base[Q:W], x[0, Q:].cuda()) and bool((base[W:] == 5).all())
+
+
+# ------------------------------------------------------------------------------------------------- the bytes
+def codes_and_scales(c, n):
+    """Codes and scales of positions [0, n) of cache row 0, layer 0, read off the buffer by the layout in csrc/kv4.cu's head
+    comment: float64 [n, 2, nkv, hd] and [n, 2, nkv, hd / 32]."""
+    hd, nkv = c.hd, c.nkv
+    G = hd // 32
+    buf = c.buf.cpu().view(-1, 18 * hd)[:nkv * -(-c.cache_len // 16)].view(nkv, -1, 18 * hd)
+    slot = {64: [0, 1], 128: [0, 2, 1, 3]}[hd]                   # of group g
+    code, scale = torch.zeros(n, 2, nkv, hd), torch.zeros(n, 2, nkv, G)
+    for p in range(n):
+        rec, j = buf[:, p // 16], p % 16
+        i, t = [(i, t) for i in range(4) for t in range(4) if j == 4 * i + (t ^ 3 if i % 2 else t)][0]
+        sw = 4 * (j >> 1 & 1) if hd == 128 else 0
+        for g in range(G):
+            for d in range(32):
+                word = j * (hd // 2) + ((d // 8) * G + slot[g]) * 4 + (d % 8) // 2
+                half = 8 * hd + j * (hd // 2) + (((d // 4) ^ sw) * G + slot[g]) * 2 + (d % 4) // 2
+                for kv, byte in enumerate((word, half)):
+                    code[p, kv, :, 32 * g + d] = ((rec[:, byte].int() >> (4 * (d % 2))) & 15).float() - 8
+            for kv in range(2):
+                at = (16 + kv) * hd + ((4 * t + i) * G + slot[g]) * 2
+                scale[p, kv, :, g] = rec[:, at:at + 2].contiguous().view(BF)[:, 0].float()
+    return code.double(), scale.double()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_bytes_are_the_documented_layout(kv4, hd):
+    n, nkv = 37, 2
+    x = rnd(30, n, 2, nkv, hd)
+    x[3, 0, 1, 32:64] = 0
+    x[5, 1, 0, :32] *= 2.0 ** -110
+    x[7, 0, 0, 40] = float("nan")
+    c = one_row(kv4, x, hd)
+    no_error(kv4)
+    code, scale = codes_and_scales(c, n)
+    want, s = R.quantise(x)
+    assert torch.equal(code, want.flatten(-2))
+    assert torch.equal(scale.isnan(), s.isnan()) and torch.equal(scale.nan_to_num(), s.nan_to_num())
+
+
+@pytest.mark.parametrize("e", [0, 119, -92, -93, -94, -97, -101, -120])
+def test_quantiser_decides_every_quotient(kv4, e):
+    """Every 8-bit significand of a group's largest (times 2^e, e to either side of where the scale's range is shifted, and the
+    largest and smallest there are) against every bf16 number within 2^-6 of it, both signs: codes as 64 bits give them."""
+    hd, rows = 128, 512
+    mags = torch.arange(128, 256).double()
+    rest = torch.cat([mags * 2.0 ** -k for k in range(7)])           # against a largest of 128 .. 255
+    rest = torch.cat([rest, -rest])
+    groups = []
+    for m in mags.tolist():
+        r = rest[rest.abs() <= m]
+        r = torch.cat([r, torch.zeros(-len(r) % 31, dtype=torch.float64)]).view(-1, 31)
+        top = torch.full((len(r), 1), m, dtype=torch.float64)
+        top[::2] *= -1
+        groups.append(torch.cat([r[:, :13], top, r[:, 13:]], 1))
+    x = torch.cat(groups) * 2.0 ** (e - 7 if e < 119 else e)         # (the largest: 255 x 2^119, the next to infinity's 2^127)
+    x = torch.cat([x, torch.zeros(-len(x) % 8, 32, dtype=torch.float64)]).view(-1, 2, 1, hd)
+    x = x.float().to(BF)
+    for part in x.split(rows):
+        c = one_row(kv4, part, hd)
+        k, v = c.load(torch.arange(len(part), dtype=I32, device="cuda"), torch.zeros(len(part), dtype=I32, device="cuda"))
+        no_error(kv4)
+        want = R.values(part)
+        for got, w in ((k, want[:, 0]), (v, want[:, 1])):
+            assert torch.equal(got.cpu().double(), w.to(BF).double())
+
+
+# ------------------------------------------------------------------------------------------------- keys behind a row
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("which", [0, 1])
+def test_prompt_and_a_large_key_behind_a_row(kv4, hd, which):
+    """A key or value far above the others, late in a 64-key tile. Rows before it do not attend it; the prompt kernel's fp16
+    operands share the tile's exponent with it. Within fp16's normal range (2^10 here) those rows keep every bit; far beyond it
+    they stay within the bound that the header gives (values held to 2^-24 of the largest in the tile)."""
+    n, nq, nkv, at = 128, 4, 2, 60
+    x, q = rnd(31, n, 2, nkv, hd), rnd(32, n, nq * hd)
+    clean = prompt(kv4, one_row(kv4, x, hd), q, n)
+    for up in (10, 18, 22):
+        y = x.clone()
+        y[at, which] = (y[at, which].float() * 2.0 ** up).to(BF)
+        got = prompt(kv4, one_row(kv4, y, hd), q, n)
+        if up == 10:
+            assert torch.equal(got[:at], clean[:at])
+        check_prompt(kv4, y, q, hd)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_logits_of_a_million(kv4, hd):
+    """Logits up to about 2^20: finite, and one key takes the row."""
+    n, nq, nkv = 100, 4, 2
+    x, q = rnd(33, n, 2, nkv, hd), rnd(34, n, nq * hd)
+    x[:, 0] = (x[:, 0].float() * 2.0 ** 9).to(BF)
+    q = (q.float() * 2.0 ** 9).to(BF)
+    c = one_row(kv4, x, hd)
+    got = prompt(kv4, c, q, n)
+    lens = torch.arange(1, n + 1, dtype=I32, device="cuda")
+    dec = c.attention(q.cuda(), lens, torch.zeros(n, dtype=I32, device="cuda")).cpu().double()
+    no_error(kv4)
+    kv, qd = R.values(x), q.double().view(n, nq, hd)
+    for h in range(nq):
+        z = (qd[:, h] @ kv[:, 0, h * nkv // nq].T * hd ** -0.5)
+        z = z.masked_fill(torch.arange(n)[None] > torch.arange(n)[:, None], float("-inf"))
+        top = z.topk(min(2, n), -1).values
+        sure = (top[:, 0] - top[:, 1]) > 2.0 ** -10 * top[:, 0].abs() + 40     # (far above any rounding of a logit)
+        best = kv[:, 1, h * nkv // nq][z.argmax(-1)]
+        for o in (got, dec):
+            o = o.view(n, nq, hd)[:, h]
+            assert bool(o.isfinite().all())
+            assert bool(((o - best).abs() <= 2.0 ** -7 * best.abs())[sure].all()) and int(sure.sum()) > n // 2
