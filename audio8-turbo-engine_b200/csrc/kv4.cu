@@ -284,7 +284,8 @@ constexpr int KV4_CTAS = 148;         // one a SM
 constexpr int KV4_STEP = 32;           // positions a warp takes at a time: two records
 // Fewer steps than CTAs x this: fewer CTAs, so that short work is joined within a CTA. Measured with 12, 16, 24, 36, 48: one
 // row of 733 keys (two heads of 23 steps) 12.8, 12.9, 9.9, 9.9, 11.3 us; 192 rows x 8 heads of 1 to 128 keys 15.9, 16.0, 16.0,
-// 16.8, 19.6; long ones the same.
+// 16.8, 19.6; long ones the same. The other side of it: one row of 768 keys (48 steps, 2 CTAs, nothing cut) takes 10.3 us, one of
+// 769 (50 steps, 3 CTAs, both units cut between them) 14.7, one of 2,047 (6 CTAs) 13.6.
 constexpr int KV4_CTA_STEPS = 24;
 constexpr int KV4_WHOLE = 8;          // a unit of at most so many steps is not cut between warps
 constexpr float KV4_LAZY = 8.f;       // a running maximum moves when a logit passes it by 2^8
@@ -405,16 +406,20 @@ __device__ __forceinline__ void kv4_cursor_next(const Kv4AttnArgs& a, Kv4Cursor&
 //   nibbles are masked to fp16 subnormals u 2^-24 (code + 8 = u: 8 times the query's sum is taken off each group's product
 //   in fp32, then it is scaled by s_k); V's become bf16 by a mask and a fused multiply-add; P is multiplied by s_v in fp32
 //   before its rounding to bf16, whose range holds the product whatever the scale (fp16 would take a running power of two of
-//   the scales); it is the rounding that the bf16 cache's decode attention gives its weights. The query is fp16, scaled by a power of two (8 bits in 11).
+//   the scales); it is the rounding that the bf16 cache's decode attention gives its weights. The query is fp16, scaled by a
+//   power of two (8 bits in 11).
 //   Running maximum per head, moved only when a logit passes it by 2^8 (then O and the sum are rescaled); sums and O fp32.
 // Why mma.sync and not tcgen05: up to 16 query heads share a kv head, a 128-row tile would be an eighth full at best, and
 // its operands would have to be written to shared memory as 16-bit values; here they never leave registers.
 // Bound: at long lengths by the instructions that unpack and scale and by their latency at four (three) warps a scheduler,
-// not by memory: hd 64 takes about 240 warp instructions a record (ALU 100, FMA 85), half of all issue slots of the
-// call below. 3 rows x 8 heads of 40,009 to 131,071 keys, hd 128: 407 MB in 100 us, 4.1 TB/s; 1,408 rows x 2 heads of 97 to
-// 911 keys, hd 64: 106 MB in 41 us, 2.6 TB/s. Short ones by latency: launch 2.5 us, lengths and the split 2.5, first
-// records and queries 1.5, joining 2.5, a cut unit's join 3 to 5: 192 rows of 1 to 2,047 keys 22 us, one row of 733 keys
-// 9.8, 192 rows x 8 heads of 1 to 128 keys (hd 128) 14.8.
+//   not by memory: about 240 warp instructions a record at hd 64, 330 at hd 128; 56 % of the issue slots of the serving call
+//   below and 59 % of the long one's are taken (ALU 46 and 53 %, tensor pipe 22 and 34 %), the rest is latency. 3 rows x 8
+//   heads of 40,009 to 131,071 keys, hd 128: 407 MB in 99 us, 4.1 TB/s; 1,408 rows x 2 heads of 97 to 911 keys, hd 64: 106 MB
+//   in 41 us, 2.6 TB/s. 16 query heads a kv head instead of 8 (two tiles of 8, 12 warps at hd 64 and 8 at hd 128 by
+//   registers): 1,000 rows x 2 heads of 1 to 2,047 keys, hd 64, 68 us against 52; 500 rows, hd 128, 71 against 54.
+//   Short ones by latency: launch 2.5 us, lengths and the split 2.5, first records and queries 1.5, joining 2.5, a cut unit's
+//   join 3 to 5: 192 rows of 1 to 2,047 keys 22 us, one row of 733 keys 9.9, 192 rows x 8 heads of 1 to 128 keys (hd 128)
+//   14.8.
 template <int HD, int NT>
 __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(const Kv4AttnArgs a) {
   using F = Kv4<HD>;

@@ -15,13 +15,16 @@
 // block's last position, keys behind a row among them. P is fp16 with weights up to 2^15 (the running maximum is moved where a
 // logit passes it by 2^8, and only looked at where a tile's weights of a row sum to more than 2^15), rounded to 11 bits; sums
 // and O in fp32.
-// Bound: 8,189 positions, 32 heads over 8, hd 128: 549 GFLOP in 606 to 629 us, 890 TFLOP/s, 0.53 of a library product's rate. A key
-// tile takes its CTA about 1.38 us, 2,700 cycles, and no one unit is full in them: the products take 1,280 (S, with both
-// operands in shared memory, 48 an instruction where its arithmetic takes 32; P V 64), the 256 x 64 exponentials 1,024, and
-// the issue slots of 8 softmax and 8 unpacking warps the most. An admission (2,048 ragged rows behind prefixes of 317, 14
-// heads over 2, hd 64) takes 21 to 29 us, as long as its longest prompt's last block and the filling of the pipeline.
+// Bound: 8,189 positions, 32 heads over 8, hd 128: 549 GFLOP in 607 to 644 us, 890 TFLOP/s, 0.53 of a library product's rate. A
+// key tile takes its CTA about 1.38 us, 2,700 cycles, and no unit is full in them (4,093 positions: tensor pipe active 36 % of
+// the cycles, exponentials' unit 37 %, ALU 30 %, issue slots 51 %): a tile's chain, unpacking -> S -> softmax -> P V, two stages
+// of S deep, waits on itself. The tile's time hardly depends on hd or on the heads it serves: 14 heads over 2, hd 64, 1.29 us
+// (8,189 positions 288 us, 418 TFLOP/s); one head a kv head, where 64 of the 256 query vectors are used, 1.06 us (8 over 8,
+// hd 128, 475 us, 289 TFLOP/s). An admission (2,048 ragged rows behind prefixes of 317, 14 heads over 2, hd 64) takes 20 to 29
+// us, as long as its longest prompt's last block, a second wave where there are more than 148 CTAs, and the filling of the
+// pipeline.
 // Measured and not kept: exponentials as polynomials on the FMA pipe for 1/4, 1/2, 3/4 of the weights (707, 740, 998 us
-// against 693 then: issue slots are short, not the exponentials' unit). On the way: S and P V issued by one warp 905 us, by
+// against 693 then). On the way: S and P V issued by one warp 905 us, by
 // two 693; every tile's maximum before its weights 693, only where their sum asks for it 673; warp indexes that the compiler
 // cannot see are uniform 650, shuffled from one lane 620; the second half of S fetched behind the first half's weights 684
 // against 646; the two tiles' softmax started half a tile apart no gain.
