@@ -214,7 +214,7 @@ def device_error():
     return tuple(out)
 
 
-# What keeps attention counters on the device between calls: objects with a reset()
+# What keeps attention counters on the device between calls: objects with a reset_counters()
 counters = weakref.WeakSet()
 
 
@@ -223,7 +223,7 @@ def clear_error():
     advanced: those of every live KV4Cache and engine scratch (a workspace of the caller's own is the caller's to zero)."""
     call("a8_clear_error")
     for o in list(counters):
-        o.reset()
+        o.reset_counters()
 
 
 def ptr(t):

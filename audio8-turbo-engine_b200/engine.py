@@ -134,10 +134,11 @@ class Scratch:
         self.rows = rows
         L.counters.add(self)
 
-    def reset(self):
+    def reset_counters(self):
         """The counters as they were at first (`clear_error` calls it; nothing may be in flight)."""
         self.attn_counters.zero_()
-        torch.cuda.synchronize(self.attn_counters.device)
+        if self.attn_counters.is_cuda:
+            torch.cuda.synchronize(self.attn_counters.device)
 
 
 class FastEngine:

@@ -50,9 +50,9 @@ class KV4Cache:
         self._ws = {}
         L.counters.add(self)
 
-    def reset(self):
-        """Drop the workspaces of `attention`: after a wait that ran out (`device_error`) their tickets may be partly taken,
-        and later calls would join too early. `clear_error` of the package calls it for every cache."""
+    def reset_counters(self):
+        """Drop the workspaces of `attention` (not what the cache holds): after a wait that ran out (`device_error`) their
+        tickets may be partly taken, and later calls would join too early. The package's `clear_error` calls it."""
         self._ws.clear()
 
     @property
