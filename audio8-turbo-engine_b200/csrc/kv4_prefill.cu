@@ -11,23 +11,25 @@
 // fp16, not bf16: code * s has 8 + 3 significant bits, so K and V are exact in fp16's 11 where bf16 would round each to 8.
 // Its narrow range is met by powers of two: a tile's K is divided by 2^ek (its largest scale in [1, 2)), which the softmax
 // multiplies back into its logit scale; V by 2^E, the largest scale met so far, which joins the running maximum's factor
-// on O when it grows; a query vector by its own largest element. The exponents are those of the tile's keys up to the
-// block's last position, keys behind a row among them. P is fp16 with weights up to 2^15 (the running maximum is moved where a
-// logit passes it by 2^8, and only looked at where a tile's weights of a row sum to more than 2^15), rounded to 11 bits; sums
-// and O in fp32.
-// Bound: 8,189 positions, 32 heads over 8, hd 128: 549 GFLOP in 607 to 644 us, 890 TFLOP/s, 0.53 of a library product's rate. A
-// key tile takes its CTA about 1.38 us, 2,700 cycles, and no unit is full in them (4,093 positions: tensor pipe active 36 % of
-// the cycles, exponentials' unit 37 %, ALU 30 %, issue slots 51 %): a tile's chain, unpacking -> S -> softmax -> P V, two stages
-// of S deep, waits on itself. The tile's time hardly depends on hd or on the heads it serves: 14 heads over 2, hd 64, 1.29 us
-// (8,189 positions 288 us, 418 TFLOP/s); one head a kv head, where 64 of the 256 query vectors are used, 1.06 us (8 over 8,
-// hd 128, 475 us, 289 TFLOP/s). An admission (2,048 ragged rows behind prefixes of 317, 14 heads over 2, hd 64) takes 20 to 29
-// us, as long as its longest prompt's last block, a second wave where there are more than 148 CTAs, and the filling of the
-// pipeline.
+// on O when it grows; a query vector by its own largest element. In a block's own tiles, the last ones, keys behind a row may
+// be far above those that it attends: where a tile's scales there lie more than 2^14 apart (past what fp16 holds exactly) each
+// key is divided by its own exponents, and each row brings its logits and weights to the largest that it attends, so that no
+// row depends on a key behind it (such tiles throughout: 8 to 33 % slower). P is fp16 with weights up to 2^15 (the running
+// maximum is moved where a logit passes it by 2^8, and only looked at where a tile's weights of a row sum to more than 2^15),
+// rounded to 11 bits; sums and O in fp32.
+// Bound: 8,189 positions, 32 heads over 8, hd 128: 549 GFLOP in 576 to 617 us, 900 to 950 TFLOP/s, 0.55 of a library product's
+// rate. A key tile takes its CTA about 1.3 us, 2,500 cycles, and no unit is full in them: a tile's chain, unpacking -> S ->
+// softmax -> P V, two stages of S deep, waits on itself. The tile's time hardly depends on hd or on the heads it serves: 14 heads
+// over 2, hd 64, 1.26 us (8,189 positions 281 us, 427 TFLOP/s); one head a kv head, where 64 of the 256 query vectors are used,
+// 1.0 us (8 over 8, hd 128, 445 us, 309 TFLOP/s). An admission (2,048 ragged rows behind prefixes of 317, 14 heads over 2, hd 64)
+// takes 20 to 29 us, as long as its longest prompt's last block, a second wave where there are more than 148 CTAs, and the
+// filling of the pipeline.
 // Measured and not kept: exponentials as polynomials on the FMA pipe for 1/4, 1/2, 3/4 of the weights (707, 740, 998 us
-// against 693 then). On the way: S and P V issued by one warp 905 us, by
-// two 693; every tile's maximum before its weights 693, only where their sum asks for it 673; warp indexes that the compiler
-// cannot see are uniform 650, shuffled from one lane 620; the second half of S fetched behind the first half's weights 684
-// against 646; the two tiles' softmax started half a tile apart no gain.
+// against 693 then). On the way: S and P V issued by one warp 905 us, by two 693; every tile's maximum before its weights 693,
+// only where their sum asks for it 673; warp indexes that the compiler cannot see are uniform 650, shuffled from one lane 620;
+// the second half of S fetched behind the first half's weights 684 against 646; the two tiles' softmax started half a tile
+// apart no gain; masks and wide scales in a loop of their own for the block's own tiles 576 against 607, where a test more
+// between the other tiles' instructions gave 617 to 730.
 // Within a chunk of eight dims Q and K keep the order 0 4 1 5 2 6 3 7, in which the codes come out of their words.
 #include "common.cuh"
 
@@ -48,6 +50,7 @@ static_assert(kv4p_registers_cover(96), "");
 constexpr int KV4P_RAW = 6;                              // raw key tiles in flight
 constexpr int KV4P_VST = 3;                              // V tiles at hand
 constexpr float KV4P_BIAS = 6.f;                         // p = 2^(x - m + 6)
+constexpr int KV4P_WIDE = 256;                           // in ek: the tile's keys have exponents of their own
 
 template <int HD>
 struct Kv4PreSmem {
@@ -62,7 +65,8 @@ struct Kv4PreSmem {
   static constexpr int SC = RAW + KV4P_RAW * RAWT;       // a raw tile's scales as fp16, divided: K [64 keys][G], V [G][64 keys]
   static constexpr int SCT = 2 * 64 * (HD / 32) * 2;
   static constexpr int MISC = SC + KV4P_RAW * SCT;       // int ek[16], ev[16], nanv[4]
-  static constexpr int BARS = MISC + 144;
+  static constexpr int KEYX = MISC + 144;                // a tile's exponents by key: K [16][64], V [16][64] bytes
+  static constexpr int BARS = KEYX + 2 * 16 * 64;
   static constexpr int TOTAL = BARS + 40 * 8 + 16 + 1024;
   static constexpr uint32_t COLS = 512;                  // TMEM: S of tile 0 and 1, two stages of 64 each (P takes
                                                          // the first half of its S); O (HD each)
@@ -80,6 +84,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
       "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, float* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const float* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0,%1,%2,%3};\n\ttcgen05.wait::st.sync.aligned;" ::"f"(v[0]),
+               "f"(v[1]), "f"(v[2]), "f"(v[3]), "r"(taddr)
+               : "memory");
 }
 
 // 64 columns at once
@@ -146,6 +162,8 @@ __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<ui
 // 2^(e - 127) for a biased exponent e, and its inverse; both normal for e in [1, 253]
 __device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float(uint32_t(e) << 23); }
 __device__ __forceinline__ float pow2_biased_inv(int e) { return __uint_as_float(uint32_t(254 - e) << 23); }
+// 2^(e - of) for e up to of; 0 below 2^-126, and whatever for a larger e (a masked key's) is finite
+__device__ __forceinline__ float pow2_diff(int e, int of) { return pow2_biased(max(127 + min(e - of, 0), 0)); }
 
 template <int HD>
 __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a) {
@@ -157,6 +175,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
   int* ek = reinterpret_cast<int*>(smem + SM::MISC);     // by tile % 16
   int* ev = ek + 16;
   int* nanv = ev + 16;                                   // [4] first position whose V group is NaN
+  uint8_t *keyk = smem + SM::KEYX, *keyv = keyk + 16 * 64;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + SM::BARS);
   uint64_t *raw_full = q_full + 1, *raw_free = raw_full + KV4P_RAW, *e_full = raw_free + KV4P_RAW, *k_full = e_full + KV4P_RAW,
            *k_free = k_full + 2, *v_full = k_free + 2, *v_free = v_full + KV4P_VST, *s_full = v_free + KV4P_VST, *p_full = s_full + 4,
@@ -180,6 +199,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
   const int head0 = kvh * a.group + 4 * hpart;
   const int ntx = (heads + 1) / 2;                       // tiles in use
   const int klen = pos0 + nrow, nt = (klen + 63) / 64;
+  const int first = (pos0 + 1) / 64;                     // the first tile that some row does not attend to its end
 
   if (tid == 0) {
     mbar_init(q_full, KV4P_SOFT);
@@ -252,17 +272,42 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
     float m = -INFINITY, l = 0.f;
     int E = 0;
     bool ok = true;
-    for (int j = 0; x < ntx && j < nt; ++j) {
+    // A key tile (false: no further). own: keys behind a row may be in it, and its scales may be wide.
+    auto tile = [&](auto own, const int j) {
       const int b = 2 * x + (j & 1), ph = (j >> 1) & 1;
-      if (!(ok = mbar_wait_all(&s_full[b], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) break;
+      if (!(ok = mbar_wait_all(&s_full[b], ph, ERR_TIMEOUT_FULL, KERNEL_ID_KV4_PREFILL))) return false;
       tc_fence_after();
+      const int kmax = pos - 64 * j;                     // keys c <= kmax of this tile are causal for this row
+      int ex = ek[j & 15], Ej = ev[j & 15];
+      bool wide = false;
+      if constexpr (decltype(own)::value) {
+        wide = ex >= KV4P_WIDE;
+        if (kmax < 0) Ej = E;                            // (a row that attends none of them keeps its E)
+      }
+      if (wide) {
+        // each key by its own exponents: the row's are the largest that it attends, and its logits are brought to them
+        const uint8_t *kx = keyk + (j & 15) * 64, *vx = keyv + (j & 15) * 64;
+        ex = 1;
+        Ej = E;
+#pragma unroll 1
+        for (int c = 0; c < 64; ++c) {
+          ex = max(ex, c <= kmax ? int(kx[c]) : 0);
+          Ej = max(Ej, c <= kmax ? int(vx[c]) : 0);
+        }
+#pragma unroll 1
+        for (int c = 0; c < 64; c += 4) {
+          float z[4];
+          tmem_ld4(tS + (j & 1) * 64 + c, z);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) z[k] *= pow2_diff(kx[c + k], ex);
+          tmem_st4(tS + (j & 1) * 64 + c, z);
+        }
+      }
       float sv[64];
       tmem_ld64(tS + (j & 1) * 64, sv);
       // (never 0, which would make a masked -infinity NaN; at this least value every logit is below 2^-110)
-      const float f = fmaxf(qs * pow2_biased(ek[j & 15]), 0x1p-126f);
-      const int Ej = ev[j & 15];
-      const int kmax = pos - 64 * j;                     // keys c <= kmax of this tile are causal for this row
-      if (__any_sync(0xffffffffu, kmax < 63)) {
+      const float f = fmaxf(qs * pow2_biased(ex), 0x1p-126f);
+      if (decltype(own)::value && __any_sync(0xffffffffu, kmax < 63)) {
 #pragma unroll
         for (int c = 0; c < 64; ++c) sv[c] = c <= kmax ? sv[c] : -INFINITY;
       }
@@ -290,7 +335,7 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
             // O is at rest once the previous tile's product is complete: scale it in place
             const float oa = al * (Ej > E ? pow2_biased(max(127 + E - Ej, 0)) : 1.f);
             if (!(ok = mbar_wait_all(&p_free[b ^ 1], ((j - 1) >> 1) & 1, ERR_TIMEOUT_OTHER, KERNEL_ID_KV4_PREFILL)))
-              break;
+              return false;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
@@ -319,13 +364,32 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
         if (full || !__any_sync(0xffffffffu, sum > 32768.f)) break;
         full = true;
       }
-      if (!ok) break;
       tmem_st32(tS + (j & 1) * 64, reinterpret_cast<const float*>(pk));
+      if (wide) {
+        // the values stand divided by their keys' exponents, O by the row's E: the weights take the difference
+        const uint8_t* vx = keyv + (j & 15) * 64;
+#pragma unroll 1
+        for (int c = 0; c < 32; c += 4) {
+          float z[4];
+          tmem_ld4(tS + (j & 1) * 64 + c, z);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 p = unpack_f16(__float_as_uint(z[k]));
+            z[k] = __uint_as_float(pack_f16(p.x * pow2_diff(vx[2 * (c + k)], E), p.y * pow2_diff(vx[2 * (c + k) + 1], E)));
+          }
+          tmem_st4(tS + (j & 1) * 64 + c, z);
+        }
+      }
       l += sum;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[b]);
-    }
+      return true;
+    };
+    // (two loops: what the last tiles need is not between the instructions of the others)
+    int j = 0;
+    while (x < ntx && j < first && tile(std::false_type(), j)) ++j;
+    while (x < ntx && ok && j < nt && tile(std::true_type(), j)) ++j;
     if (x < ntx && ok) {
       ok = mbar_wait_all(&p_free[2 * x + ((nt - 1) & 1)], ((nt - 1) >> 1) & 1, ERR_TIMEOUT_ACCUM, KERNEL_ID_KV4_PREFILL);
       tc_fence_after();
@@ -518,6 +582,13 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
         for (int i = 0; i < G / 2; ++i) m = __vmaxu2(m, __vmaxu2(w[0][i], w[1][i]));
         return __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
       };
+      // the smallest of the lane's scales but zero, less 32,769 (a zero counts as large: as a signed number of 16 bits, w + 0x7FFF)
+      auto least = [](const uint32_t (&w)[2][G / 2]) {
+        uint32_t m = 0x7FFF7FFFu;
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i) m = __vmins2(m, __vmins2(w[0][i] + 0x7FFF7FFFu, w[1][i] + 0x7FFF7FFFu));
+        return min(int(int16_t(m)), int(m) >> 16);
+      };
       auto without_nan = [](const uint32_t (&w)[2][G / 2], uint32_t (&o)[2][G / 2]) {
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -570,11 +641,16 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
           }
           topv = largest(vw);
         }
-        const int ex = min(max(int(topk >> 7), 1), 253);
+        const int ex = min(max(int(topk >> 7), 1), 253), before = E;
         E = max(E, min(int(topv >> 7), 253));
+        const float dk = pow2_biased_inv(ex), dv = pow2_biased_inv(E);
+        // Scales 2^14 below the largest are past what fp16 holds exactly, and in the block's own tiles the largest may be that
+        // of a key behind a row.
+        const bool wide = 64 * j + 63 > pos0 &&
+                          __any_sync(0xffffffffu, least(kw) < (ex - 14) * 128 - 32769 || least(vw) < (E - 14) * 128 - 32769 ||
+                                                      (before > 1 && before + 14 < E));
         __half* tk = reinterpret_cast<__half*>(smem + SM::SC + rs * SM::SCT);
         __half* tv = tk + 64 * G;
-        const float dk = pow2_biased_inv(ex), dv = pow2_biased_inv(E);
 #pragma unroll
         for (int i = 0; i < G / 2; ++i) {
           float2 v[2];
@@ -587,9 +663,36 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
           *reinterpret_cast<uint32_t*>(tv + 2 * i * 64 + k0) = pack_f16(v[0].x, v[1].x);
           *reinterpret_cast<uint32_t*>(tv + (2 * i + 1) * 64 + k0) = pack_f16(v[0].y, v[1].y);
         }
+        if (wide) {
+          // each key divided by its own largest scale's exponents instead; each row goes by the keys that it attends
+#pragma unroll 1
+          for (int k = k0; k < k0 + 2; ++k) {
+            const uint32_t* ks = reinterpret_cast<const uint32_t*>(raw + F::KS0 + (k >> 4) * F::REC + F::scale(k & 15, 0));
+            const uint32_t* vs = ks + (F::VS0 - F::KS0) / 4;
+            uint32_t kt = 0, vt = 0;
+            auto finite = [](uint32_t h) { return h < 0x7F80u ? h : 0u; };
+#pragma unroll
+            for (int i = 0; i < G / 2; ++i) {
+              kt = max(kt, max(finite(ks[i] & 0xFFFFu), finite(ks[i] >> 16)));
+              vt = max(vt, max(finite(vs[i] & 0xFFFFu), finite(vs[i] >> 16)));
+            }
+            const int ak = k < left ? min(max(int(kt >> 7), 1), 253) : 1, av = k < left ? min(max(int(vt >> 7), 1), 253) : 1;
+            keyk[(j & 15) * 64 + k] = uint8_t(ak);
+            keyv[(j & 15) * 64 + k] = uint8_t(av);
+#pragma unroll
+            for (int i = 0; i < G / 2; ++i) {
+              const float2 x = unpack_bf16(k < left ? ks[i] : 0u);
+              *reinterpret_cast<uint32_t*>(tk + k * G + 2 * i) = pack_f16(x.x * pow2_biased_inv(ak), x.y * pow2_biased_inv(ak));
+              const uint32_t w = k < left ? vs[i] : 0u;
+              const float2 y = unpack_bf16(finite(w & 0xFFFFu) | finite(w >> 16) << 16);
+              tv[2 * i * 64 + k] = __float2half_rn(y.x * pow2_biased_inv(av));
+              tv[(2 * i + 1) * 64 + k] = __float2half_rn(y.y * pow2_biased_inv(av));
+            }
+          }
+        }
         __syncwarp();
         if (lane == 0) {
-          ek[j & 15] = ex;
+          ek[j & 15] = ex | (wide ? KV4P_WIDE : 0);
           ev[j & 15] = E;
           mbar_arrive(&e_full[rs]);
           mbar_arrive(&raw_free[rs]);

@@ -65,15 +65,17 @@ def prompt_slack(q, k, v, first, scale):
     the tile. A scale's quotient and its product with a code (8 and 8 + 3 bits, below 2 and 14) are exact while they are
     normal fp16 numbers; below 2^-14 each is off by at most half a subnormal step, 2^-25, the quotient's error times a code
     of up to 7. So an element of V is off by at most (7 + 1) 2^-25 2^E, of K by 8 2^-25 2^e, and of q (one rounding) by
-    2^-25 2^f. With s <= (max|x| / 7)(1 + 2^-8), 2^e <= max|k| / 6.9 over the tile (the weights add up to one, so V's term
-    passes to the output as it is); a logit moves by at most scale (sum_d |q_d| 8 2^-25 max|k| / 6.9 +
-    sum_d |k_d| 2^-25 max|q|), a weight by as much of itself, in the numerator and in the sum below."""
-    m, n = q.shape[0], k.shape[0]
+    2^-25 2^f. Where a tile's scales lie further apart and keys behind a row are in it, each key has its own exponents, below those
+    of the largest that the row attends. With s <= (max|x| / 7)(1 + 2^-8), 2^e <= max|k| / 6.9 over the keys that the row
+    attends (the weights add up to one, so V's term passes to the output as it is); a logit moves by at most
+    scale (sum_d |q_d| 8 2^-25 max|k| / 6.9 + sum_d |k_d| 2^-25 max|q|), a weight by as much of itself, in the numerator and in
+    the sum below. A weight below 2^-14 of its scale is off by 2^-25, against a sum of at least 2^6 (the largest is 2^6 or
+    more), times up to 14 2^E of V: 14 2^-31 max|v| / 6.9 a key."""
+    m = q.shape[0]
     out = torch.zeros(m, q.shape[1], dtype=torch.float64)
     for i in range(m):
         last = first + i + 1
-        seen = min(n, -(-last // 64) * 64)               # the row's last tile whole: later keys of it set exponents too
-        kmax, vmax = k[:seen].abs().max(), v[:seen].abs().max()
+        kmax, vmax = k[:last].abs().max(), v[:last].abs().max()
         move = scale * 2.0 ** -25 * (8 / 6.9 * q[i].abs().sum() * kmax + k[:last].abs().sum(1).max() * q[i].abs().max())
-        out[i] = 8 / 6.9 * 2.0 ** -25 * vmax + 2 * move * v[:last].abs().max(0).values
+        out[i] = (8 / 6.9 * 2.0 ** -25 + last * 14 / 6.9 * 2.0 ** -31) * vmax + 2 * move * v[:last].abs().max(0).values
     return out

@@ -253,9 +253,8 @@ def test_quantiser_decides_every_quotient(kv4, e):
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("which", [0, 1])
 def test_prompt_and_a_large_key_behind_a_row(kv4, hd, which):
-    """A key or value far above the others, late in a 64-key tile. Rows before it do not attend it; the prompt kernel's fp16
-    operands share the tile's exponent with it. Within fp16's normal range (2^10 here) those rows keep every bit; far beyond it
-    they stay within the bound that the header gives (values held to 2^-24 of the largest in the tile)."""
+    """A key or value far above the others, late in a 64-key tile: rows before it, which do not attend it, keep every bit, the
+    others are within their bound."""
     n, nq, nkv, at = 128, 4, 2, 60
     x, q = rnd(31, n, 2, nkv, hd), rnd(32, n, nq * hd)
     clean = prompt(kv4, one_row(kv4, x, hd), q, n)
@@ -263,8 +262,7 @@ def test_prompt_and_a_large_key_behind_a_row(kv4, hd, which):
         y = x.clone()
         y[at, which] = (y[at, which].float() * 2.0 ** up).to(BF)
         got = prompt(kv4, one_row(kv4, y, hd), q, n)
-        if up == 10:
-            assert torch.equal(got[:at], clean[:at])
+        assert torch.equal(got[:at], clean[:at])
         check_prompt(kv4, y, q, hd)
 
 
@@ -291,3 +289,42 @@ def test_logits_of_a_million(kv4, hd):
             o = o.view(n, nq, hd)[:, h]
             assert bool(o.isfinite().all())
             assert bool(((o - best).abs() <= 2.0 ** -7 * best.abs())[sure].all()) and int(sure.sum()) > n // 2
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("pos0", [0, 37])
+def test_prompt_rows_do_not_depend_on_keys_behind_them(kv4, hd, which, pos0):
+    """However large a key or value is that a row does not attend, the row keeps every bit: within a tile, in a block over two
+    tiles, among zeros, with an infinity."""
+    n, nq, nkv, at = 64, 4, 2, pos0 + 43
+    S = pos0 + n
+    x, q = rnd(35, S, 2, nkv, hd), rnd(36, n, nq * hd)
+    blocks = torch.tensor([[0, n, 0, pos0]], dtype=I32, device="cuda")
+
+    def run(y):
+        out = one_row(kv4, y, hd).prefill_attention(q.cuda(), blocks)
+        no_error(kv4)
+        return out.cpu()[:at - pos0]
+    for thin in (False, True):
+        x = x.clone()
+        if thin:                                          # (the tile's own exponent is then the large key's alone)
+            x[at // 64 * 64:at] = 0
+            x[at + 1:] = 0
+        clean = run(x)
+        assert bool(clean.isfinite().all())
+        for up in (10, 16, 18, 22, 40, 60, 100, 120, float("inf")):
+            y = x.clone()
+            y[at, which] = (y[at, which].float().clamp(-2, 2) * 2.0 ** up).to(BF)
+            assert torch.equal(run(y), clean), up
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_with_keys_and_values_of_every_size(kv4, hd):
+    """Scales over 2^40 within a tile, in any order."""
+    n, nq, nkv = 200, 4, 2
+    g = torch.Generator().manual_seed(37)
+    x, q = rnd(38, n, 2, nkv, hd), rnd(39, n, nq * hd)
+    x[:, 0] *= (2.0 ** torch.randint(-40, 3, (n,), generator=g).float()).to(BF)[:, None, None]
+    x[:, 1] *= (2.0 ** torch.randint(-20, 21, (n,), generator=g).float()).to(BF)[:, None, None]
+    check_prompt(kv4, x, q, hd)
