@@ -13,8 +13,8 @@
 // multiplies back into its logit scale; V by 2^E, the largest scale met so far, which joins the running maximum's factor
 // on O when it grows; a query vector by its own largest element. In a block's own tiles, the last ones, keys behind a row may
 // be far above those that it attends: where a tile's scales there lie more than 2^14 apart (past what fp16 holds exactly) each
-// key is divided by its own exponents, and each row brings its logits and weights to the largest that it attends, so that no
-// row depends on a key behind it (such tiles throughout: 8 to 33 % slower). P is fp16 with weights up to 2^15 (the running
+// key is divided by its own exponents, and each row brings its logits and weights to the largest that it attends, so that
+// keys behind a row cost it no bits (such tiles throughout: 8 to 33 % slower). P is fp16 with weights up to 2^15 (the running
 // maximum is moved where a logit passes it by 2^8, and only looked at where a tile's weights of a row sum to more than 2^15),
 // rounded to 11 bits; sums and O in fp32.
 // Bound: 8,189 positions, 32 heads over 8, hd 128: 549 GFLOP in 576 to 617 us, 900 to 950 TFLOP/s, 0.55 of a library product's
@@ -313,7 +313,8 @@ __global__ void __launch_bounds__(KV4P_THREADS, 1) k_kv4_prefill(const Kv4AttnAr
       }
       // The weights are formed against the maximum at hand; only where their sum says that one may pass fp16's range (or in
       // the first tile, or when E grows) is the tile's own maximum looked for, the running maximum moved where a logit
-      // passes it by 2^8, and the weights formed again.
+      // passes it by 2^8, and the weights formed again. (For the whole warp: a row's maximum may move because another row's
+      // does, a rounding of its weights apart. A test of each row's own sum spills at hd 128, 633 us against 576.)
       bool full = __any_sync(0xffffffffu, j == 0 || Ej > E);
       uint32_t pk[32];
       float sum;

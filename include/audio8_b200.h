@@ -191,7 +191,7 @@ int a8_kv4_attention(const A8KV4* c, int layer, const void* q, int q_stride, int
  * block whose rows, cache row or positions are out of range writes nothing and records ERR_BOUNDS. hd 64 or 128, nq / nkv
  * from 1 to 16; out may be q (of the same stride). Codes times scales are exact in the fp16 that the products take, except
  * for values below 2^-14 of the largest that the row attends in their 64-key tile (or, of V, in an earlier one): those are
- * held to 2^-24 of it. Keys behind a row do not touch it. Softmax weights are rounded to fp16; logits and sums are fp32, |scale q.K| below 2^24 as above. */
+ * held to 2^-24 of it. Keys behind a row cost it no bits. Softmax weights are rounded to fp16; logits and sums are fp32, |scale q.K| below 2^24 as above. */
 int a8_kv4_prefill_attention(const A8KV4* c, int layer, const void* q, int q_stride, int nq, const int* blocks,
                              int nblocks, int rows, float scale, void* out, int out_stride, a8_stream_t stream);
 
