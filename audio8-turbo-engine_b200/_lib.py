@@ -219,8 +219,8 @@ counters = weakref.WeakSet()
 
 
 def clear_error():
-    """Clear the device-side error record, and the counters that a kernel which gave up a wait may have left partly
-    advanced: those of every live KV4Cache and engine scratch (a workspace of the caller's own is the caller's to zero)."""
+    """Clear the device-side error record, and bring the counters that kernels join by back to zero, whatever happened to
+    them: those of every live KV4Cache and engine scratch (a workspace of the caller's own is the caller's to zero)."""
     call("a8_clear_error")
     for o in list(counters):
         o.reset_counters()

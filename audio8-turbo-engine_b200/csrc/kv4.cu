@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
   extern __shared__ __align__(128) uint8_t smem[];
   int* pre = reinterpret_cast<int*>(smem + SM::PRE);
   int* meta = reinterpret_cast<int*>(smem + SM::META);
-  __shared__ int s_sum[32], s_runs, s_pieces, s_last[2], s_split[4];
+  __shared__ int s_sum[32], s_runs, s_pieces, s_last[2], s_split[4], s_lost;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::BARS) + warp * NST;
   uint8_t* ring = smem + warp * SM::RING;
@@ -437,6 +437,7 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     for (int s = 0; s < NST; ++s) mbar_init(&full[s], 1);
   fence_mbar_init();
   if (tid < 2 * NW) meta[4 * tid] = -1;
+  if (tid == 0) s_lost = 0;
   pdl_wait();
 
   // ---- how many steps every row has: a prefix by thread (rows in equal runs), and zeros into rows without keys
@@ -516,12 +517,16 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
     const int x = int((long long)T * b / ctas);
     return b == 0 || b == ctas ? x : moved(x, share / 2);
   };
-  int b0 = begin(blockIdx.x), b1 = begin(blockIdx.x + 1);
-  int w0 = b0 + int((long long)(b1 - b0) * warp / NW), w1 = b0 + int((long long)(b1 - b0) * (warp + 1) / NW);
-  if (T <= (long long)KV4_WHOLE * a.rows * a.c.nkv) {
-    if (warp > 0) w0 = max(b0, moved(w0, KV4_WHOLE));
-    if (warp < NW - 1) w1 = min(b1, moved(w1, KV4_WHOLE));
-  }
+  int b0 = begin(blockIdx.x), b1 = begin(blockIdx.x + 1), w0, w1;
+  auto own = [&](int& w0, int& w1) {
+    w0 = b0 + int((long long)(b1 - b0) * warp / NW);
+    w1 = b0 + int((long long)(b1 - b0) * (warp + 1) / NW);
+    if (T <= (long long)KV4_WHOLE * a.rows * a.c.nkv) {
+      if (warp > 0) w0 = max(b0, moved(w0, KV4_WHOLE));
+      if (warp < NW - 1) w1 = min(b1, moved(w1, KV4_WHOLE));
+    }
+  };
+  own(w0, w1);
   if (tid == 0) {                                      // (not in registers until the join)
     s_split[0] = b0;
     s_split[1] = b1;
@@ -825,14 +830,37 @@ __global__ void __launch_bounds__(Kv4DecSmem<HD, NT>::NW * 32, 1) k_kv4_attn(con
       }
       if (i < n) kv4_cursor_next<HD>(a, cc);
     }
-    if (!ok)                                           // a copy did not arrive: wait (bounded) for what is in flight
+    if (!ok) {                                         // a copy did not arrive: wait (bounded) for what is in flight
       for (int s = 0; s < NST; ++s) mbar_wait_all(&full[s], ph ^ (s < slot), ERR_TIMEOUT_FULL, KERNEL_ID_KV4_ATTN);
+      pieces = true;
+      if (lane == 0) s_lost = 1;
+    }
   }
   if (!__syncthreads_or(pieces)) return;
   b0 = s_split[0];
   b1 = s_split[1];
   T = s_split[2];
   ctas = s_split[3];
+  if (s_lost) {
+    // Units that warps share still get every warp's piece, a NaN from one that gave up: every CTA takes its tickets, and the
+    // counters come back to zero.
+    own(w0, w1);
+    for (int piece = 0; piece < 2 && w0 < w1; ++piece) {
+      const int x = piece == 0 ? w0 : w1 - 1;
+      int at, nb, *e = meta + 4 * (2 * warp + piece);
+      const int r = locate(x, at, nb), h = (x - at) / nb, us = at + h * nb;
+      if ((us >= w0 && us + nb <= w1) || e[0] >= 0 || (piece == 1 && us <= w0)) continue;      // (whole, there, the first again)
+      float* part = reinterpret_cast<float*>(piece == 0 ? smem + SM::HEADP + warp * SM::PART : ring) + 8 * NT * HD;
+      if (lane < 8 * NT) *reinterpret_cast<float2*>(part + 2 * lane) = make_float2(0.f, __int_as_float(0x7FFFFFFF));
+      __syncwarp();
+      if (lane == 0) {
+        e[0] = r * a.c.nkv + h;
+        e[1] = us;
+        e[2] = us + nb;
+      }
+    }
+    __syncthreads();
+  }
 
   // ---- join the warps' pieces of each unit, in key order: the runs of pieces of one unit, each piece's weight
   int *runs = reinterpret_cast<int*>(smem + SM::RUNS), *list = runs + 4 * NW, *rof = list + 2 * NW;

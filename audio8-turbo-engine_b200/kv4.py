@@ -51,8 +51,8 @@ class KV4Cache:
         L.counters.add(self)
 
     def reset_counters(self):
-        """Drop the workspaces of `attention` (not what the cache holds): after a wait that ran out (`device_error`) their
-        tickets may be partly taken, and later calls would join too early. The package's `clear_error` calls it."""
+        """Drop the workspaces of `attention` (not what the cache holds): their tickets are zero between calls, and later
+        calls join too early where they are not. The package's `clear_error` calls it."""
         self._ws.clear()
 
     @property

@@ -176,8 +176,8 @@ int a8_kv4_attention_workspace(const A8KV4* c, int nq, int rows, int max_len, lo
  * cache row rowmap[r] (NULL: r), kv head h / (nq / nkv), L_r = min(lens[r], max_len). q / out bf16 [rows, stride] (16-byte
  * aligned, strides multiples of 8), nq / nkv from 1 to 16. L_r <= 0 gives zeros. A row whose cache row is out of range
  * gives zeros and records ERR_BOUNDS. scale <= 0: hd^-0.5. out may be q (of the same stride), else it does not overlap
- * it. counters: n_counters ints, zero before the first call (a call leaves them zero; after a recorded timeout, zero them
- * again); ws (16-byte aligned) and counters belong to one call at a time. The order of every sum depends only on the shape,
+ * it. counters: n_counters ints, zero before the first call (a call leaves them zero, one that recorded a timeout too: the
+ * rows that it could not finish are NaN or as they were); ws (16-byte aligned) and counters belong to one call at a time. The order of every sum depends only on the shape,
  * lens, cache rows and max_len of a call, so equal calls give equal bits. Logits, sums and results are fp32; a softmax weight
  * times its value's scale is rounded to bf16 (as a8_attention rounds its weights). Meant for |q| below 2^110 and
  * |scale q.K| below 2^24; a larger one may give a NaN. */
